@@ -1,0 +1,640 @@
+"""The operators of a decoding step over a paged key-value cache, as hand-written HIP kernels.
+
+    q = decode.append_kv(k, v, k_cache, v_cache, block_table, seq_lens, q=q, cos=cos, sin=sin)
+    o = decode.paged_attention(q, k_cache, v_cache, block_table, seq_lens)
+    logits = decode.adjust_logits(logits, tokens=tokens, token_lens=lens, repetition=1.1)
+
+A cache is two arrays `[pages, page size, key heads, head dimension]`, in any order in memory
+(`x.permute(0, 2, 1, 3)` of one that keeps a page's heads together is as good): the elements of
+a head are adjacent, and both caches have the same strides. `block_table[b, i]` is the page of
+sequence b's tokens `i * page size` on, `seq_lens[b]` its length with the new tokens.
+
+Arrays are torch-ROCm tensors, `enceladus.Tensor`s or NumPy arrays (which are copied to the GPU
+and back), on one device; the work goes to its current stream and nothing waits for it. What the
+device alone knows is checked there: a page outside the cache is neither read nor written, a
+length beyond the block table counts as the whole of it, a negative one as none. Nothing is kept
+from one call for the next but compiled kernels, so calls on several streams and captured graphs
+do not meet; a call inside a capture needs one before it, which loads the kernel. There are no
+gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+import sys
+import threading
+
+import numpy as np
+
+from enceladus_amd.runtime import compile as C
+from enceladus_amd.runtime import debug as _trace
+from enceladus_amd.runtime import device as D
+from enceladus_amd.runtime import hip
+from enceladus_amd.runtime import tensor as T
+from enceladus_amd.runtime import timing as _timing
+from enceladus_amd.runtime.probe import check_mfma_layout
+
+__all__ = ["append_kv", "paged_attention", "adjust_logits"]
+
+_SOURCES = hip.INCLUDE_DIR.parent / "kernels"
+_SIZE = {"fp32": 4, "fp16": 2, "bf16": 2, "fp8": 1, "i32": 4}
+_Q = {"fp32": 0, "fp16": 1, "bf16": 2}
+MAX_HEAD_DIM = 256
+MAX_TOKENS = 1 << 30               # of a block table's row: positions are 32-bit
+
+
+# -- kernels -----------------------------------------------------------------------------
+
+_lock = threading.Lock()
+_texts: dict[str, str] = {}
+_functions: dict[tuple, ctypes.c_void_p] = {}
+_modules: dict[tuple, ctypes.c_void_p] = {}
+
+
+def _source(file: str, macros: tuple) -> str:
+    text = _texts.get(file)
+    if text is None:
+        text = _texts[file] = (_SOURCES / file).read_text()
+    return "".join(f"#define {k} {v}\n" for k, v in macros) + text
+
+
+def _code(file: str, macros: tuple) -> bytes:
+    return C.compile_code(_source(file, macros), file.removesuffix(".hip"))
+
+
+def _function(file: str, macros: tuple, name: str, device: int):
+    """The kernel `name` of a compiled source on `device`, which is the current one."""
+    f = _functions.get((file, macros, name, device))
+    if f is not None:
+        return f
+    if file == "paged_attention.hip":
+        check_mfma_layout()
+    with _lock:
+        mod = _modules.get((file, macros, device))
+        if mod is None:
+            code = _code(file, macros)
+            mod = ctypes.c_void_p()
+            hip.call("ek_module_load", ctypes.create_string_buffer(code, len(code)), len(code),
+                     ctypes.byref(mod))
+            _modules[file, macros, device] = mod
+        f = ctypes.c_void_p()
+        hip.call("ek_module_function", mod, name.encode(), ctypes.byref(f))
+        _functions[file, macros, name, device] = f
+    return f
+
+
+def _launch(fn, name: str, grid, block: int, kernarg: bytes, stream: int) -> None:
+    grid = (*grid, 1)
+    timer = _timing.current()
+    if timer is not None:
+        timer.launch(stream, fn, grid, block, kernarg, len(kernarg))
+        return
+    t0 = _trace.before_launch(stream) if _trace._active is not None else None
+    hip.call("ek_launch", stream or None, fn, *grid, block, 1, 1, 0, kernarg, len(kernarg))
+    if t0 is not None:
+        _trace.after_launch(t0, stream, name, grid, block, 0)
+
+
+# -- arguments ---------------------------------------------------------------------------
+
+_torch_kinds: dict = {}
+
+
+def _torch():
+    torch = sys.modules.get("torch")
+    if torch is not None and not _torch_kinds:
+        _torch_kinds.update({torch.float32: "fp32", torch.float16: "fp16",
+                             torch.bfloat16: "bf16", torch.int32: "i32"})
+        if hasattr(torch, "float8_e4m3fn"):
+            _torch_kinds[torch.float8_e4m3fn] = "fp8"
+    return torch
+
+
+class _Array:
+    """An array argument: its element kind, shape, strides in elements and device (-1: the
+    host, or the framework's own)."""
+
+    __slots__ = ("obj", "kind", "shape", "strides", "device", "size")
+
+    def __init__(self, name: str, obj):
+        torch = _torch()
+        self.obj = obj
+        if torch is not None and isinstance(obj, torch.Tensor):
+            self.kind = _torch_kinds.get(obj.dtype, str(obj.dtype))
+            self.shape, self.strides = tuple(obj.shape), obj.stride()
+            self.device = obj.device.index if obj.device.type == "cuda" else -1
+            if obj.device.type not in ("cuda", "cpu") or obj.layout is not torch.strided:
+                raise ValueError(f"`{name}` is not a dense tensor on a GPU or the host")
+            if self.device < 0 and self.kind == "fp8":
+                raise ValueError(f"`{name}` holds float8 values on the host: move it to the GPU")
+        elif T.is_array_like(obj):
+            self.kind = T.elem_dtype(obj).name
+            self.shape, self.strides = tuple(obj.shape), T.element_strides(obj)
+            self.device = -1
+            if any(s < 0 for s in self.strides):
+                raise ValueError(f"`{name}` has negative strides")
+        else:
+            raise TypeError(f"`{name}` must be an array, got {type(obj).__name__}")
+        self.size = _SIZE.get(self.kind, 0)
+
+    def span(self, first: int = 0) -> int:
+        """Bytes from the first element to the last one's end (of dimensions `first` on)."""
+        if 0 in self.shape:
+            return 0
+        return self.size * (1 + sum((n - 1) * s for n, s in
+                                    zip(self.shape[first:], self.strides[first:])))
+
+    def address(self) -> int:
+        if isinstance(self.obj, T.Tensor):
+            return self.obj.ptr
+        if isinstance(self.obj, np.ndarray):
+            return self.obj.__array_interface__["data"][0]
+        return self.obj.data_ptr()
+
+
+def _need(ok: bool, text: str) -> None:
+    if not ok:
+        raise ValueError(text)
+
+
+def _array(name: str, obj, kinds, ndim: int, shape=None, dense: bool = True) -> _Array:
+    """`obj` as an array of one of `kinds` and of `ndim` dimensions (`shape`: its extents,
+    None where any will do), with adjacent elements in the last one when `dense`."""
+    a = _Array(name, obj)
+    if a.kind not in kinds:
+        raise TypeError(f"`{name}` must hold {' or '.join(kinds)}, got {a.kind}")
+    _need(len(a.shape) == ndim, f"`{name}` must have {ndim} dimensions, got shape {a.shape}")
+    if shape is not None:
+        _need(all(w is None or w == n for w, n in zip(shape, a.shape)),
+              f"`{name}` must have shape "
+              f"({', '.join('any' if w is None else str(w) for w in shape)}), got {a.shape}")
+    if dense and a.shape[-1] > 1:
+        _need(a.strides[-1] == 1, f"the last dimension of `{name}` must be contiguous "
+                                  f"(strides {tuple(a.strides)})")
+    return a
+
+
+def _written(name: str, a: _Array) -> None:
+    """Refuses an array whose elements share memory, or that may not be written."""
+    _need(all(s != 0 or n <= 1 for n, s in zip(a.shape, a.strides)),
+          f"`{name}` is written: it can't be an expanded view (strides {tuple(a.strides)})")
+    if isinstance(a.obj, np.ndarray):
+        _need(a.obj.flags.writeable, f"`{name}` is a read-only NumPy array")
+
+
+def _apart(name: str, out: _Array, other: str, a: _Array, same_ok: bool = True) -> None:
+    """Refuses an output that overlaps an input, unless it is the input itself."""
+    p, q = out.address(), a.address()
+    if same_ok and p == q and out.shape == a.shape and tuple(out.strides) == tuple(a.strides) \
+            and out.size == a.size:
+        return
+    if p + out.span() <= q or q + a.span() <= p:
+        return
+    # rows side by side in one wider array
+    step = out.strides[0] * out.size
+    if step > 0 and step == a.strides[0] * a.size:
+        at = (p - q) % step
+        if a.span(1) <= at and at + out.span(1) <= step:
+            return
+    raise ValueError(f"`{name}` overlaps `{other}`")
+
+
+def _device_of(arrays) -> int:
+    """The GPU that the arrays are on: torch's, or -1 where none says one. Refuses two."""
+    found = {a.device for _, a in arrays if a is not None and a.device >= 0}
+    _need(len(found) < 2, "the arrays are on different GPUs: " + ", ".join(
+        f"`{n}` on {a.device}" for n, a in arrays if a is not None and a.device >= 0))
+    return found.pop() if found else -1
+
+
+class _On:
+    """The device of a call as the current one, and its current stream."""
+
+    def __init__(self, device: int):
+        torch = _torch()
+        self.guard, self.device, self.stream = None, 0, 0
+        if torch is not None and torch.cuda.is_available():
+            here = torch.cuda.current_device()
+            self.device = here if device < 0 else device
+            if self.device != here:
+                self.guard = torch.cuda.device(self.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        self.stream = D.current_stream()
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _pointers(arrays, writes):
+    """(device addresses, bindings) of the arrays in order, 0 for those that are None."""
+    given = [a.obj for _, a in arrays if a is not None]
+    at = {i: k for k, i in enumerate(i for i, (_, a) in enumerate(arrays) if a is not None)}
+    got, bindings = T.bind_arrays(given, {at[i] for i in writes if i in at})
+    return [got[at[i]] if i in at else 0 for i in range(len(arrays))], bindings
+
+
+def _workspace(like: _Array, nbytes: int):
+    """Device memory for one call, on the call's device, and its address."""
+    torch = _torch()
+    if torch is not None and like.device >= 0:
+        t = torch.empty(nbytes, dtype=torch.uint8, device=like.obj.device)
+        return t, t.data_ptr()
+    t = T.empty((nbytes,), "uint8")
+    return t, t.ptr
+
+
+def _caches(k_cache, v_cache, heads, dim, kinds):
+    kc = _array("k_cache", k_cache, kinds, 4, (None, None, heads, dim))
+    vc = _array("v_cache", v_cache, (kc.kind,), 4, kc.shape)
+    _need(tuple(kc.strides) == tuple(vc.strides), "`k_cache` and `v_cache` must have the same "
+          f"strides, got {tuple(kc.strides)} and {tuple(vc.strides)}")
+    _need(kc.shape[1] > 0, "a page of `k_cache` must hold at least one token")
+    return kc, vc
+
+
+def _sequences(block_table, seq_lens, batch):
+    bt = _array("block_table", block_table, ("i32",), 2, (batch, None))
+    sl = _array("seq_lens", seq_lens, ("i32",), 1, (batch,), dense=False)
+    return bt, sl
+
+
+def _capacity(bt: _Array, kc: _Array) -> int:
+    n = bt.shape[1] * kc.shape[1]
+    _need(n <= MAX_TOKENS, f"`block_table` covers {n} tokens of a sequence: at most "
+                           f"{MAX_TOKENS} are supported")
+    return n
+
+
+def _page_division(page: int) -> tuple[int, int]:
+    """(multiplier, shift) with n // page == (n * multiplier >> 32) >> shift for n < 2^31 and
+    page > 1: with 2^(b - 1) < page <= 2^b the multiplier, 2^(31 + b) / page rounded up, is off
+    by less than one in 2^31."""
+    bits = (page - 1).bit_length()
+    return ((1 << (31 + bits)) // page + 1) & 0xFFFFFFFF, max(bits - 1, 0)
+
+
+def _head_dim(dim: int, cache: str) -> None:
+    _need(0 < dim <= MAX_HEAD_DIM and dim % (16 if cache == "fp8" else 8) == 0,
+          f"the head dimension must be a multiple of {16 if cache == 'fp8' else 8} up to "
+          f"{MAX_HEAD_DIM}, got {dim}")
+
+
+def _scale_arg(name: str, x) -> float:
+    x = float(x)
+    _need(math.isfinite(x) and x > 0, f"`{name}` must be a positive number, got {x}")
+    return x
+
+
+# -- appending to the cache ----------------------------------------------------------------
+
+_APPEND = struct.Struct("<11Q16q11i2f4x")
+
+
+def _vector(size: int, rotary: int, dim: int, interleaved: bool) -> int:
+    """Elements of an access: up to 16 bytes, dividing each part of a head."""
+    v = 16 // size
+    parts = (rotary, dim) if interleaved else (rotary // 2, dim - rotary)
+    while any(p % v for p in parts):
+        v //= 2
+    return v
+
+
+def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, q=None,
+              q_out=None, cos=None, sin=None, interleaved: bool = False, k_scale: float = 1.0,
+              v_scale: float = 1.0):
+    """Writes new keys and values into a paged cache, the keys rotated by their positions,
+    and returns the queries rotated likewise.
+
+    Sequence b's new tokens are the rows `cu_tokens[b]` to `cu_tokens[b + 1]` (without
+    `cu_tokens`, row b alone); they are its last ones, so that the i-th of n is at position
+    `seq_lens[b] - n + i`. Rows of no sequence (padding behind the last, or before the first),
+    and rows whose position is negative, not covered by the block table or not in `cos`, or
+    whose page is not in the cache, are skipped: neither cache nor `q_out` is written for them.
+    Two rows must not share a slot of the cache.
+
+    With `cos` and `sin`, the first R elements of each key and query head are rotated in pairs,
+    (j, j + R / 2), or (2 j, 2 j + 1) when `interleaved`: (x, y) becomes
+    (x cos - y sin, y cos + x sin).
+
+    Args:
+        k, v: `[tokens, key heads, dim]`, float32, float16 or bfloat16; `dim` a multiple of 8
+            up to 256 (of 16 with a float8 cache).
+        k_cache, v_cache: `[pages, page size, key heads, dim]` of the type of `k`, or
+            float8_e4m3fn; written in place.
+        block_table: int32 `[batch, pages of a sequence]`.
+        seq_lens: int32 `[batch]`, counting the new tokens.
+        cu_tokens: int32 `[batch + 1]`, not descending.
+        q: queries `[tokens, heads, dim]` of the type of `k`, to be rotated beside the keys.
+        q_out: where the rotated queries go (`q` itself will do); new without it.
+        cos, sin: float32 `[positions, R / 2]`.
+        k_scale, v_scale: cached values are divided by these (float8: then saturated to +-448).
+
+    Returns:
+        The rotated queries, or None without `q`.
+    """
+    kinds = ("fp32", "fp16", "bf16")
+    ka = _array("k", k, kinds, 3)
+    tokens, kv_heads, dim = ka.shape
+    va = _array("v", v, (ka.kind,), 3, ka.shape)
+    kc, vc = _caches(k_cache, v_cache, kv_heads, dim, (ka.kind, "fp8"))
+    _head_dim(dim, kc.kind)
+    cu = None
+    if cu_tokens is not None:
+        cu = _array("cu_tokens", cu_tokens, ("i32",), 1, dense=False)
+        _need(cu.shape[0] > 0, "`cu_tokens` must have one entry more than there are sequences")
+        batch = cu.shape[0] - 1
+    else:
+        batch = tokens
+    bt, sl = _sequences(block_table, seq_lens, batch)
+    capacity = _capacity(bt, kc)
+    qa = qo = None
+    heads = 0
+    if q is not None:
+        qa = _array("q", q, (ka.kind,), 3, (tokens, None, dim))
+        heads = qa.shape[1]
+        if q_out is None:
+            q_out = T.new_empty(q)
+        qo = _array("q_out", q_out, (ka.kind,), 3, qa.shape)
+        _written("q_out", qo)
+        for n, a in (("q", qa), ("k", ka), ("v", va)):
+            _apart("q_out", qo, n, a, same_ok=n == "q")
+    else:
+        _need(q_out is None, "`q_out` is given without `q`")
+    _written("k_cache", kc)
+    _written("v_cache", vc)
+    _need((cos is None) == (sin is None), "`cos` and `sin` go together")
+    ca = sa = None
+    rotary = 0
+    if cos is not None:
+        ca = _array("cos", cos, ("fp32",), 2)
+        sa = _array("sin", sin, ("fp32",), 2, ca.shape)
+        rotary = 2 * ca.shape[1]
+        _need(0 < rotary <= dim, f"`cos` rotates {rotary} elements of heads of {dim}")
+    k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
+    if tokens == 0 or batch == 0 or kv_heads + heads == 0 or capacity == 0 or kc.shape[0] == 0:
+        return q_out
+    arrays = [("q", qa), ("k", ka), ("v", va), ("q_out", qo), ("k_cache", kc), ("v_cache", vc),
+              ("block_table", bt), ("seq_lens", sl), ("cu_tokens", cu), ("cos", ca),
+              ("sin", sa)]
+    interleaved = bool(interleaved) and rotary > 0
+    vec = _vector(ka.size, rotary, dim, interleaved)
+    macros = (("EK_Q", _Q[ka.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_V", vec),
+              ("EK_PAIRS", int(interleaved)))
+    # One wave per token, unless that leaves CUs without one: then as many as it has rows for.
+    places = dim // vec if interleaved else (dim - rotary // 2) // vec
+    rows = heads + 2 * kv_heads
+    most = -(-rows // max(1, 64 // places))
+    parts = max(1, min(most, 4096 // tokens))
+    with _On(_device_of(arrays)) as on:
+        ptrs, bindings = _pointers(arrays, {3, 4, 5})
+        zero = (0, 0, 0)
+        qs, os = (a.strides if a is not None else zero for a in (qa, qo))
+        kernarg = _APPEND.pack(
+            *ptrs, qs[0], qs[1], ka.strides[0], ka.strides[1], va.strides[0], va.strides[1],
+            os[0], os[1], *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0],
+            cu.strides[0] if cu else 0, ca.strides[0] if ca else 0, sa.strides[0] if sa else 0,
+            tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
+            ca.shape[0] if ca else 0, parts, 1.0 / k_scale, 1.0 / v_scale)
+        fn = _function("append_kv.hip", macros, "ek_append_kv", on.device)
+        _launch(fn, "ek_append_kv", (-(-tokens * parts // 4), 1), 256, kernarg, on.stream)
+        T.complete_bindings(bindings)
+    return q_out
+
+
+# -- attention over the cache ----------------------------------------------------------------
+
+_ATTEND = struct.Struct("<8Q9q8iI3i3f4x")
+_UNIT = 64                          # tokens: what a sequence is split in multiples of
+_MIN_UNITS = 2
+_WORKGROUPS = 4                     # chunks of all sequences and key heads, per CU
+
+
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float | None = None,
+                    window: int = 0, softcap: float = 0.0, k_scale: float = 1.0,
+                    v_scale: float = 1.0, out=None, return_lse: bool = False):
+    """Attention of one token per sequence over a paged cache (which holds its own key and
+    value already).
+
+    For query head h of sequence b: s_j = `scale` * q . k_j over the sequence's tokens, of
+    which only the last `window` count when that is above 0, made `softcap` * tanh(s_j /
+    `softcap`) when that is above 0; the result is the sum of softmax(s)_j v_j. `heads` is a
+    multiple of the key heads: head h reads key head h // (heads / key heads). A sequence
+    without tokens gives zeros. Tokens on a page outside the cache count as absent. Cache
+    memory that no sequence's length reaches may hold anything, NaN included.
+
+    Args:
+        q: `[batch, heads, dim]`, float32, float16 or bfloat16; `dim` a multiple of 8 up to
+            256 (of 16 with a float8 cache).
+        k_cache, v_cache: `[pages, page size, key heads, dim]` of the type of `q`, or
+            float8_e4m3fn (not with float32).
+        block_table: int32 `[batch, pages of a sequence]`.
+        seq_lens: int32 `[batch]`.
+        scale: of the scores; 1 / sqrt(dim) without it.
+        k_scale, v_scale: what cached values are multiplied by.
+        out: where the result goes (`q` itself will do); new without it.
+        return_lse: also return the log of each head's sum of exp(s_j), float32
+            `[batch, heads]` (-inf without tokens), by which results over parts of a sequence
+            are joined.
+
+    Returns:
+        The result, `[batch, heads, dim]` of the type of `q`; `(result, lse)` when
+        `return_lse`.
+    """
+    qa = _array("q", q, ("fp32", "fp16", "bf16"), 3)
+    batch, heads, dim = qa.shape
+    kc, vc = _caches(k_cache, v_cache, None, dim,
+                     (qa.kind,) if qa.kind == "fp32" else (qa.kind, "fp8"))
+    kv_heads = kc.shape[2]
+    _head_dim(dim, kc.kind)
+    _need(kv_heads > 0 and heads % kv_heads == 0,
+          f"{heads} query heads are not a multiple of {kv_heads} key heads")
+    _need(heads <= 65535, f"at most 65535 query heads are supported, got {heads}")
+    bt, sl = _sequences(block_table, seq_lens, batch)
+    capacity = _capacity(bt, kc)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    _need(math.isfinite(scale), f"`scale` must be finite, got {scale}")
+    softcap, window = float(softcap), int(window)
+    _need(math.isfinite(softcap) and softcap >= 0, f"`softcap` must be at least 0, got {softcap}")
+    _need(window >= 0, f"`window` must be at least 0, got {window}")
+    k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
+    if out is None:
+        out = T.new_empty(q)
+    oa = _array("out", out, (qa.kind,), 3, qa.shape)
+    _written("out", oa)
+    _apart("out", oa, "q", qa)
+    _apart("out", oa, "k_cache", kc, same_ok=False)
+    _apart("out", oa, "v_cache", vc, same_ok=False)
+    lse = T.new_empty(q, (batch, heads), np.float32) if return_lse else None
+    if batch and heads:
+        la = _Array("lse", lse) if return_lse else None
+        arrays = [("q", qa), ("k_cache", kc), ("v_cache", vc), ("block_table", bt),
+                  ("seq_lens", sl), ("out", oa), ("lse", la)]
+        if kc.shape[0] == 0:
+            capacity = 0
+        window = min(window, MAX_TOKENS)
+        most = -(-(min(window, capacity) if window else capacity) // _UNIT)
+        group = heads // kv_heads
+        y = kv_heads * (-(-group // 16))
+        items = max(1, min(_WORKGROUPS * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
+        single = most <= _MIN_UNITS
+        page = kc.shape[1]
+        width = 64 if dim <= 64 else 128 if dim <= 128 else 256
+        macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
+                  ("EK_PAD", int(dim != width)))
+        log2e = 1.4426950408889634
+        with _On(_device_of(arrays)) as on:
+            ptrs, bindings = _pointers(arrays, {5, 6})
+            part = keep = None
+            if not single:
+                keep, part = _workspace(qa, (items + batch) * heads * (dim + 2) * 4)
+            kernarg = _ATTEND.pack(
+                *ptrs, part or 0, qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
+                *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch,
+                heads, group, dim, page, kc.shape[0], capacity, window,
+                *_page_division(page), items, _MIN_UNITS, scale * k_scale * log2e, softcap * log2e, v_scale)
+            fn = _function("paged_attention.hip", macros, "ek_paged_attention", on.device)
+            _launch(fn, "ek_paged_attention", (items + batch, y), 256, kernarg, on.stream)
+            if not single:
+                fn = _function("paged_attention.hip", macros, "ek_paged_attention_join",
+                               on.device)
+                _launch(fn, "ek_paged_attention_join", (batch, heads), 256, kernarg, on.stream)
+            T.complete_bindings(bindings)
+            del keep
+    return (out, lse) if return_lse else out
+
+
+# -- logits ----------------------------------------------------------------------------------
+
+_LOGITS = struct.Struct("<12Q12q3i4f4x")
+
+
+def _per_row(name: str, x, rows: int, default: float):
+    """(array or None, number) of a per-row setting given as a number or an array."""
+    if x is None:
+        return None, default
+    if T.is_array_like(x):
+        return _array(name, x, ("fp32",), 1, (rows,), dense=False), default
+    return None, float(x)
+
+
+def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
+                  repetition=None, frequency=None, presence=None, bias_ids=None, bias=None,
+                  allowed=None, temperature=None, out=None):
+    """Penalties for repeated tokens, biases, a temperature and a mask on rows of logits, in
+    this order, computed in 32 bits and rounded once:
+
+    1. tokens that occur in the row's history: x / `repetition` where x > 0, else
+       x * `repetition`;
+    2. with c the number of times a token occurs in the generated part of the history:
+       x - `frequency` * c, and - `presence` where c > 0;
+    3. plus the sum of the row's biases for that token;
+    4. divided by `temperature` where that is above 0;
+    5. -inf where the token is not allowed, whatever the logit was. A row that allows none is
+       -inf throughout.
+
+    Args:
+        logits: `[rows, vocabulary]`, float32, float16 or bfloat16.
+        tokens: the history, int32 `[rows, length]`; ids outside the vocabulary are ignored.
+        token_lens: how much of each row of `tokens` counts, int32 `[rows]`; all without it.
+        prompt_lens: how much of that is the prompt, int32 `[rows]`; none without it.
+        repetition, frequency, presence, temperature: a number, or float32 `[rows]`.
+        bias_ids, bias: int32 and float32 `[rows, entries]`; ids outside the vocabulary are
+            ignored, entries with the same id add up in their order.
+        allowed: int32 `[rows, words]`, 32 tokens to a word: token t is bit t % 32 of word
+            t // 32. One mask for all rows is an expanded array.
+        out: where the result goes (`logits` itself will do); new without it.
+
+    Returns:
+        The adjusted logits, of the type of `logits`.
+    """
+    la = _array("logits", logits, ("fp32", "fp16", "bf16"), 2)
+    rows, vocab = la.shape
+    ta = tl = pl = None
+    if tokens is not None:
+        ta = _array("tokens", tokens, ("i32",), 2, (rows, None))
+        if token_lens is not None:
+            tl = _array("token_lens", token_lens, ("i32",), 1, (rows,), dense=False)
+        if prompt_lens is not None:
+            pl = _array("prompt_lens", prompt_lens, ("i32",), 1, (rows,), dense=False)
+    else:
+        _need(all(x is None for x in (token_lens, prompt_lens, repetition, frequency,
+                                      presence)),
+              "lengths and penalties need the history (`tokens`)")
+    _need((bias_ids is None) == (bias is None), "`bias_ids` and `bias` go together")
+    ia = ba = None
+    if bias is not None:
+        ia = _array("bias_ids", bias_ids, ("i32",), 2, (rows, None))
+        ba = _array("bias", bias, ("fp32",), 2, ia.shape)
+    aa = None
+    if allowed is not None:
+        aa = _array("allowed", allowed, ("i32",), 2, (rows, None))
+        _need(aa.shape[1] * 32 >= vocab, f"`allowed` has {aa.shape[1]} words: {vocab} tokens "
+                                         f"need {-(-vocab // 32)}")
+    rep_a, rep = _per_row("repetition", repetition, rows, 1.0)
+    freq_a, freq = _per_row("frequency", frequency, rows, 0.0)
+    pres_a, pres = _per_row("presence", presence, rows, 0.0)
+    temp_a, temp = _per_row("temperature", temperature, rows, 0.0)
+    _need(rep > 0, f"`repetition` must be above 0, got {rep}")
+    if out is None:
+        out = T.new_empty(logits)
+    oa = _array("out", out, (la.kind,), 2, la.shape)
+    _written("out", oa)
+    _apart("out", oa, "logits", la)
+    arrays = [("logits", la), ("out", oa), ("tokens", ta), ("token_lens", tl),
+              ("prompt_lens", pl), ("repetition", rep_a), ("frequency", freq_a),
+              ("presence", pres_a), ("temperature", temp_a), ("bias_ids", ia), ("bias", ba),
+              ("allowed", aa)]
+    for n, a in arrays[2:]:
+        if a is not None:
+            _apart("out", oa, n, a, same_ok=False)
+    if rows == 0 or vocab == 0:
+        return out
+    _need(vocab < 1 << 30 and rows * vocab < 1 << 41,
+          f"logits of shape {la.shape} are too large for one call")
+    biases = ia.shape[1] if ia else 0
+    n, threads = (2048, 128) if rows * vocab < 1 << 21 else (8192, 256)
+    if la.kind == "fp32" and n == 2048:
+        threads = 256
+    macros = (("EK_Q", _Q[la.kind]), ("EK_N", n), ("EK_THREADS", threads),
+              ("EK_BIAS", int(biases > 0)))
+
+    def step(a):
+        return a.strides[0] if a is not None else 0
+
+    with _On(_device_of(arrays)) as on:
+        ptrs, bindings = _pointers(arrays, {1})
+        if ta is not None and ta.shape[1] == 0:
+            ptrs[2] = 0
+        kernarg = _LOGITS.pack(*ptrs, step(la), step(oa), step(ta), step(ia), step(ba), step(aa),
+                               step(tl), step(pl), step(rep_a), step(freq_a), step(pres_a),
+                               step(temp_a), vocab, ta.shape[1] if ta else 0, biases, rep, freq,
+                               pres, temp)
+        fn = _function("adjust_logits.hip", macros, "ek_adjust_logits", on.device)
+        _launch(fn, "ek_adjust_logits", (-(-vocab // n) * rows, 1), threads, kernarg, on.stream)
+        T.complete_bindings(bindings)
+    return out
+
+
+def specializations():
+    """(source, macros) of the kernels that are worth compiling ahead."""
+    for q, fp8 in ((2, 0), (1, 0), (0, 0), (2, 1), (1, 1)):
+        for width in (64, 128, 256):
+            for pad in (0, 1):
+                yield "paged_attention.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_DP", width),
+                                              ("EK_PAD", pad))
+        for pairs in (0, 1):
+            yield "append_kv.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_V", 8 if q else 4),
+                                    ("EK_PAIRS", pairs))
+    for q in (0, 1, 2):
+        for n, threads in ((2048, 128 if q else 256), (8192, 256)):
+            for bias in (0, 1):
+                yield "adjust_logits.hip", (("EK_Q", q), ("EK_N", n), ("EK_THREADS", threads),
+                                            ("EK_BIAS", bias))

@@ -4,7 +4,8 @@ Compiling here (no GPU needed: hiprtc cross-compiles gfx950) fills the code-obje
 GPU runs start without compile latency; it is also the compile-only coverage check. The
 list is every variant of the benchmark's workload table (`examples/workloads.py`, with
 torch "meta" tensors standing in for the full-size buffers: same shapes, dtypes and
-argument facts, no memory) plus the example wrappers' own default launches.
+argument facts, no memory), the example wrappers' own default launches, and the hand-written
+kernels of `enceladus.decode`.
 """
 
 from __future__ import annotations
@@ -112,8 +113,19 @@ def compile_all(verbose: bool = False) -> int:
         kern, types, facts, consts, nw, dw = job
         return kern._compile_for(types, facts, consts, nw, dw).ck
 
+    from enceladus_amd import decode
+    hand = list(decode.specializations())
+
+    def one_hand(spec):
+        decode._code(*spec)
+        return spec
+
     with ThreadPoolExecutor(max_workers=8) as ex:
         for ck in ex.map(one, jobs):
             if verbose:
                 print(f"  compiled {ck.name} (lds {ck.lds_bytes} B)", flush=True)
-    return len(jobs)
+        for file, macros in ex.map(one_hand, hand):
+            if verbose:
+                print(f"  compiled {file} ({', '.join(f'{k}={v}' for k, v in macros)})",
+                      flush=True)
+    return len(jobs) + len(hand)

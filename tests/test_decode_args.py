@@ -1,0 +1,210 @@
+"""`enceladus.decode`: what its operators refuse, before anything is launched (CPU)."""
+
+import numpy as np
+import pytest
+import torch
+
+import enceladus
+from enceladus import decode
+
+
+def _attend(**kw):
+    d = dict(q=torch.zeros(3, 8, 64), k_cache=torch.zeros(10, 16, 2, 64),
+             v_cache=torch.zeros(10, 16, 2, 64),
+             block_table=torch.zeros(3, 4, dtype=torch.int32),
+             seq_lens=torch.ones(3, dtype=torch.int32))
+    d.update(kw)
+    return d.pop("q"), d.pop("k_cache"), d.pop("v_cache"), d.pop("block_table"), \
+        d.pop("seq_lens"), d
+
+
+def _append(**kw):
+    d = dict(k=torch.zeros(3, 2, 64), v=torch.zeros(3, 2, 64),
+             k_cache=torch.zeros(10, 16, 2, 64), v_cache=torch.zeros(10, 16, 2, 64),
+             block_table=torch.zeros(3, 4, dtype=torch.int32),
+             seq_lens=torch.ones(3, dtype=torch.int32))
+    d.update(kw)
+    return tuple(d.pop(n) for n in ("k", "v", "k_cache", "v_cache", "block_table",
+                                    "seq_lens")) + (d,)
+
+
+def _f8(*shape):
+    return torch.zeros(*shape).to(torch.float8_e4m3fn)
+
+
+ATTEND = [
+    (dict(q=torch.zeros(3, 8, 64, dtype=torch.float64)), TypeError, "`q` must hold"),
+    (dict(q=[1.0]), TypeError, "must be an array"),
+    (dict(q=torch.zeros(3, 512)), ValueError, "3 dimensions"),
+    (dict(q=torch.zeros(3, 64, 8).transpose(1, 2)), ValueError, "contiguous"),
+    (dict(q=torch.zeros(3, 7, 64)), ValueError, "not a multiple"),
+    (dict(q=torch.zeros(3, 8, 64).half()), TypeError, "`k_cache` must hold"),
+    (dict(k_cache=torch.zeros(10, 16, 2, 32)), ValueError, "`k_cache` must have shape"),
+    (dict(v_cache=torch.zeros(10, 8, 2, 64)), ValueError, "`v_cache` must have shape"),
+    (dict(v_cache=torch.zeros(10, 2, 16, 64).transpose(1, 2)), ValueError, "same strides"),
+    (dict(v_cache=torch.zeros(10, 16, 2, 64).half()), TypeError, "`v_cache` must hold"),
+    (dict(k_cache=torch.zeros(10, 0, 2, 64), v_cache=torch.zeros(10, 0, 2, 64)), ValueError,
+     "at least one token"),
+    (dict(k_cache=torch.zeros(10, 16, 0, 64), v_cache=torch.zeros(10, 16, 0, 64)), ValueError,
+     "key heads"),
+    (dict(k_cache=_f8(10, 16, 2, 64)), ValueError, "host"),
+    (dict(block_table=torch.zeros(3, 4, dtype=torch.int64)), TypeError, "`block_table`"),
+    (dict(block_table=torch.zeros(2, 4, dtype=torch.int32)), ValueError, "`block_table`"),
+    (dict(block_table=torch.zeros(3, 1 << 26, dtype=torch.int32)[:, ::1],
+          k_cache=torch.zeros(1, 32, 2, 64), v_cache=torch.zeros(1, 32, 2, 64)), ValueError,
+     "at most"),
+    (dict(seq_lens=torch.ones(4, dtype=torch.int32)), ValueError, "`seq_lens`"),
+    (dict(seq_lens=np.ones(3, np.float32)), TypeError, "`seq_lens`"),
+    (dict(seq_lens=np.ones(3, np.int32)[::-1]), ValueError, "negative strides"),
+    (dict(window=-1), ValueError, "window"),
+    (dict(softcap=-1.0), ValueError, "softcap"),
+    (dict(softcap=float("nan")), ValueError, "softcap"),
+    (dict(scale=float("inf")), ValueError, "scale"),
+    (dict(k_scale=0.0), ValueError, "k_scale"),
+    (dict(v_scale=float("nan")), ValueError, "v_scale"),
+    (dict(out=torch.zeros(3, 8, 32)), ValueError, "`out`"),
+    (dict(out=torch.zeros(3, 8, 64).half()), TypeError, "`out`"),
+    (dict(out=torch.zeros(3, 1, 64).expand(3, 8, 64)), ValueError, "expanded"),
+    (dict(q=np.zeros((3, 8, 12), np.float32), k_cache=np.zeros((4, 4, 2, 12), np.float32),
+          v_cache=np.zeros((4, 4, 2, 12), np.float32)), ValueError, "head dimension"),
+    (dict(q=np.zeros((3, 8, 264), np.float32), k_cache=np.zeros((4, 4, 2, 264), np.float32),
+          v_cache=np.zeros((4, 4, 2, 264), np.float32)), ValueError, "head dimension"),
+]
+
+
+@pytest.mark.parametrize("change,error,text", ATTEND)
+def test_paged_attention_refuses(change, error, text):
+    *args, kw = _attend(**change)
+    with pytest.raises(error, match=text):
+        decode.paged_attention(*args, **kw)
+
+
+def test_paged_attention_refuses_overlap():
+    buf = torch.zeros(4 * 8 * 64)
+    q, out = buf[:3 * 512].view(3, 8, 64), buf[512:].view(3, 8, 64)
+    *args, _ = _attend(q=q)
+    with pytest.raises(ValueError, match="`out` overlaps `q`"):
+        decode.paged_attention(*args, out=out)
+    *args, kw = _attend()
+    with pytest.raises(ValueError, match="overlaps `v_cache`"):
+        decode.paged_attention(*args, out=args[2].view(-1)[:1536].view(3, 8, 64))
+
+
+APPEND = [
+    (dict(k=torch.zeros(3, 2, 64, dtype=torch.int32)), TypeError, "`k` must hold"),
+    (dict(v=torch.zeros(3, 2, 32)), ValueError, "`v` must have shape"),
+    (dict(k_cache=torch.zeros(10, 16, 3, 64)), ValueError, "`k_cache`"),
+    (dict(k_cache=torch.zeros(10, 16, 2, 64).half()), TypeError, "`k_cache`"),
+    (dict(k_cache=torch.zeros(1, 16, 2, 64).expand(10, 16, 2, 64),
+          v_cache=torch.zeros(1, 16, 2, 64).expand(10, 16, 2, 64)), ValueError, "expanded"),
+    (dict(seq_lens=torch.ones(2, dtype=torch.int32)), ValueError, "seq_lens"),
+    (dict(cu_tokens=torch.zeros(3, dtype=torch.int32)), ValueError, "block_table"),
+    (dict(cu_tokens=torch.zeros(4)), TypeError, "cu_tokens"),
+    (dict(cu_tokens=torch.zeros(0, dtype=torch.int32)), ValueError, "cu_tokens"),
+    (dict(cos=torch.zeros(8, 32)), ValueError, "go together"),
+    (dict(cos=torch.zeros(8, 32), sin=torch.zeros(8, 16)), ValueError, "`sin`"),
+    (dict(cos=torch.zeros(8, 33), sin=torch.zeros(8, 33)), ValueError, "rotates 66"),
+    (dict(cos=torch.zeros(8, 0), sin=torch.zeros(8, 0)), ValueError, "rotates 0"),
+    (dict(cos=torch.zeros(8, 32).half(), sin=torch.zeros(8, 32).half()), TypeError, "`cos`"),
+    (dict(q=torch.zeros(2, 8, 64)), ValueError, "`q`"),
+    (dict(q=torch.zeros(3, 8, 64).half()), TypeError, "`q`"),
+    (dict(q_out=torch.zeros(3, 8, 64)), ValueError, "without `q`"),
+    (dict(q=torch.zeros(3, 8, 64), q_out=torch.zeros(3, 4, 64)), ValueError, "`q_out`"),
+    (dict(k_scale=-1.0), ValueError, "k_scale"),
+]
+
+
+@pytest.mark.parametrize("change,error,text", APPEND)
+def test_append_kv_refuses(change, error, text):
+    *args, kw = _append(**change)
+    with pytest.raises(error, match=text):
+        decode.append_kv(*args, **kw)
+
+
+def test_overlap_of_rows_side_by_side():
+    wide = torch.zeros(3, 100)
+    arr = {n: decode._Array(n, x) for n, x in (("a", wide[:, :40]), ("b", wide[:, 40:100]),
+                                               ("c", wide[:, 39:60]), ("d", wide[1:, :40]),
+                                               ("e", wide.view(-1)[95:215].view(3, 40)))}
+    for x, y in ("ab", "ba", "db", "bd"):
+        decode._apart(x, arr[x], y, arr[y])
+    for x, y in ("ac", "ca", "bc", "cb", "ad", "da", "be", "eb", "ae"):
+        with pytest.raises(ValueError, match="overlaps"):
+            decode._apart(x, arr[x], y, arr[y])
+
+
+def test_append_kv_refuses_overlap_and_read_only():
+    rows = torch.zeros(4, 8, 64)
+    *args, _ = _append()
+    with pytest.raises(ValueError, match="`q_out` overlaps `q`"):
+        decode.append_kv(*args, q=rows[:3], q_out=rows[1:])
+    cache = np.zeros((10, 16, 2, 64), np.float32)
+    cache.flags.writeable = False
+    *args, _ = _append(k_cache=cache)
+    with pytest.raises(ValueError, match="read-only"):
+        decode.append_kv(*args)
+
+
+LOGITS = [
+    (dict(logits=torch.zeros(3, 100, dtype=torch.int32)), TypeError, "`logits`"),
+    (dict(logits=torch.zeros(300)), ValueError, "2 dimensions"),
+    (dict(logits=torch.zeros(100, 3).t()), ValueError, "contiguous"),
+    (dict(tokens=torch.zeros(2, 5, dtype=torch.int32)), ValueError, "`tokens`"),
+    (dict(tokens=torch.zeros(3, 5, dtype=torch.int64)), TypeError, "`tokens`"),
+    (dict(tokens=torch.zeros(3, 5, dtype=torch.int32),
+          token_lens=torch.zeros(2, dtype=torch.int32)), ValueError, "`token_lens`"),
+    (dict(repetition=1.2), ValueError, "need the history"),
+    (dict(token_lens=torch.zeros(3, dtype=torch.int32)), ValueError, "need the history"),
+    (dict(tokens=torch.zeros(3, 5, dtype=torch.int32), repetition=0.0), ValueError, "repetition"),
+    (dict(tokens=torch.zeros(3, 5, dtype=torch.int32), repetition=torch.zeros(2)), ValueError,
+     "`repetition`"),
+    (dict(temperature=torch.zeros(3).half()), TypeError, "`temperature`"),
+    (dict(bias=torch.zeros(3, 5)), ValueError, "go together"),
+    (dict(bias=torch.zeros(3, 5), bias_ids=torch.zeros(3, 4, dtype=torch.int32)), ValueError,
+     "`bias`"),
+    (dict(allowed=torch.zeros(3, 3, dtype=torch.int32)), ValueError, "need 4"),
+    (dict(allowed=torch.zeros(3, 4, dtype=torch.int64)), TypeError, "`allowed`"),
+    (dict(out=torch.zeros(3, 99)), ValueError, "`out`"),
+    (dict(out=torch.zeros(3, 1).expand(3, 100)), ValueError, "contiguous|expanded"),
+]
+
+
+@pytest.mark.parametrize("change,error,text", LOGITS)
+def test_adjust_logits_refuses(change, error, text):
+    kw = dict(logits=torch.zeros(3, 100))
+    kw.update(change)
+    with pytest.raises(error, match=text):
+        decode.adjust_logits(kw.pop("logits"), **kw)
+
+
+def test_calls_without_work_launch_nothing():
+    *args, kw = _attend(q=torch.zeros(0, 8, 64), seq_lens=torch.ones(0, dtype=torch.int32),
+                        block_table=torch.zeros(0, 4, dtype=torch.int32))
+    assert decode.paged_attention(*args, **kw).shape == (0, 8, 64)
+    *args, kw = _append(k=torch.zeros(0, 2, 64), v=torch.zeros(0, 2, 64),
+                        seq_lens=torch.ones(0, dtype=torch.int32),
+                        block_table=torch.zeros(0, 4, dtype=torch.int32))
+    assert decode.append_kv(*args, **kw) is None
+    assert decode.adjust_logits(torch.zeros(0, 50)).shape == (0, 50)
+    assert decode.adjust_logits(torch.zeros(3, 0)).shape == (3, 0)
+
+
+def test_page_division_is_exact():
+    """The multiplier that replaces the division by the page size, over all its uses: quotients
+    of positions below 2^30."""
+    rng = np.random.default_rng(0)
+    for page in [1, 2, 3, 5, 7, 8, 16, 24, 31, 64, 100, 127, 128, 1000, 4097, (1 << 29) - 1]:
+        mul, shift = decode._page_division(page)
+        assert 0 <= mul < 1 << 32
+        n = np.concatenate([rng.integers(0, 1 << 30, 20000), np.arange(5000),
+                            np.arange(1, 200) * page % (1 << 30),
+                            np.arange(1, 200) * page % (1 << 30) - 1,
+                            [(1 << 30) - 1]]).astype(object)
+        got = [int(x) if page == 1 else (int(x) * mul >> 32) >> shift for x in n]
+        assert got == [int(x) // page for x in n], page
+
+
+def test_module_is_public():
+    assert enceladus.decode is decode
+    for name in decode.__all__:
+        assert getattr(decode, name).__doc__
