@@ -181,6 +181,27 @@ int ek_launch(void* stream, void* function, uint32_t gx, uint32_t gy, uint32_t g
   return 0;
 }
 
+int ek_launch_list(const void* packed, size_t bytes, char* err, size_t errlen) {
+  ek_launch_list_head head;
+  if (bytes < sizeof(head)) return fail(err, errlen, "ek_launch_list: no head");
+  std::memcpy(&head, packed, sizeof(head));
+  const char* items = static_cast<const char*>(packed) + sizeof(head);
+  const size_t listed = (size_t)head.count * sizeof(ek_launch_list_item);
+  if (bytes != sizeof(head) + listed + head.kernarg_size) {
+    return fail(err, errlen, "ek_launch_list: the sizes do not add up");
+  }
+  void* kernarg = const_cast<char*>(items + listed);
+  for (uint32_t i = 0; i < head.count; ++i) {
+    ek_launch_list_item it;
+    std::memcpy(&it, items + i * sizeof(it), sizeof(it));
+    if (int rc = ek_launch(head.stream, it.function, it.gx, it.gy, it.gz, it.block, 1, 1, 0,
+                           kernarg, head.kernarg_size, err, errlen)) {
+      return rc;
+    }
+  }
+  return 0;
+}
+
 int ek_launch_timed_events(void* stream, void* function, uint32_t gx, uint32_t gy,
                            uint32_t gz, uint32_t bx, uint32_t by, uint32_t bz,
                            uint32_t dyn_lds, void* kernarg, size_t kernarg_size,

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 import sys
 import threading
@@ -34,6 +35,7 @@ from enceladus_amd.runtime import device as D
 from enceladus_amd.runtime import hip
 from enceladus_amd.runtime import tensor as T
 from enceladus_amd.runtime import timing as _timing
+from enceladus_amd.runtime.jit import _errbuf
 from enceladus_amd.runtime.probe import check_mfma_layout
 
 __all__ = ["append_kv", "paged_attention", "adjust_logits"]
@@ -85,16 +87,141 @@ def _function(file: str, macros: tuple, name: str, device: int):
     return f
 
 
-def _launch(fn, name: str, grid, block: int, kernarg: bytes, stream: int) -> None:
-    grid = (*grid, 1)
-    timer = _timing.current()
-    if timer is not None:
-        timer.launch(stream, fn, grid, block, kernarg, len(kernarg))
-        return
-    t0 = _trace.before_launch(stream) if _trace._active is not None else None
-    hip.call("ek_launch", stream or None, fn, *grid, block, 1, 1, 0, kernarg, len(kernarg))
-    if t0 is not None:
-        _trace.after_launch(t0, stream, name, grid, block, 0)
+class _Plan:
+    """A call as its arrays' types, shapes and strides and its options decide it: the kernels,
+    their grids and the bytes of their arguments but for the addresses. `arrays` (name, array
+    or None) are in the order of the kernels' pointers, and `written` are the ones that they
+    write; a workspace's address, if there is one, comes last."""
+
+    def __init__(self, file: str, macros: tuple, launches: list, arrays: list, written: set,
+                 workspace: int, tail: bytes, apart=()):
+        self.file, self.macros, self.launches = file, macros, launches
+        self.written, self.workspace, self.tail = written, workspace, tail
+        self.device = _device_of(arrays)
+        torch = _torch()
+        self.on_gpu = all(a is None or (a.device >= 0) for _, a in arrays)
+        self.where = torch.device("cuda", self.device) if self.device >= 0 else None
+        count = len(arrays) + (workspace > 0)
+        self.kernarg = struct.Struct(f"<{count}Q{len(tail)}s")
+        self.packed = struct.Struct(
+            f"<Q{8 + _ITEM.size * len(launches)}s{count}Q{len(tail)}s")
+        self.items = None
+        # (output, input, whether the input itself will do), by place and with their spans
+        self.apart = [(i, j, same, arrays[i][1].span(), arrays[j][1].span(),
+                       arrays[i][0], arrays[j][0])
+                      for i, j, same in apart if arrays[i][1] and arrays[j][1]]
+
+    def check_apart(self, objs: list) -> None:
+        """Refuses an output that overlaps an input."""
+        for i, j, same, n, m, name, other in self.apart:
+            a, b = _Array(name, objs[i]), _Array(other, objs[j])
+            p, q = a.address(), b.address()
+            if p < q + m and q < p + n:
+                _apart(name, a, other, b, same)
+
+    def functions(self, device: int) -> list:
+        return [_function(self.file, self.macros, name, device)
+                for name, _, _ in self.launches]
+
+    def run(self, objs: list) -> None:
+        """Launches the kernels for `objs` (in the order of the plan's arrays)."""
+        if not self.on_gpu:
+            return self._run_general(objs)
+        device = self.device
+        if _cuda.here() != device:
+            with _torch().cuda.device(device):
+                return self.run(objs)
+        ptrs = [0 if x is None else x.data_ptr() for x in objs]
+        if self.workspace:
+            keep = _cuda.empty(self.workspace, dtype=_cuda.uint8, device=self.where)
+            ptrs.append(keep.data_ptr())
+        stream = _cuda.stream(device)
+        if _timing.current() is not None or _trace._active is not None:
+            return self._launch(device, stream, self.kernarg.pack(*ptrs, self.tail))
+        if self.items is None:
+            self.items = _LIST.pack(len(self.launches), self.kernarg.size) + b"".join(
+                _ITEM.pack(f.value, *grid, 1, block)
+                for f, (_, grid, block) in zip(self.functions(device), self.launches))
+        packed = self.packed.pack(stream, self.items, *ptrs, self.tail)
+        err = _errbuf()
+        if _cuda.launch_list(packed, len(packed), err, 1024):
+            raise hip.HipError(f"ek_launch_list: {err.value.decode(errors='replace')}")
+
+    def _run_general(self, objs: list) -> None:
+        """With arrays on the host or of the framework's own: copied as a kernel's are."""
+        torch = _torch()
+        device = 0
+        if torch is not None and torch.cuda.is_available():
+            device = torch.cuda.current_device()
+            if 0 <= self.device != device:
+                with torch.cuda.device(self.device):
+                    return self._run_general(objs)
+        at = [i for i, x in enumerate(objs) if x is not None]
+        got, bindings = T.bind_arrays([objs[i] for i in at],
+                                      {k for k, i in enumerate(at) if i in self.written})
+        ptrs = [0] * len(objs)
+        for i, p in zip(at, got):
+            ptrs[i] = p
+        if self.workspace:
+            keep = T.empty((self.workspace,), "uint8")
+            ptrs.append(keep.ptr)
+        self._launch(device, D.current_stream(), self.kernarg.pack(*ptrs, self.tail))
+        T.complete_bindings(bindings)
+        if self.workspace:
+            hip.call("ek_stream_sync", D.current_stream() or None)   # before it is freed
+
+    def _launch(self, device: int, stream: int, kernarg: bytes) -> None:
+        timer = _timing.current()
+        for fn, (name, grid, block) in zip(self.functions(device), self.launches):
+            grid = (*grid, 1)
+            if timer is not None:
+                timer.launch(stream, fn, grid, block, kernarg, len(kernarg))
+                continue
+            t0 = _trace.before_launch(stream) if _trace._active is not None else None
+            hip.call("ek_launch", stream or None, fn, *grid, block, 1, 1, 0, kernarg,
+                     len(kernarg))
+            if t0 is not None:
+                _trace.after_launch(t0, stream, name, grid, block, 0)
+
+
+_LIST = struct.Struct("<II")
+_ITEM = struct.Struct("<Q4I")
+
+
+class _Cuda:
+    """What a plan's warm run calls, looked up once torch's GPU side is in use."""
+
+    def __getattr__(self, name):
+        torch = _torch()
+        self.here = torch.cuda.current_device
+        self.stream = lambda device: torch.cuda.current_stream(device).cuda_stream
+        if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+            self.stream = torch._C._cuda_getCurrentRawStream
+        if hasattr(torch._C, "_cuda_getDevice") and torch.cuda.is_initialized():
+            self.here = torch._C._cuda_getDevice
+        self.empty, self.uint8 = torch.empty, torch.uint8
+        self.launch_list = hip.load_library().ek_launch_list
+        return self.__dict__[name]
+
+
+_cuda = _Cuda()
+
+# Plans of the calls seen, by all that decides them (no address, and nothing of the arrays'
+# contents); started over when there are many.
+_plans: dict[tuple, tuple] = {}
+_MOST_PLANS = 4096
+
+
+def _keep(key, plan) -> None:
+    if key is not None and plan.on_gpu:
+        if len(_plans) >= _MOST_PLANS:
+            _plans.clear()
+        _plans[key] = plan
+
+
+def _of(x):
+    """What a plan depends on of an optional array."""
+    return None if x is None else (x.dtype, x.shape, x.stride(), x.get_device())
 
 
 # -- arguments ---------------------------------------------------------------------------
@@ -209,48 +336,6 @@ def _device_of(arrays) -> int:
     return found.pop() if found else -1
 
 
-class _On:
-    """The device of a call as the current one, and its current stream."""
-
-    def __init__(self, device: int):
-        torch = _torch()
-        self.guard, self.device, self.stream = None, 0, 0
-        if torch is not None and torch.cuda.is_available():
-            here = torch.cuda.current_device()
-            self.device = here if device < 0 else device
-            if self.device != here:
-                self.guard = torch.cuda.device(self.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        self.stream = D.current_stream()
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
-def _pointers(arrays, writes):
-    """(device addresses, bindings) of the arrays in order, 0 for those that are None."""
-    given = [a.obj for _, a in arrays if a is not None]
-    at = {i: k for k, i in enumerate(i for i, (_, a) in enumerate(arrays) if a is not None)}
-    got, bindings = T.bind_arrays(given, {at[i] for i in writes if i in at})
-    return [got[at[i]] if i in at else 0 for i in range(len(arrays))], bindings
-
-
-def _workspace(like: _Array, nbytes: int):
-    """Device memory for one call, on the call's device, and its address."""
-    torch = _torch()
-    if torch is not None and like.device >= 0:
-        t = torch.empty(nbytes, dtype=torch.uint8, device=like.obj.device)
-        return t, t.data_ptr()
-    t = T.empty((nbytes,), "uint8")
-    return t, t.ptr
-
-
 def _caches(k_cache, v_cache, heads, dim, kinds):
     kc = _array("k_cache", k_cache, kinds, 4, (None, None, heads, dim))
     vc = _array("v_cache", v_cache, (kc.kind,), 4, kc.shape)
@@ -295,7 +380,7 @@ def _scale_arg(name: str, x) -> float:
 
 # -- appending to the cache ----------------------------------------------------------------
 
-_APPEND = struct.Struct("<11Q16q11i2f4x")
+_APPEND = struct.Struct("<16q11i2f4x")
 
 
 def _vector(size: int, rotary: int, dim: int, interleaved: bool) -> int:
@@ -340,19 +425,45 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     Returns:
         The rotated queries, or None without `q`.
     """
-    kinds = ("fp32", "fp16", "bf16")
-    ka = _array("k", k, kinds, 3)
+    try:
+        key = (0, k.dtype, k.shape, k.stride(), k.get_device(), v.dtype, v.shape, v.stride(),
+               v.get_device(), k_cache.dtype, k_cache.shape, k_cache.stride(),
+               k_cache.get_device(), v_cache.dtype, v_cache.shape, v_cache.stride(),
+               v_cache.get_device(), _of(block_table), _of(seq_lens), _of(cu_tokens), _of(q),
+               _of(q_out), _of(cos), _of(sin), interleaved, k_scale, v_scale)
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None              # arrays of another kind, or no arrays
+    given = q_out is not None
+    if plan is None:
+        plan, q_out = _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q,
+                                   q_out, cos, sin, interleaved, k_scale, v_scale)
+        if plan is None:
+            return q_out
+        _keep(key, plan)
+    elif q is not None and not given:
+        q_out = T.new_empty(q)
+    arrays = [q, k, v, q_out, k_cache, v_cache, block_table, seq_lens, cu_tokens, cos, sin]
+    if given:
+        plan.check_apart(arrays)
+    plan.run(arrays)
+    return q_out
+
+
+def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_out, cos, sin,
+                 interleaved, k_scale, v_scale):
+    """The checked call's plan (None: nothing to do) and its `q_out`."""
+    ka = _array("k", k, ("fp32", "fp16", "bf16"), 3)
     tokens, kv_heads, dim = ka.shape
     va = _array("v", v, (ka.kind,), 3, ka.shape)
     kc, vc = _caches(k_cache, v_cache, kv_heads, dim, (ka.kind, "fp8"))
     _head_dim(dim, kc.kind)
     cu = None
+    batch = tokens
     if cu_tokens is not None:
         cu = _array("cu_tokens", cu_tokens, ("i32",), 1, dense=False)
         _need(cu.shape[0] > 0, "`cu_tokens` must have one entry more than there are sequences")
         batch = cu.shape[0] - 1
-    else:
-        batch = tokens
     bt, sl = _sequences(block_table, seq_lens, batch)
     capacity = _capacity(bt, kc)
     qa = qo = None
@@ -364,8 +475,6 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
             q_out = T.new_empty(q)
         qo = _array("q_out", q_out, (ka.kind,), 3, qa.shape)
         _written("q_out", qo)
-        for n, a in (("q", qa), ("k", ka), ("v", va)):
-            _apart("q_out", qo, n, a, same_ok=n == "q")
     else:
         _need(q_out is None, "`q_out` is given without `q`")
     _written("k_cache", kc)
@@ -379,11 +488,12 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
         rotary = 2 * ca.shape[1]
         _need(0 < rotary <= dim, f"`cos` rotates {rotary} elements of heads of {dim}")
     k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
-    if tokens == 0 or batch == 0 or kv_heads + heads == 0 or capacity == 0 or kc.shape[0] == 0:
-        return q_out
     arrays = [("q", qa), ("k", ka), ("v", va), ("q_out", qo), ("k_cache", kc), ("v_cache", vc),
               ("block_table", bt), ("seq_lens", sl), ("cu_tokens", cu), ("cos", ca),
               ("sin", sa)]
+    _device_of(arrays)
+    if tokens == 0 or batch == 0 or kv_heads + heads == 0 or capacity == 0 or kc.shape[0] == 0:
+        return None, q_out
     interleaved = bool(interleaved) and rotary > 0
     vec = _vector(ka.size, rotary, dim, interleaved)
     macros = (("EK_Q", _Q[ka.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_V", vec),
@@ -393,25 +503,22 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     rows = heads + 2 * kv_heads
     most = -(-rows // max(1, 64 // places))
     parts = max(1, min(most, 4096 // tokens))
-    with _On(_device_of(arrays)) as on:
-        ptrs, bindings = _pointers(arrays, {3, 4, 5})
-        zero = (0, 0, 0)
-        qs, os = (a.strides if a is not None else zero for a in (qa, qo))
-        kernarg = _APPEND.pack(
-            *ptrs, qs[0], qs[1], ka.strides[0], ka.strides[1], va.strides[0], va.strides[1],
-            os[0], os[1], *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0],
-            cu.strides[0] if cu else 0, ca.strides[0] if ca else 0, sa.strides[0] if sa else 0,
-            tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
-            ca.shape[0] if ca else 0, parts, 1.0 / k_scale, 1.0 / v_scale)
-        fn = _function("append_kv.hip", macros, "ek_append_kv", on.device)
-        _launch(fn, "ek_append_kv", (-(-tokens * parts // 4), 1), 256, kernarg, on.stream)
-        T.complete_bindings(bindings)
-    return q_out
+    zero = (0, 0, 0)
+    qs, os = (a.strides if a is not None else zero for a in (qa, qo))
+    tail = _APPEND.pack(
+        qs[0], qs[1], ka.strides[0], ka.strides[1], va.strides[0], va.strides[1], os[0], os[1],
+        *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0],
+        cu.strides[0] if cu else 0, ca.strides[0] if ca else 0, sa.strides[0] if sa else 0,
+        tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
+        ca.shape[0] if ca else 0, parts, 1.0 / k_scale, 1.0 / v_scale)
+    return _Plan("append_kv.hip", macros,
+                 [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
+                 tail, [(3, 0, True), (3, 1, False), (3, 2, False)]), q_out
 
 
 # -- attention over the cache ----------------------------------------------------------------
 
-_ATTEND = struct.Struct("<8Q9q8iI3i3f4x")
+_ATTEND = struct.Struct("<9q8iI3i3f4x")
 _UNIT = 64                          # tokens: what a sequence is split in multiples of
 _MIN_UNITS = 2
 _WORKGROUPS = 4                     # chunks of all sequences and key heads, per CU
@@ -448,6 +555,34 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
         The result, `[batch, heads, dim]` of the type of `q`; `(result, lse)` when
         `return_lse`.
     """
+    try:
+        key = (1, q.dtype, q.shape, q.stride(), q.get_device(), k_cache.dtype, k_cache.shape,
+               k_cache.stride(), k_cache.get_device(), v_cache.dtype, v_cache.shape,
+               v_cache.stride(), v_cache.get_device(), _of(block_table), _of(seq_lens),
+               _of(out), scale, window, type(window), softcap, k_scale, v_scale)
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None              # arrays of another kind, or no arrays
+    given = out is not None
+    if plan is None:
+        plan, out = _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window,
+                                    softcap, k_scale, v_scale, out)
+        if plan is not None:
+            _keep(key, plan)
+    elif not given:
+        out = T.new_empty(q)
+    lse = T.new_empty(q, tuple(q.shape[:2]), np.float32) if return_lse else None
+    if plan is not None:
+        arrays = [q, k_cache, v_cache, block_table, seq_lens, out, lse]
+        if given:
+            plan.check_apart(arrays)
+        plan.run(arrays)
+    return (out, lse) if return_lse else out
+
+
+def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, softcap, k_scale,
+                    v_scale, out):
+    """The checked call's plan (None: nothing to do) and its `out`."""
     qa = _array("q", q, ("fp32", "fp16", "bf16"), 3)
     batch, heads, dim = qa.shape
     kc, vc = _caches(k_cache, v_cache, None, dim,
@@ -461,7 +596,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
     capacity = _capacity(bt, kc)
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     _need(math.isfinite(scale), f"`scale` must be finite, got {scale}")
-    softcap, window = float(softcap), int(window)
+    softcap, window = float(softcap), operator.index(window)
     _need(math.isfinite(softcap) and softcap >= 0, f"`softcap` must be at least 0, got {softcap}")
     _need(window >= 0, f"`window` must be at least 0, got {window}")
     k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
@@ -469,51 +604,41 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
         out = T.new_empty(q)
     oa = _array("out", out, (qa.kind,), 3, qa.shape)
     _written("out", oa)
-    _apart("out", oa, "q", qa)
-    _apart("out", oa, "k_cache", kc, same_ok=False)
-    _apart("out", oa, "v_cache", vc, same_ok=False)
-    lse = T.new_empty(q, (batch, heads), np.float32) if return_lse else None
-    if batch and heads:
-        la = _Array("lse", lse) if return_lse else None
-        arrays = [("q", qa), ("k_cache", kc), ("v_cache", vc), ("block_table", bt),
-                  ("seq_lens", sl), ("out", oa), ("lse", la)]
-        if kc.shape[0] == 0:
-            capacity = 0
-        window = min(window, MAX_TOKENS)
-        most = -(-(min(window, capacity) if window else capacity) // _UNIT)
-        group = heads // kv_heads
-        y = kv_heads * (-(-group // 16))
-        items = max(1, min(_WORKGROUPS * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
-        single = most <= _MIN_UNITS
-        page = kc.shape[1]
-        width = 64 if dim <= 64 else 128 if dim <= 128 else 256
-        macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
-                  ("EK_PAD", int(dim != width)))
-        log2e = 1.4426950408889634
-        with _On(_device_of(arrays)) as on:
-            ptrs, bindings = _pointers(arrays, {5, 6})
-            part = keep = None
-            if not single:
-                keep, part = _workspace(qa, (items + batch) * heads * (dim + 2) * 4)
-            kernarg = _ATTEND.pack(
-                *ptrs, part or 0, qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
-                *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch,
-                heads, group, dim, page, kc.shape[0], capacity, window,
-                *_page_division(page), items, _MIN_UNITS, scale * k_scale * log2e, softcap * log2e, v_scale)
-            fn = _function("paged_attention.hip", macros, "ek_paged_attention", on.device)
-            _launch(fn, "ek_paged_attention", (items + batch, y), 256, kernarg, on.stream)
-            if not single:
-                fn = _function("paged_attention.hip", macros, "ek_paged_attention_join",
-                               on.device)
-                _launch(fn, "ek_paged_attention_join", (batch, heads), 256, kernarg, on.stream)
-            T.complete_bindings(bindings)
-            del keep
-    return (out, lse) if return_lse else out
+    arrays = [("q", qa), ("k_cache", kc), ("v_cache", vc), ("block_table", bt),
+              ("seq_lens", sl), ("out", oa), ("lse", None)]
+    _device_of(arrays)
+    if batch == 0 or heads == 0:
+        return None, out
+    if kc.shape[0] == 0:
+        capacity = 0
+    window = min(window, MAX_TOKENS)
+    most = -(-(min(window, capacity) if window else capacity) // _UNIT)
+    group = heads // kv_heads
+    y = kv_heads * (-(-group // 16))
+    items = max(1, min(_WORKGROUPS * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
+    width = 64 if dim <= 64 else 128 if dim <= 128 else 256
+    macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
+              ("EK_PAD", int(dim != width)))
+    log2e = 1.4426950408889634
+    launches = [("ek_paged_attention", (items + batch, y), 256)]
+    workspace = 0
+    if most > _MIN_UNITS:              # some sequence may have more than one chunk
+        launches.append(("ek_paged_attention_join", (batch, heads), 256))
+        workspace = (items + batch) * heads * (dim + 2) * 4
+    tail = _ATTEND.pack(
+        qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
+        *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch, heads,
+        group, dim, kc.shape[1], kc.shape[0], capacity, window, *_page_division(kc.shape[1]),
+        items, _MIN_UNITS, scale * k_scale * log2e, softcap * log2e, v_scale)
+    if not workspace:
+        tail = bytes(8) + tail         # the address of the partial results
+    return _Plan("paged_attention.hip", macros, launches, arrays, {5, 6}, workspace, tail,
+                 [(5, 0, True), (5, 1, False), (5, 2, False)]), out
 
 
 # -- logits ----------------------------------------------------------------------------------
 
-_LOGITS = struct.Struct("<12Q12q3i4f4x")
+_LOGITS = struct.Struct("<12q3i4f4x")
 
 
 def _per_row(name: str, x, rows: int, default: float):
@@ -555,6 +680,40 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
     Returns:
         The adjusted logits, of the type of `logits`.
     """
+    try:
+        key = (2, logits.dtype, logits.shape, logits.stride(), logits.get_device(), _of(tokens),
+               _of(token_lens), _of(prompt_lens), _number_or(repetition), _number_or(frequency),
+               _number_or(presence), _number_or(temperature), _of(bias_ids), _of(bias),
+               _of(allowed), _of(out))
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None              # arrays of another kind, or no arrays
+    given = out is not None
+    if plan is None:
+        plan, out = _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency,
+                                 presence, temperature, bias_ids, bias, allowed, out)
+        if plan is None:
+            return out
+        _keep(key, plan)
+    elif not given:
+        out = T.new_empty(logits)
+    arrays = [logits, out, tokens, token_lens, prompt_lens,
+              *(x if hasattr(x, "shape") else None
+                for x in (repetition, frequency, presence, temperature)),
+              bias_ids, bias, allowed]
+    if given:
+        plan.check_apart(arrays)
+    plan.run(arrays)
+    return out
+
+
+def _number_or(x):
+    return _of(x) if hasattr(x, "stride") else x
+
+
+def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency, presence,
+                 temperature, bias_ids, bias, allowed, out):
+    """The checked call's plan (None: nothing to do) and its `out`."""
     la = _array("logits", logits, ("fp32", "fp16", "bf16"), 2)
     rows, vocab = la.shape
     ta = tl = pl = None
@@ -587,16 +746,13 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
         out = T.new_empty(logits)
     oa = _array("out", out, (la.kind,), 2, la.shape)
     _written("out", oa)
-    _apart("out", oa, "logits", la)
     arrays = [("logits", la), ("out", oa), ("tokens", ta), ("token_lens", tl),
               ("prompt_lens", pl), ("repetition", rep_a), ("frequency", freq_a),
               ("presence", pres_a), ("temperature", temp_a), ("bias_ids", ia), ("bias", ba),
               ("allowed", aa)]
-    for n, a in arrays[2:]:
-        if a is not None:
-            _apart("out", oa, n, a, same_ok=False)
+    _device_of(arrays)
     if rows == 0 or vocab == 0:
-        return out
+        return None, out
     _need(vocab < 1 << 30 and rows * vocab < 1 << 41,
           f"logits of shape {la.shape} are too large for one call")
     biases = ia.shape[1] if ia else 0
@@ -609,18 +765,12 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
     def step(a):
         return a.strides[0] if a is not None else 0
 
-    with _On(_device_of(arrays)) as on:
-        ptrs, bindings = _pointers(arrays, {1})
-        if ta is not None and ta.shape[1] == 0:
-            ptrs[2] = 0
-        kernarg = _LOGITS.pack(*ptrs, step(la), step(oa), step(ta), step(ia), step(ba), step(aa),
-                               step(tl), step(pl), step(rep_a), step(freq_a), step(pres_a),
-                               step(temp_a), vocab, ta.shape[1] if ta else 0, biases, rep, freq,
-                               pres, temp)
-        fn = _function("adjust_logits.hip", macros, "ek_adjust_logits", on.device)
-        _launch(fn, "ek_adjust_logits", (-(-vocab // n) * rows, 1), threads, kernarg, on.stream)
-        T.complete_bindings(bindings)
-    return out
+    tail = _LOGITS.pack(step(la), step(oa), step(ta), step(ia), step(ba), step(aa), step(tl),
+                        step(pl), step(rep_a), step(freq_a), step(pres_a), step(temp_a), vocab,
+                        ta.shape[1] if ta else 0, biases, rep, freq, pres, temp)
+    return _Plan("adjust_logits.hip", macros,
+                 [("ek_adjust_logits", (-(-vocab // n) * rows, 1), threads)], arrays, {1}, 0,
+                 tail, [(1, 0, True)] + [(1, i, False) for i in range(2, 12)]), out
 
 
 def specializations():

@@ -70,6 +70,7 @@ _SIGS = {
     "ek_function_get_attrs": [ctypes.c_void_p, ctypes.POINTER(FunctionAttrs)],
     "ek_launch": [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_uint32] * 7 +
                  [ctypes.c_void_p, ctypes.c_size_t],
+    "ek_launch_list": [ctypes.c_void_p, ctypes.c_size_t],
     "ek_stream_new": [ctypes.POINTER(ctypes.c_void_p)],
     "ek_stream_free": [ctypes.c_void_p],
     "ek_stream_sync": [ctypes.c_void_p],

@@ -70,6 +70,22 @@ int ek_launch(void* stream, void* function, uint32_t gx, uint32_t gy, uint32_t g
               uint32_t bx, uint32_t by, uint32_t bz, uint32_t dyn_lds, void* kernarg,
               size_t kernarg_size, char* err, size_t errlen);
 
+/* No counterpart in the reference. Launches kernels that share one argument block, in order, from
+ * one packed buffer (one call of a foreign-function interface instead of one per kernel and
+ * argument): ek_launch_list_head, then `count` ek_launch_list_item, then the kernarg bytes (as
+ * for ek_launch). Blocks are 1-D. Fails, launching nothing, when the sizes do not add up to
+ * `bytes`; a failing launch leaves the ones before it in the stream. */
+typedef struct ek_launch_list_head {
+  void* stream;
+  uint32_t count;
+  uint32_t kernarg_size;
+} ek_launch_list_head;
+typedef struct ek_launch_list_item {
+  void* function;
+  uint32_t gx, gy, gz, block;
+} ek_launch_list_item;
+int ek_launch_list(const void* packed, size_t bytes, char* err, size_t errlen);
+
 /* Streams. Replaces fr_stream_new/fr_stream_sync (reference _C/enceladus_rt.mm:357-577). */
 int ek_stream_new(void** stream, char* err, size_t errlen);
 int ek_stream_free(void* stream, char* err, size_t errlen);

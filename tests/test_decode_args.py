@@ -57,6 +57,7 @@ ATTEND = [
     (dict(seq_lens=np.ones(3, np.float32)), TypeError, "`seq_lens`"),
     (dict(seq_lens=np.ones(3, np.int32)[::-1]), ValueError, "negative strides"),
     (dict(window=-1), ValueError, "window"),
+    (dict(window=1.5), TypeError, "integer"),
     (dict(softcap=-1.0), ValueError, "softcap"),
     (dict(softcap=float("nan")), ValueError, "softcap"),
     (dict(scale=float("inf")), ValueError, "scale"),
