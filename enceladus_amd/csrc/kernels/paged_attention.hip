@@ -22,10 +22,10 @@
 // - The weights are split into two terms of the 16-bit type (p = hi + lo), two products each:
 //   the matrix units idle anyway, and the output keeps the accuracy of 32-bit weights.
 //
-// Work: a chunk of one sequence is an item; a workgroup (4 waves, tiles in turn) takes one item
-// of one key head. The chunk's length comes from all sequences' lengths, on the device, so that
-// ragged batches give items of about one size. Sequences of one chunk are finished here;
-// the others leave (m, l, O) per chunk to the second kernel.
+// Work: a chunk of one sequence is an item; one wave takes an item of one key head, by itself.
+// The chunks' length comes from all sequences' lengths, on the device, so that ragged batches
+// give items of about one size. Sequences of one chunk are finished here; the others leave
+// (O, m, l) per chunk to the second kernel.
 //
 // Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_FP8 (the cache is e4m3), EK_DP (64, 128 or 256: the
 // head dimension it is compiled for), EK_PAD (the head dimension is smaller than EK_DP).
@@ -40,12 +40,17 @@ typedef ek::bf16 T;
 #endif
 constexpr int DP = EK_DP;
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
-constexpr int WAVES = 4;
 constexpr float LN2 = 0.69314718055994531f;
-// Keys per wave and step: 16 KB of keys and values, where the products' shapes allow it.
-constexpr int KT0 = 8192 / (DP * CS);
-constexpr int KTMIN = EK_Q == 0 ? 16 : 32;
-constexpr int KT = KT0 < KTMIN ? KTMIN : KT0 > 64 ? 64 : KT0;
+// Keys per wave and step.
+#ifndef EK_KT
+#define EK_KT 0
+#endif
+constexpr int KT0 = 4096 / (DP * CS);
+constexpr int KTMIN = 16;
+constexpr int KT = EK_KT ? EK_KT : KT0 < KTMIN ? KTMIN : KT0 > 64 ? 64 : KT0;
+#ifndef EK_OCC
+#define EK_OCC 2
+#endif
 constexpr int ST = KT / 16;                         // score tiles
 constexpr int KE = 16 / CS;                         // elements of a 16-byte key load
 constexpr int KL = DP / (4 * KE);                   // key loads per score tile and lane
@@ -55,7 +60,7 @@ constexpr int VE = VE0 * 16 > DP ? DP / 16 : VE0;
 constexpr int PANELS = DP / (16 * VE);
 constexpr int VR = KT / 4;                          // value rows per lane
 constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value load
-constexpr int UNIT = 64;                            // keys: what chunks are multiples of
+constexpr int UNIT = 16;                            // keys: what chunks are multiples of
 // Weights are exp2(s - m + LIFT). Fp16 has no more than 24 binary places below 1: lifted to
 // 2^14, a weight keeps them down to 2^-39 of the largest one (131072 keys of a weight of 2^-26
 // each are 0.2% of the sum). bf16 and fp32 have the exponents for it.
@@ -63,11 +68,14 @@ constexpr float LIFT = EK_Q == 1 ? 14.0f : 0.0f;
 
 typedef uint32_t u32;
 template <int W> struct words { u32 w[W]; };
-template <int W> EK_INLINE words<W> load_words(const char* p) {
+template <int W, bool NT = false> EK_INLINE words<W> load_words(const char* p) {
   words<W> r;
-  ek::vload_u<uint8_t, W * 4>((uint8_t*)r.w, (const uint8_t*)p);
+  if constexpr (NT) ek::vload_nt_u<uint8_t, W * 4>((uint8_t*)r.w, (const uint8_t*)p);
+  else ek::vload_u<uint8_t, W * 4>((uint8_t*)r.w, (const uint8_t*)p);
   return r;
 }
+
+template <bool B> struct flag { static constexpr bool value = B; };
 
 struct Params {
   const T* q;
@@ -77,13 +85,14 @@ struct Params {
   const int32_t* lens;
   T* out;
   float* lse;
-  float* part;                       // [item][head][dim + 2]: O, m, l
+  float* part;   // [item][head][dim]: O; then [item][head][2]: m, l; then [sequence][2] words:
+                 // its first item and how many; or null: no sequence has two chunks
   int64_t q_row, q_head, out_row, out_head;   // elements
   int64_t c_page, c_token, c_head;   // bytes
   int64_t table_row, lens_step;      // elements
   int32_t batch, heads, group, dim, page, pages, capacity, window;
   uint32_t page_mul;
-  int32_t page_shift, items, min_units;
+  int32_t page_shift, items, min_units, join_waves, stream;
   float scale, cap, v_scale;         // scale includes log2(e); cap in the same unit, or 0
 };
 
@@ -101,26 +110,93 @@ EK_INLINE void span_of(const Params& a, int b, int& first, int& count) {
 
 EK_INLINE int units_of(int count) { return (count + UNIT - 1) / UNIT; }
 
-// The units of 64 keys per chunk, the same for every wave of both kernels.
-EK_INLINE int chunk_units(const Params& a) {
-  const int lane = ek::lane_id();
-  int total = 0;
-  for (int b = lane; b - lane < a.batch; b += 64) {
-    int first, count;
-    span_of(a, b, first, count);
-    total += units_of(count);
-  }
-  total = ek::reduce_xor<ek::Sum, 1>(total);
-  total = ek::reduce_xor<ek::Sum, 2>(total);
-  total = ek::reduce_xor<ek::Sum, 4>(total);
-  total = ek::reduce_xor<ek::Sum, 8>(total);
-  total = ek::reduce_xor<ek::Sum, 16>(total);
-  total = ek::reduce_xor<ek::Sum, 32>(total);
-  const int u = (total + a.items - 1) / a.items;
-  return u < a.min_units ? a.min_units : u;
+EK_INLINE int chunks_of(int units, int per) { return (units + per - 1) / per; }
+
+template <typename OP, typename V> EK_INLINE V wave_all(V x) {
+  x = ek::reduce_xor<OP, 1>(x);
+  x = ek::reduce_xor<OP, 2>(x);
+  x = ek::reduce_xor<OP, 4>(x);
+  x = ek::reduce_xor<OP, 8>(x);
+  x = ek::reduce_xor<OP, 16>(x);
+  return ek::reduce_xor<OP, 32>(x);
 }
 
-EK_INLINE int chunks_of(int units, int per) { return (units + per - 1) / per; }
+// What an item is: chunk `index` of the `chunks` of sequence b, or, with chunks 0, an empty
+// sequence b; b is -1 for items without work. `start` is the sequence's first item.
+struct Item {
+  int b, first, count, index, chunks, start;
+};
+
+// The chunks of all sequences in their order are items 0, 1, ...: at most `items` of them and
+// one more for each sequence with tokens, so that the grid's further `batch` items are enough
+// to give every empty sequence one as well. A chunk has as many units of 64 keys as give
+// `items` chunks in all. Every wave finds its own from the lengths: 64 sequences at a time, a
+// lane each, of which the first HELD times 64 stay in registers between the sum and the search.
+EK_INLINE Item find_item(const Params& a, int item) {
+  constexpr int HELD = 4;
+  const int lane = ek::lane_id();
+  int f[HELD], n[HELD], total = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    f[i] = n[i] = 0;
+    if (i == 0 || i * 64 < a.batch) span_of(a, i * 64 + lane, f[i], n[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) total += units_of(n[i]);
+  for (int base = HELD * 64; base < a.batch; base += 64) {
+    int first, count;
+    span_of(a, base + lane, first, count);
+    total += units_of(count);
+  }
+  total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
+  // each sequence may take a chunk more than its share: kept within the items, if they are many
+  const int share = a.items > 2 * a.batch ? a.items - a.batch : (a.items + 1) / 2;
+  int per = (total + share - 1) / share;
+  per = per < a.min_units ? a.min_units : per;
+
+  int before = 0;
+  const auto search = [&](int base, int first, int count, Item& it) {
+    const int mine = chunks_of(units_of(count), per);
+    const int end = before + ek::wave_prefix_sum(mine);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(item < end);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      it.b = base + at;
+      it.first = __builtin_amdgcn_readlane(first, at);
+      it.count = __builtin_amdgcn_readlane(count, at);
+      it.chunks = __builtin_amdgcn_readlane(mine, at);
+      it.start = __builtin_amdgcn_readlane(end, at) - it.chunks;
+      it.index = item - it.start;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(end, 63);
+    return false;
+  };
+  Item it = {-1, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (i * 64 < a.batch && search(i * 64, f[i], n[i], it)) return it;
+  for (int base = HELD * 64; base < a.batch; base += 64) {
+    int first, count;
+    span_of(a, base + lane, first, count);
+    if (search(base, first, count, it)) return it;
+  }
+  // past the last chunk: the empty sequence of that rank
+  int rank = item - before;
+  for (int base = 0; base < a.batch; base += 64) {
+    int first, count;
+    span_of(a, base + lane, first, count);
+    uint64_t none = __builtin_amdgcn_ballot_w64(base + lane < a.batch && count == 0);
+    const int here = __builtin_popcountll(none);
+    if (rank < here) {
+      for (; rank > 0; --rank) none &= none - 1;
+      it.b = base + __builtin_ctzll(none);
+      return it;
+    }
+    rank -= here;
+  }
+  return it;
+}
 
 EK_INLINE float tanh_f(float x) {
   const float y = __builtin_fabsf(x);
@@ -133,7 +209,7 @@ EK_INLINE float tanh_f(float x) {
   s = __builtin_fmaf(z, s, -1.0f / 3.0f);
   s = __builtin_fmaf(z * s, y, y);
   const float e = ek::exp2_fast(y * -2.8853900817779268f);
-  const float r = (1.0f - e) / (1.0f + e);
+  const float r = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
   return __builtin_copysignf(y < 0.35f ? s : r, x);
 }
 
@@ -163,6 +239,16 @@ EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32* b) {
                                                 acc, 0, 0, 0);
 #endif
 }
+// The same over 16 k values: two words per lane and operand.
+EK_INLINE void mma16(ek::f32x4& acc, const u32* a, const u32* b) {
+#if EK_Q == 1
+  acc = __builtin_amdgcn_mfma_f32_16x16x16f16(ek::pack<ek::f16x4>(a), ek::pack<ek::f16x4>(b),
+                                              acc, 0, 0, 0);
+#else
+  acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(ek::pack<ek::s16x4>(a), ek::pack<ek::s16x4>(b),
+                                                  acc, 0, 0, 0);
+#endif
+}
 #if EK_Q == 1
 typedef _Float16 half_t;
 #else
@@ -188,64 +274,35 @@ struct Tile {
   words<VW> v[VR][PANELS];
 };
 
-extern "C" __global__ __launch_bounds__(256) void ek_paged_attention(Params a) {
-  __shared__ float s_o[WAVES][16][DP + 4];
-  __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Params a) {
   const int lane = ek::lane_id(), r = lane & 15, c = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles16 = (a.group + 15) / 16;
   const int g = blockIdx.y / tiles16, h0 = (blockIdx.y - g * tiles16) * 16;
   const int nh = a.group - h0 < 16 ? a.group - h0 : 16;
 
-  // which sequence and chunk this item is
-  const int per = chunk_units(a);
-  int item = blockIdx.x, b = -1, first = 0, count = 0, chunks = 0, all = 0;
-  for (int base = 0; base < a.batch; base += 64) {
-    int f, n;
-    span_of(a, base + lane, f, n);
-    const int mine = chunks_of(units_of(n), per);
-    const int end = all + ek::wave_prefix_sum(mine);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(item < end);
-    if (hit != 0) {
-      const int at = __builtin_ctzll(hit);
-      b = base + at;
-      first = __builtin_amdgcn_readlane(f, at);
-      count = __builtin_amdgcn_readlane(n, at);
-      chunks = __builtin_amdgcn_readlane(mine, at);
-      item -= __builtin_amdgcn_readlane(end, at) - chunks;
-      break;
-    }
-    all = __builtin_amdgcn_readlane(end, 63);
+  const Item it = find_item(a, blockIdx.x);
+  const int b = it.b, chunks = it.chunks;
+  if (b < 0) return;
+  if (a.part && it.index == 0 && blockIdx.y == 0 && lane == 0) {
+    // for the second kernel: which items the sequence's chunks are
+    int32_t* info = (int32_t*)(a.part + (int64_t)(a.items + a.batch) * a.heads * (a.dim + 2));
+    info[2 * b] = it.start;
+    info[2 * b + 1] = chunks;
   }
-  if (b < 0) {
-    // there are at least as many items past the last one as sequences without tokens
-    // (chunks <= items + sequences with tokens): each finishes one of those
-    int skip = blockIdx.x - all;
-    for (int base = 0; base < a.batch; base += 64) {
-      int f, n;
-      span_of(a, base + lane, f, n);
-      uint64_t none = __builtin_amdgcn_ballot_w64(base + lane < a.batch && n == 0);
-      const int here = __builtin_popcountll(none);
-      if (skip >= here) {
-        skip -= here;
-        continue;
-      }
-      for (; skip > 0; --skip) none &= none - 1;
-      const int64_t e = base + __builtin_ctzll(none);
-      for (int x = threadIdx.x; x < nh * a.dim; x += 256) {
-        const int h = x / a.dim, d = x - h * a.dim, head = g * a.group + h0 + h;
-        a.out[e * a.out_row + head * a.out_head + d] = ek::cvt<T>(0.0f);
-        if (a.lse && d == 0) a.lse[e * a.heads + head] = -__builtin_inff();
-      }
-      return;
+  if (chunks == 0) {
+    for (int x = lane; x < nh * a.dim; x += 64) {
+      const int h = x / a.dim, d = x - h * a.dim, head = g * a.group + h0 + h;
+      a.out[b * a.out_row + head * a.out_head + d] = ek::cvt<T>(0.0f);
+      if (a.lse && d == 0) a.lse[(int64_t)b * a.heads + head] = -__builtin_inff();
     }
     return;
   }
-  const int units = units_of(count);
-  const int lo_u = (int)((int64_t)units * item / chunks);
-  const int hi_u = (int)((int64_t)units * (item + 1) / chunks);
-  const int lo = first + lo_u * UNIT;
-  const int hi = hi_u == units ? first + count : first + hi_u * UNIT;
+  // units are spread evenly over the chunks: the first few have one more
+  const int units = units_of(it.count), each = units / chunks, more = units - each * chunks;
+  const int lo_u = it.index * each + (it.index < more ? it.index : more);
+  const int hi_u = lo_u + each + (it.index < more);
+  const int lo = it.first + lo_u * UNIT;
+  const int hi = hi_u == units ? it.first + it.count : it.first + hi_u * UNIT;
 
   const char* kbase = a.k + g * a.c_head;
   const char* vbase = a.v + g * a.c_head;
@@ -277,6 +334,7 @@ extern "C" __global__ __launch_bounds__(256) void ek_paged_attention(Params a) {
 #endif
   }
 
+  const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
   float m = -__builtin_inff(), l = 0.0f;
   ek::f32x4 o[PANELS][VE];
 #pragma unroll
@@ -297,280 +355,318 @@ extern "C" __global__ __launch_bounds__(256) void ek_paged_attention(Params a) {
     return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : 0;
   };
   const auto load_k = [&](Tile& t, int64_t off) {
-#pragma unroll
-    for (int s = 0; s < ST; ++s) {
-      const char* p = kbase + ek::shfl(off, s * 16 + r);
-#pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int d = (i * 4 + c) * KE;
-        if (EK_PAD) {
-          t.k[s][i] = words<4>{{0, 0, 0, 0}};
-          if (d < a.dim) t.k[s][i] = load_words<4>(p + d * CS);
-        } else {
-          t.k[s][i] = load_words<4>(p + d * CS);
-        }
-      }
-    }
-  };
-  const auto load_v = [&](Tile& t, int64_t off) {
-#pragma unroll
-    for (int j = 0; j < VR; ++j) {
-      const char* p = vbase + ek::shfl(off, (j / 4) * 16 + c * 4 + (j & 3));
-#pragma unroll
-      for (int i = 0; i < PANELS; ++i) {
-        const int d = i * 16 * VE + r * VE;
-        if (EK_PAD) {
-          t.v[j][i] = words<VW>{};
-          if (d < a.dim) t.v[j][i] = load_words<VW>(p + d * CS);
-        } else {
-          t.v[j][i] = load_words<VW>(p + d * CS);
-        }
-      }
-    }
-  };
-
-  const int step = WAVES * KT;
-  int base = lo + wave * KT;
-  if (base < hi) {
-    Tile t;
-    uint64_t live, live_next = 0;
-    int64_t off = offset(base, page_id(base), live);
-    load_k(t, off);
-    load_v(t, off);
-    int id = page_id(base + step);
-    for (;;) {
-      // scores of KT keys: acc[s][i] is key 16 s + 4 c + i of head r
-      ek::f32x4 acc[ST];
+    const auto go = [&](auto nt) {
 #pragma unroll
       for (int s = 0; s < ST; ++s) {
-        acc[s] = ek::f32x4{0, 0, 0, 0};
+        const char* p = kbase + ek::shfl(off, s * 16 + r);
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
+          const int d = (i * 4 + c) * KE;
+          if (EK_PAD) t.k[s][i] = words<4>{{0, 0, 0, 0}};
+          if (!EK_PAD || d < a.dim) t.k[s][i] = load_words<4, nt.value>(p + d * CS);
+        }
+      }
+    };
+    if (a.stream) go(flag<true>());
+    else go(flag<false>());
+  };
+  const auto load_v = [&](Tile& t, int64_t off) {
+    const auto go = [&](auto nt) {
+#pragma unroll
+      for (int j = 0; j < VR; ++j) {
+        const char* p = vbase + ek::shfl(off, (j / 4) * 16 + c * 4 + (j & 3));
+#pragma unroll
+        for (int i = 0; i < PANELS; ++i) {
+          const int d = i * 16 * VE + r * VE;
+          if (EK_PAD) t.v[j][i] = words<VW>{};
+          if (!EK_PAD || d < a.dim) t.v[j][i] = load_words<VW, nt.value>(p + d * CS);
+        }
+      }
+    };
+    if (a.stream) go(flag<true>());
+    else go(flag<false>());
+  };
+
+  Tile t;
+  uint64_t live = 0;
+  int64_t off = offset(lo, page_id(lo), live);
+  load_k(t, off);
+  load_v(t, off);
+  int id = page_id(lo + KT);
+  for (int base = lo; base < hi; base += KT) {
+    const int next = base + KT;
+    uint64_t live_next = 0;
+    // scores of KT keys: acc[s][i] is key 16 s + 4 c + i of head r
+    ek::f32x4 acc[ST];
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+      acc[s] = ek::f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
 #if EK_Q == 0
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(t.k[s][i].w[e]),
-                                                          q.w[i][e], acc[s], 0, 0, 0);
+        for (int e = 0; e < 4; ++e)
+          acc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(t.k[s][i].w[e]),
+                                                        q.w[i][e], acc[s], 0, 0, 0);
 #elif EK_FP8
-          u32 x[8];
+        u32 x[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) widen4(t.k[s][i].w[e], &x[2 * e], &x[2 * e + 1]);
-          mma(acc[s], x, q.w[2 * i]);
-          mma(acc[s], x + 4, q.w[2 * i + 1]);
+        for (int e = 0; e < 4; ++e) widen4(t.k[s][i].w[e], &x[2 * e], &x[2 * e + 1]);
+        mma(acc[s], x, q.w[2 * i]);
+        mma(acc[s], x + 4, q.w[2 * i + 1]);
 #else
-          mma(acc[s], t.k[s][i].w, q.w[i]);
+        mma(acc[s], t.k[s][i].w, q.w[i]);
 #endif
-        }
       }
-      const int next = base + step;
-      if (next < hi) {
-        off = offset(next, id, live_next);
-        id = page_id(next + step);
-        load_k(t, off);
+    }
+    if (next < hi) {
+      off = offset(next, id, live_next);
+      id = page_id(next + KT);
+      load_k(t, off);
+    }
+    // softmax
+    float mt = -__builtin_inff();
+    const bool full = live == ~0ull;
+#pragma unroll
+    for (int s = 0; s < ST; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = acc[s][i] * a.scale;
+        if (a.cap > 0.0f) x = a.cap * tanh_f(x * inv_cap);
+        if (!full && !(live >> (s * 16 + c * 4 + i) & 1)) x = -__builtin_inff();
+        acc[s][i] = x;
+        mt = __builtin_fmaxf(mt, x);
       }
-      // softmax
-      float mt = -__builtin_inff();
-      const bool full = live == ~0ull;
-#pragma unroll
-      for (int s = 0; s < ST; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = acc[s][i] * a.scale;
-          if (a.cap > 0.0f) x = a.cap * tanh_f(x / a.cap);
-          if (!full && !(live >> (s * 16 + c * 4 + i) & 1)) x = -__builtin_inff();
-          acc[s][i] = x;
-          mt = __builtin_fmaxf(mt, x);
-        }
-      mt = ek::reduce_xor<ek::Max, 16>(mt);
-      mt = ek::reduce_xor<ek::Max, 32>(mt);
-      const float m_new = __builtin_fmaxf(m, mt);
-      const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-      const float alpha = ek::exp2_fast(m - m_use);
-      m = m_new;
+    mt = ek::reduce_xor<ek::Max, 16>(mt);
+    mt = ek::reduce_xor<ek::Max, 32>(mt);
+    const float m_new = __builtin_fmaxf(m, mt);
+    const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
+    const float alpha = ek::exp2_fast(m - m_use);
+    m = m_new;
+    // most steps raise no head's maximum
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
       l *= alpha;
 #pragma unroll
       for (int p = 0; p < PANELS; ++p)
 #pragma unroll
         for (int e = 0; e < VE; ++e) o[p][e] *= alpha;
+    }
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
+    for (int s = 0; s < ST; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[s][i] = ek::exp2_fast(acc[s][i] - (m_use - LIFT));
-          l += acc[s][i];
-        }
-      // values without a key are taken as zeros: their memory may hold anything
-      if (!full) {
-#pragma unroll
-        for (int j = 0; j < VR; ++j) {
-          const bool ok = live >> ((j / 4) * 16 + c * 4 + (j & 3)) & 1;
-#pragma unroll
-          for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) t.v[j][p].w[w] = ok ? t.v[j][p].w[w] : 0;
-        }
+      for (int i = 0; i < 4; ++i) {
+        acc[s][i] = ek::exp2_fast(acc[s][i] - (m_use - LIFT));
+        l += acc[s][i];
       }
-#if EK_Q == 0
+    // values without a key are taken as zeros: their memory may hold anything
+    if (!full) {
 #pragma unroll
-      for (int j = 0; j < VR; ++j)
+      for (int j = 0; j < VR; ++j) {
+        const bool ok = live >> ((j / 4) * 16 + c * 4 + (j & 3)) & 1;
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
 #pragma unroll
-          for (int e = 0; e < VE; ++e)
-            o[p][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(t.v[j][p].w[e]),
-                                                           acc[j / 4][j & 3], o[p][e], 0, 0, 0);
+          for (int w = 0; w < VW; ++w) t.v[j][p].w[w] = ok ? t.v[j][p].w[w] : 0;
+      }
+    }
+#if EK_Q == 0
+#pragma unroll
+    for (int j = 0; j < VR; ++j)
+#pragma unroll
+      for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          o[p][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(t.v[j][p].w[e]),
+                                                         acc[j / 4][j & 3], o[p][e], 0, 0, 0);
 #else
+    constexpr int SS = ST == 1 ? 1 : 2;            // score tiles of a product
 #pragma unroll
-      for (int s = 0; s < ST; s += 2) {
-        u32 ph[4], pl[4];
+    for (int s = 0; s < ST; s += SS) {
+      u32 ph[2 * SS], pl[2 * SS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = acc[s + i / 2][(i & 1) * 2], y = acc[s + i / 2][(i & 1) * 2 + 1];
-          const half_t xh = (half_t)x, yh = (half_t)y;
-          ph[i] = pack2(xh, yh);
-          pl[i] = pack2((half_t)(x - (float)xh), (half_t)(y - (float)yh));
-        }
+      for (int i = 0; i < 2 * SS; ++i) {
+        const float x = acc[s + i / 2][(i & 1) * 2], y = acc[s + i / 2][(i & 1) * 2 + 1];
+        const half_t xh = (half_t)x, yh = (half_t)y;
+        ph[i] = pack2(xh, yh);
+        pl[i] = pack2((half_t)(x - (float)xh), (half_t)(y - (float)yh));
+      }
 #pragma unroll
-        for (int p = 0; p < PANELS; ++p) {
-          // eight keys' VE elements, 16 bits each
-          u32 x[8][VE / 2];
+      for (int p = 0; p < PANELS; ++p) {
+        // 4 SS keys' VE elements, 16 bits each
+        u32 x[4 * SS][VE / 2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const words<VW>& v = t.v[s * 4 + j][p];
+        for (int j = 0; j < 4 * SS; ++j) {
+          const words<VW>& v = t.v[s * 4 + j][p];
 #if EK_FP8
 #pragma unroll
-            for (int w = 0; w < VW; ++w) widen4(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
+          for (int w = 0; w < VW; ++w) widen4(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
 #else
 #pragma unroll
-            for (int w = 0; w < VW; ++w) x[j][w] = v.w[w];
+          for (int w = 0; w < VW; ++w) x[j][w] = v.w[w];
 #endif
-          }
+        }
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            u32 w[4];
+        for (int e = 0; e < VE; ++e) {
+          u32 w[2 * SS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
-                                           e & 1 ? 0x07060302u : 0x05040100u);
+          for (int i = 0; i < 2 * SS; ++i)
+            w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
+                                         e & 1 ? 0x07060302u : 0x05040100u);
+          if constexpr (SS == 2) {
             mma(o[p][e], w, ph);
             mma(o[p][e], w, pl);
+          } else {
+            mma16(o[p][e], w, ph);
+            mma16(o[p][e], w, pl);
           }
         }
       }
-#endif
-      if (next >= hi) break;
-      load_v(t, off);
-      base = next;
-      live = live_next;
     }
+#endif
+    if (next < hi) load_v(t, off);
+    live = live_next;
   }
 
-  // the four waves' parts of the chunk
   l = ek::reduce_xor<ek::Sum, 16>(l);
   l = ek::reduce_xor<ek::Sum, 32>(l);
-  if (c == 0) {
-    s_m[wave][r] = m - LIFT;
-    s_l[wave][r] = l;
-  }
+  if (r >= nh) return;
+  const int head = g * a.group + h0 + r;
+  if (chunks == 1) {
+    const bool any = l > 0.0f || l != l;
+    const float f = any ? a.v_scale / l : 0.0f;
+    T* dst = a.out + b * a.out_row + head * a.out_head;
 #pragma unroll
-  for (int p = 0; p < PANELS; ++p)
+    for (int p = 0; p < PANELS; ++p)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        const int d = p * 16 * VE + (c * 4 + i) * VE;
+        T y[VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) s_o[wave][r][p * 16 * VE + (c * 4 + i) * VE + e] = o[p][e][i];
-  __syncthreads();
-  const int total = nh * a.dim;
-  for (int x = threadIdx.x; x < total; x += 256) {
-    const int h = x / a.dim, d = x - h * a.dim;
-    float mm = s_m[0][h];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) mm = __builtin_fmaxf(mm, s_m[w][h]);
-    const float mu = mm == -__builtin_inff() ? 0.0f : mm;
-    float ll = 0.0f, oo = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float f = ek::exp2_fast(s_m[w][h] - mu);
-      ll += s_l[w][h] * f;
-      oo += s_o[w][h][d] * f;
-    }
-    const int head = g * a.group + h0 + h;
-    if (chunks == 1) {
-      const float y = ll > 0.0f || ll != ll ? oo / ll * a.v_scale : 0.0f;
-      a.out[b * a.out_row + head * a.out_head + d] = ek::cvt<T>(y);
-      if (a.lse && d == 0)
-        a.lse[(int64_t)b * a.heads + head] =
-            ll > 0.0f || ll != ll ? (mm + __builtin_log2f(ll)) * LN2 : -__builtin_inff();
-    } else {
-      float* dst = a.part + ((int64_t)blockIdx.x * a.heads + head) * (a.dim + 2);
-      dst[d] = oo;
-      if (d == 0) {
-        dst[a.dim] = mm;
-        dst[a.dim + 1] = ll;
+        for (int e = 0; e < VE; ++e) y[e] = ek::cvt<T>(any ? o[p][e][i] * f : 0.0f);
+        if (!EK_PAD || d < a.dim) ek::vstore_u<T, VE>(dst + d, y);
       }
+    if (a.lse && c == 0)
+      a.lse[(int64_t)b * a.heads + head] =
+          any ? (m - LIFT + __builtin_log2f(l)) * LN2 : -__builtin_inff();
+  } else {
+    const int64_t at = (int64_t)blockIdx.x * a.heads + head;
+    float* dst = a.part + at * a.dim;
+#pragma unroll
+    for (int p = 0; p < PANELS; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = p * 16 * VE + (c * 4 + i) * VE;
+        float y[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y[e] = o[p][e][i];
+        if (!EK_PAD || d < a.dim) {
+#pragma unroll
+          for (int e = 0; e < VE; e += 4) ek::vstore_u<float, 4>(dst + d + e, y + e);
+        }
+      }
+    if (c == 0) {
+      float* ml = a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim + at * 2;
+      ml[0] = m - LIFT;
+      ml[1] = l;
     }
   }
 }
 
-// One workgroup per sequence and query head: joins the chunks of a sequence that has several.
-extern "C" __global__ __launch_bounds__(256) void ek_paged_attention_join(Params a) {
-  __shared__ float s_o[WAVES][DP];
-  __shared__ float s_m[WAVES], s_l[WAVES];
+// Joins the chunks of the sequences that have several: `join_waves` waves for a sequence and
+// head, each with every join_waves-th chunk, joined once more through the LDS.
+extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Params a) {
+  __shared__ float s_o[16][DP];
+  __shared__ float s_m[16], s_l[16];
   const int lane = ek::lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.x, head = blockIdx.y;
-  const int per = chunk_units(a);
-  int start = 0, chunks = 0;
-  for (int base = 0; base <= b; base += 64) {
-    int f, n;
-    span_of(a, base + lane, f, n);
-    const int mine = chunks_of(units_of(n), per);
-    const int end = ek::wave_prefix_sum(mine);
-    const int at = b - base < 63 ? b - base : 63;
-    start += __builtin_amdgcn_readlane(end, at);
-    chunks = __builtin_amdgcn_readlane(mine, at);
-  }
-  start -= chunks;
-  if (chunks <= 1) return;
+  const int waves = a.join_waves, per_group = (blockDim.x >> 6) / waves;
+  const int sub = wave / waves, part = wave - sub * waves;
+  const int b = blockIdx.x, head = blockIdx.y * per_group + sub;
+  const float* ml = a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim;
+  const int32_t* info = (const int32_t*)(ml + (int64_t)(a.items + a.batch) * a.heads * 2);
+  const int start = info[2 * b], chunks = info[2 * b + 1];
+  if (chunks <= 1) return;           // all of the workgroup's waves: they share the sequence
+  const bool live = head < a.heads;
   float m = -__builtin_inff(), l = 0.0f, o[DP / 64];
 #pragma unroll
-  for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
-  for (int i = wave; i < chunks; i += WAVES) {
-    const float* src = a.part + ((int64_t)(start + i) * a.heads + head) * (a.dim + 2);
-    const float mi = src[a.dim], li = src[a.dim + 1];
-    const float m_new = __builtin_fmaxf(m, mi);
-    const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-    const float fa = ek::exp2_fast(m - mu), fb = ek::exp2_fast(mi - mu);
-    m = m_new;
-    l = l * fa + li * fb;
+  for (int k = 0; k < DP / 64; ++k) o[k] = 0.0f;
+  if (live) {
+    // 64 chunks at a time, a lane each: the largest m, then the chunks' weights
+    for (int i0 = part; i0 < chunks; i0 += 64 * waves) {
+      const int mine = i0 + lane * waves;
+      const int64_t at = (int64_t)(start + mine) * a.heads + head;
+      const int left = (chunks - i0 + waves - 1) / waves, count = left < 64 ? left : 64;
+      const float* src = a.part + ((int64_t)(start + i0) * a.heads + head) * a.dim;
+      const int64_t step = (int64_t)waves * a.heads * a.dim;
+      // eight rows on their way at once, the first ones beside m and l; past the last row, that
+      // one again, without weight
+      float v[8][DP / 64];
+      const auto load_rows = [&](int i) {
 #pragma unroll
-    for (int k = 0; k < DP / 64; ++k) {
-      const int d = k * 64 + lane;
-      if (!EK_PAD || d < a.dim) o[k] = o[k] * fa + src[d] * fb;
+        for (int j = 0; j < 8; ++j) {
+          const float* row = src + (i + j < count ? i + j : count - 1) * step;
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k) {
+            const int d = k * 64 + lane;
+            v[j][k] = !EK_PAD || d < a.dim ? row[d] : 0.0f;
+          }
+        }
+      };
+      load_rows(0);
+      const float mi = mine < chunks ? ml[at * 2] : -__builtin_inff();
+      const float li = mine < chunks ? ml[at * 2 + 1] : 0.0f;
+      const float mt = wave_all<ek::Max>(mi);
+      const float m_new = __builtin_fmaxf(m, mt);
+      const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+      const float fa = ek::exp2_fast(m - mu), fb = ek::exp2_fast(mi - mu);
+      m = m_new;
+      l = l * fa + wave_all<ek::Sum>(li * fb);
+#pragma unroll
+      for (int k = 0; k < DP / 64; ++k) o[k] *= fa;
+      for (int i = 0; i < count; i += 8) {
+        if (i > 0) load_rows(i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = __builtin_bit_cast(
+              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fb), (i + j) & 63));
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k)
+            o[k] = i + j < count ? __builtin_fmaf(v[j][k], w, o[k]) : o[k];
+        }
+      }
     }
   }
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_l[wave] = l;
-  }
-#pragma unroll
-  for (int k = 0; k < DP / 64; ++k) s_o[wave][k * 64 + lane] = o[k];
-  __syncthreads();
-  float mm = s_m[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) mm = __builtin_fmaxf(mm, s_m[w]);
-  const float mu = mm == -__builtin_inff() ? 0.0f : mm;
-  for (int d = threadIdx.x; d < a.dim; d += 256) {
-    float ll = 0.0f, oo = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float f = ek::exp2_fast(s_m[w] - mu);
-      ll += s_l[w] * f;
-      oo += s_o[w][d] * f;
+  if (waves > 1) {
+    if (lane == 0) {
+      s_m[wave] = m;
+      s_l[wave] = l;
     }
-    const bool any = ll > 0.0f || ll != ll;
-    a.out[b * a.out_row + head * a.out_head + d] =
-        ek::cvt<T>(any ? oo / ll * a.v_scale : 0.0f);
-    if (a.lse && d == 0)
-      a.lse[(int64_t)b * a.heads + head] =
-          any ? (mm + __builtin_log2f(ll)) * LN2 : -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < DP / 64; ++k) s_o[wave][k * 64 + lane] = o[k];
+    __syncthreads();
+    if (part != 0) return;
+    m = -__builtin_inff();
+    for (int w = 0; w < waves; ++w) m = __builtin_fmaxf(m, s_m[wave + w]);
+    const float mu = m == -__builtin_inff() ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DP / 64; ++k) o[k] = 0.0f;
+    for (int w = 0; w < waves; ++w) {
+      const float f = ek::exp2_fast(s_m[wave + w] - mu);
+      l += s_l[wave + w] * f;
+#pragma unroll
+      for (int k = 0; k < DP / 64; ++k) o[k] += s_o[wave + w][k * 64 + lane] * f;
+    }
   }
+  if (!live) return;
+  const bool any = l > 0.0f || l != l;
+  const float f = any ? a.v_scale / l : 0.0f;
+  T* dst = a.out + b * a.out_row + head * a.out_head;
+#pragma unroll
+  for (int k = 0; k < DP / 64; ++k) {
+    const int d = k * 64 + lane;
+    if (!EK_PAD || d < a.dim) dst[d] = ek::cvt<T>(any ? o[k] * f : 0.0f);
+  }
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)b * a.heads + head] =
+        any ? (m + __builtin_log2f(l)) * LN2 : -__builtin_inff();
 }

@@ -518,10 +518,11 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
 
 # -- attention over the cache ----------------------------------------------------------------
 
-_ATTEND = struct.Struct("<9q8iI3i3f4x")
-_UNIT = 64                          # tokens: what a sequence is split in multiples of
-_MIN_UNITS = 2
-_WORKGROUPS = 4                     # chunks of all sequences and key heads, per CU
+_ATTEND = struct.Struct("<9q8iI5i3f4x")
+_UNIT = 16                          # tokens: what a sequence is split in multiples of
+_MIN_UNITS = 4
+_STREAM = 256 << 20                # bytes of caches that do not stay in the last-level cache
+_WAVES = 12                         # chunks of all sequences and key heads, per CU
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float | None = None,
@@ -615,21 +616,24 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     most = -(-(min(window, capacity) if window else capacity) // _UNIT)
     group = heads // kv_heads
     y = kv_heads * (-(-group // 16))
-    items = max(1, min(_WORKGROUPS * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
+    items = max(1, min(_WAVES * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
               ("EK_PAD", int(dim != width)))
     log2e = 1.4426950408889634
-    launches = [("ek_paged_attention", (items + batch, y), 256)]
-    workspace = 0
+    launches = [("ek_paged_attention", (items + batch, y), 64)]
+    workspace, waves = 0, 1
     if most > _MIN_UNITS:              # some sequence may have more than one chunk
-        launches.append(("ek_paged_attention_join", (batch, heads), 256))
-        workspace = (items + batch) * heads * (dim + 2) * 4
+        waves = 16 if batch * heads <= 512 else 4 if batch * heads <= 2048 else 1
+        launches.append(("ek_paged_attention_join",
+                         (batch, heads if waves > 1 else -(-heads // 4)),
+                         64 * max(4, waves)))
+        workspace = (items + batch) * heads * (dim + 2) * 4 + batch * 8
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch, heads,
         group, dim, kc.shape[1], kc.shape[0], capacity, window, *_page_division(kc.shape[1]),
-        items, _MIN_UNITS, scale * k_scale * log2e, softcap * log2e, v_scale)
+        items, _MIN_UNITS, waves, int(2 * kc.span() > _STREAM), scale * k_scale * log2e, softcap * log2e, v_scale)
     if not workspace:
         tail = bytes(8) + tail         # the address of the partial results
     return _Plan("paged_attention.hip", macros, launches, arrays, {5, 6}, workspace, tail,
