@@ -41,16 +41,10 @@ typedef ek::bf16 T;
 constexpr int DP = EK_DP;
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
 constexpr float LN2 = 0.69314718055994531f;
-// Keys per wave and step.
-#ifndef EK_KT
-#define EK_KT 0
-#endif
-constexpr int KT0 = 4096 / (DP * CS);
-constexpr int KTMIN = 16;
-constexpr int KT = EK_KT ? EK_KT : KT0 < KTMIN ? KTMIN : KT0 > 64 ? 64 : KT0;
-#ifndef EK_OCC
-#define EK_OCC 2
-#endif
+// Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that.
+// (32 x 128 bf16, that is 16 KB, needs 177 registers instead of 125 and gains nothing: 64 ragged
+// sequences, 501 MB: 94.1 us with 16 keys, 94.9 with 32 at their best numbers of waves.)
+constexpr int KT = 4096 / (DP * CS) < 16 ? 16 : 4096 / (DP * CS) > 32 ? 32 : 4096 / (DP * CS);
 constexpr int ST = KT / 16;                         // score tiles
 constexpr int KE = 16 / CS;                         // elements of a 16-byte key load
 constexpr int KL = DP / (4 * KE);                   // key loads per score tile and lane
@@ -92,8 +86,9 @@ struct Params {
   int64_t table_row, lens_step;      // elements
   int32_t batch, heads, group, dim, page, pages, capacity, window;
   uint32_t page_mul;
-  int32_t page_shift, items, min_units, join_waves, stream;
-  float scale, cap, v_scale;         // scale includes log2(e); cap in the same unit, or 0
+  int32_t page_shift, items, min_units, stream;
+  uint32_t q_sign;                   // the sign bits of the queries' words, if scale is negative
+  float scale, cap, v_scale;         // scale > 0, with log2(e); cap in the same unit, or 0
 };
 
 EK_INLINE int page_of(const Params& a, int key) {
@@ -149,9 +144,7 @@ EK_INLINE Item find_item(const Params& a, int item) {
     total += units_of(count);
   }
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
-  // each sequence may take a chunk more than its share: kept within the items, if they are many
-  const int share = a.items > 2 * a.batch ? a.items - a.batch : (a.items + 1) / 2;
-  int per = (total + share - 1) / share;
+  int per = (total + a.items - 1) / a.items;
   per = per < a.min_units ? a.min_units : per;
 
   int before = 0;
@@ -274,7 +267,40 @@ struct Tile {
   words<VW> v[VR][PANELS];
 };
 
-extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Params a) {
+// A sequence's chunks are joined in groups of up to 16, or in 16 groups: its group size.
+EK_INLINE int group_of(int chunks) {
+  return chunks <= 256 ? (chunks < 16 ? chunks : 16) : (chunks + 15) / 16;
+}
+
+// A head's value: o f, rounded once to T.
+EK_INLINE T result(float o, float f, bool any) { return ek::cvt<T>(any ? o * f : 0.0f); }
+
+EK_INLINE float* part_ml(const Params& a) {
+  return a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim;
+}
+
+// The weights of up to 16 parts (m, l) of a head, one in each lane of a group of 16 (m -inf
+// where there is none): m and l become the whole's, in all 16 lanes.
+EK_INLINE float weigh16(float& m, float& l) {
+  const float mine = m;
+  m = ek::reduce_xor<ek::Max, 1>(m);
+  m = ek::reduce_xor<ek::Max, 2>(m);
+  m = ek::reduce_xor<ek::Max, 4>(m);
+  m = ek::reduce_xor<ek::Max, 8>(m);
+  const float w = ek::exp2_fast(mine - (m == -__builtin_inff() ? 0.0f : m));
+  l *= w;
+  l = ek::reduce_xor<ek::Sum, 1>(l);
+  l = ek::reduce_xor<ek::Sum, 2>(l);
+  l = ek::reduce_xor<ek::Sum, 4>(l);
+  l = ek::reduce_xor<ek::Sum, 8>(l);
+  return w;
+}
+
+EK_INLINE float lane_value(float x, int lane) {
+  return ek::bits_f32((u32)__builtin_amdgcn_readlane((int)ek::f32_bits(x), lane));
+}
+
+extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void ek_paged_attention(Params a) {
   const int lane = ek::lane_id(), r = lane & 15, c = lane >> 4;
   const int tiles16 = (a.group + 15) / 16;
   const int g = blockIdx.y / tiles16, h0 = (blockIdx.y - g * tiles16) * 16;
@@ -318,7 +344,7 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = s * 16 + c * 4 + i;
-        q.w[s][i] = head && d < a.dim ? src[d] : 0.0f;
+        q.w[s][i] = head && d < a.dim ? ek::bits_f32(ek::f32_bits(src[d]) ^ a.q_sign) : 0.0f;
       }
 #else
 #pragma unroll
@@ -329,12 +355,14 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
         words<4> x = {{0, 0, 0, 0}};
         if (head && d < a.dim) x = load_words<4>((const char*)(src + d));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.w[s * (KE / 8) + e][i] = x.w[i];
+        for (int i = 0; i < 4; ++i) q.w[s * (KE / 8) + e][i] = x.w[i] ^ a.q_sign;
       }
 #endif
   }
 
-  const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+  // what the scores are multiplied by for exp2: positive, since the queries took the sign
+  const float to_cap = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
+  const float scale = a.cap > 0.0f ? 1.0f : a.scale;
   float m = -__builtin_inff(), l = 0.0f;
   ek::f32x4 o[PANELS][VE];
 #pragma unroll
@@ -424,21 +452,29 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
       id = page_id(next + KT);
       load_k(t, off);
     }
-    // softmax
-    float mt = -__builtin_inff();
+    // softmax: scores stay as the product gave them (or capped, in log2 units) until exp2, whose
+    // argument is one fma of them; m is in log2 units
     const bool full = live == ~0ull;
+    if (a.cap > 0.0f) {
+#pragma unroll
+      for (int s = 0; s < ST; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[s][i] = a.cap * tanh_f(acc[s][i] * to_cap);
+    }
+    if (!full) {
+#pragma unroll
+      for (int s = 0; s < ST; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[s][i] = live >> (s * 16 + c * 4 + i) & 1 ? acc[s][i] : -__builtin_inff();
+    }
+    float mt = -__builtin_inff();
 #pragma unroll
     for (int s = 0; s < ST; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = acc[s][i] * a.scale;
-        if (a.cap > 0.0f) x = a.cap * tanh_f(x * inv_cap);
-        if (!full && !(live >> (s * 16 + c * 4 + i) & 1)) x = -__builtin_inff();
-        acc[s][i] = x;
-        mt = __builtin_fmaxf(mt, x);
-      }
+      for (int i = 0; i < 4; ++i) mt = __builtin_fmaxf(mt, acc[s][i]);
     mt = ek::reduce_xor<ek::Max, 16>(mt);
-    mt = ek::reduce_xor<ek::Max, 32>(mt);
+    mt = ek::reduce_xor<ek::Max, 32>(mt) * scale;
     const float m_new = __builtin_fmaxf(m, mt);
     const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
     const float alpha = ek::exp2_fast(m - m_use);
@@ -455,7 +491,7 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
     for (int s = 0; s < ST; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        acc[s][i] = ek::exp2_fast(acc[s][i] - (m_use - LIFT));
+        acc[s][i] = ek::exp2_fast(__builtin_fmaf(acc[s][i], scale, LIFT - m_use));
         l += acc[s][i];
       }
     // values without a key are taken as zeros: their memory may hold anything
@@ -542,7 +578,7 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
         const int d = p * 16 * VE + (c * 4 + i) * VE;
         T y[VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) y[e] = ek::cvt<T>(any ? o[p][e][i] * f : 0.0f);
+        for (int e = 0; e < VE; ++e) y[e] = result(o[p][e][i], f, any);
         if (!EK_PAD || d < a.dim) ek::vstore_u<T, VE>(dst + d, y);
       }
     if (a.lse && c == 0)
@@ -565,106 +601,120 @@ extern "C" __global__ __launch_bounds__(64, EK_OCC) void ek_paged_attention(Para
         }
       }
     if (c == 0) {
-      float* ml = a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim + at * 2;
+      float* ml = part_ml(a) + at * 2;
       ml[0] = m - LIFT;
       ml[1] = l;
     }
   }
 }
 
-// Joins the chunks of the sequences that have several: `join_waves` waves for a sequence and
-// head, each with every join_waves-th chunk, joined once more through the LDS.
+// Joins the chunks of a sequence that has several, for one head: a wave per group, then the
+// groups.
 extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Params a) {
+  constexpr int DW = (DP + 127) / 128;
   __shared__ float s_o[16][DP];
   __shared__ float s_m[16], s_l[16];
   const int lane = ek::lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = a.join_waves, per_group = (blockDim.x >> 6) / waves;
-  const int sub = wave / waves, part = wave - sub * waves;
-  const int b = blockIdx.x, head = blockIdx.y * per_group + sub;
-  const float* ml = a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim;
+  const int waves = blockDim.x >> 6, b = blockIdx.x, head = blockIdx.y;
+  const float* ml = part_ml(a);
   const int32_t* info = (const int32_t*)(ml + (int64_t)(a.items + a.batch) * a.heads * 2);
   const int start = info[2 * b], chunks = info[2 * b + 1];
-  if (chunks <= 1) return;           // all of the workgroup's waves: they share the sequence
-  const bool live = head < a.heads;
-  float m = -__builtin_inff(), l = 0.0f, o[DP / 64];
+  if (chunks <= 1) return;
+  const int gs = group_of(chunks), groups = (chunks + gs - 1) / gs;
+  float x[DW][2];
+  for (int group = wave; group < groups; group += waves) {
+    const int begin = start + group * gs;
+    const int size = chunks - group * gs < gs ? chunks - group * gs : gs;
+    float mm = -__builtin_inff(), ll = 0.0f;
 #pragma unroll
-  for (int k = 0; k < DP / 64; ++k) o[k] = 0.0f;
-  if (live) {
-    // 64 chunks at a time, a lane each: the largest m, then the chunks' weights
-    for (int i0 = part; i0 < chunks; i0 += 64 * waves) {
-      const int mine = i0 + lane * waves;
-      const int64_t at = (int64_t)(start + mine) * a.heads + head;
-      const int left = (chunks - i0 + waves - 1) / waves, count = left < 64 ? left : 64;
-      const float* src = a.part + ((int64_t)(start + i0) * a.heads + head) * a.dim;
-      const int64_t step = (int64_t)waves * a.heads * a.dim;
-      // eight rows on their way at once, the first ones beside m and l; past the last row, that
-      // one again, without weight
-      float v[8][DP / 64];
-      const auto load_rows = [&](int i) {
+    for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
+    for (int i0 = 0; i0 < size; i0 += 16) {
+      const int count = size - i0 < 16 ? size - i0 : 16, i = lane & 15;
+      float m = -__builtin_inff(), l = 0.0f;
+      if (i < count) {
+        m = ml[((int64_t)(begin + i0 + i) * a.heads + head) * 2];
+        l = ml[((int64_t)(begin + i0 + i) * a.heads + head) * 2 + 1];
+      }
+      float v[16][DW][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float* row = src + (i + j < count ? i + j : count - 1) * step;
+      for (int j = 0; j < 16; ++j)
 #pragma unroll
-          for (int k = 0; k < DP / 64; ++k) {
-            const int d = k * 64 + lane;
-            v[j][k] = !EK_PAD || d < a.dim ? row[d] : 0.0f;
-          }
+        for (int k = 0; k < DW; ++k) {
+          const int d = k * 128 + lane * 2;
+          v[j][k][0] = v[j][k][1] = 0.0f;
+          if (j < count && d < a.dim)
+            ek::vload_u<float, 2>(v[j][k],
+                                  a.part + ((int64_t)(begin + i0 + j) * a.heads + head) * a.dim + d);
         }
-      };
-      load_rows(0);
-      const float mi = mine < chunks ? ml[at * 2] : -__builtin_inff();
-      const float li = mine < chunks ? ml[at * 2 + 1] : 0.0f;
-      const float mt = wave_all<ek::Max>(mi);
-      const float m_new = __builtin_fmaxf(m, mt);
-      const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-      const float fa = ek::exp2_fast(m - mu), fb = ek::exp2_fast(mi - mu);
-      m = m_new;
-      l = l * fa + wave_all<ek::Sum>(li * fb);
+      float w = weigh16(m, l), f = 0.0f;
+      if (i0 > 0) {                    // more than 16 chunks: onto what came before
+        const float m_new = __builtin_fmaxf(mm, m);
+        const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+        f = ek::exp2_fast(mm - mu);
+        const float part = ek::exp2_fast(m - mu);
+        w *= part;
+        l = __builtin_fmaf(ll, f, l * part);
+        m = m_new;
 #pragma unroll
-      for (int k = 0; k < DP / 64; ++k) o[k] *= fa;
-      for (int i = 0; i < count; i += 8) {
-        if (i > 0) load_rows(i);
+        for (int k = 0; k < DW; ++k) x[k][0] *= f, x[k][1] *= f;
+      }
+      mm = m;
+      ll = l;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = __builtin_bit_cast(
-              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fb), (i + j) & 63));
+      for (int j = 0; j < 16; ++j) {
+        const float y = lane_value(w, j);
 #pragma unroll
-          for (int k = 0; k < DP / 64; ++k)
-            o[k] = i + j < count ? __builtin_fmaf(v[j][k], w, o[k]) : o[k];
+        for (int k = 0; k < DW; ++k) {
+          x[k][0] = j < count ? __builtin_fmaf(v[j][k][0], y, x[k][0]) : x[k][0];
+          x[k][1] = j < count ? __builtin_fmaf(v[j][k][1], y, x[k][1]) : x[k][1];
+        }
+      }
+    }
+    if (lane == 0) {
+      s_m[group] = lane_value(mm, 0);
+      s_l[group] = lane_value(ll, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < DW; ++k) {
+      const int d = k * 128 + lane * 2;
+      if (d < DP) {
+        s_o[group][d] = x[k][0];
+        s_o[group][d + 1] = x[k][1];
+      }
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  float m = (lane & 15) < groups ? s_m[lane & 15] : -__builtin_inff();
+  float l = (lane & 15) < groups ? s_l[lane & 15] : 0.0f;
+  if (groups > 1) {
+    const float w = weigh16(m, l);
+#pragma unroll
+    for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
+    for (int j = 0; j < groups; ++j) {
+      const float f = lane_value(w, j);
+#pragma unroll
+      for (int k = 0; k < DW; ++k) {
+        const int d = k * 128 + lane * 2;
+        if (d < DP) {
+          x[k][0] = __builtin_fmaf(s_o[j][d], f, x[k][0]);
+          x[k][1] = __builtin_fmaf(s_o[j][d + 1], f, x[k][1]);
         }
       }
     }
   }
-  if (waves > 1) {
-    if (lane == 0) {
-      s_m[wave] = m;
-      s_l[wave] = l;
-    }
-#pragma unroll
-    for (int k = 0; k < DP / 64; ++k) s_o[wave][k * 64 + lane] = o[k];
-    __syncthreads();
-    if (part != 0) return;
-    m = -__builtin_inff();
-    for (int w = 0; w < waves; ++w) m = __builtin_fmaxf(m, s_m[wave + w]);
-    const float mu = m == -__builtin_inff() ? 0.0f : m;
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < DP / 64; ++k) o[k] = 0.0f;
-    for (int w = 0; w < waves; ++w) {
-      const float f = ek::exp2_fast(s_m[wave + w] - mu);
-      l += s_l[wave + w] * f;
-#pragma unroll
-      for (int k = 0; k < DP / 64; ++k) o[k] += s_o[wave + w][k * 64 + lane] * f;
-    }
-  }
-  if (!live) return;
+  m = lane_value(m, 0);
+  l = lane_value(l, 0);
   const bool any = l > 0.0f || l != l;
   const float f = any ? a.v_scale / l : 0.0f;
   T* dst = a.out + b * a.out_row + head * a.out_head;
 #pragma unroll
-  for (int k = 0; k < DP / 64; ++k) {
-    const int d = k * 64 + lane;
-    if (!EK_PAD || d < a.dim) dst[d] = ek::cvt<T>(any ? o[k] * f : 0.0f);
+  for (int k = 0; k < DW; ++k) {
+    const int d = k * 128 + lane * 2;
+    if (d < a.dim) {
+      T y[2] = {result(x[k][0], f, any), result(x[k][1], f, any)};
+      ek::vstore_u<T, 2>(dst + d, y);
+    }
   }
   if (a.lse && lane == 0)
     a.lse[(int64_t)b * a.heads + head] =

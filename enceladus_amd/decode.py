@@ -518,11 +518,14 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
 
 # -- attention over the cache ----------------------------------------------------------------
 
-_ATTEND = struct.Struct("<9q8iI5i3f4x")
+_ATTEND = struct.Struct("<9q8iI4iI3f4x")
 _UNIT = 16                          # tokens: what a sequence is split in multiples of
-_MIN_UNITS = 4
+_MIN_UNITS = 4                      # of a chunk
 _STREAM = 256 << 20                # bytes of caches that do not stay in the last-level cache
-_WAVES = 12                         # chunks of all sequences and key heads, per CU
+# Chunks of all sequences and key heads, per CU, by the bytes of a cached element: as many as keep
+# 64 KB on their way into a CU at once. More of them leave more partial results (one sequence of
+# 131075, fp16: 94.8 us with 8, 102.3 with 16), fewer leave loads out (100.4 with 6).
+_WAVES = {1: 10, 2: 8, 4: 6}
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float | None = None,
@@ -616,24 +619,26 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     most = -(-(min(window, capacity) if window else capacity) // _UNIT)
     group = heads // kv_heads
     y = kv_heads * (-(-group // 16))
-    items = max(1, min(_WAVES * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
+    items = max(1, min(_WAVES[kc.size] * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
               ("EK_PAD", int(dim != width)))
     log2e = 1.4426950408889634
     launches = [("ek_paged_attention", (items + batch, y), 64)]
-    workspace, waves = 0, 1
+    workspace = 0
     if most > _MIN_UNITS:              # some sequence may have more than one chunk
-        waves = 16 if batch * heads <= 512 else 4 if batch * heads <= 2048 else 1
-        launches.append(("ek_paged_attention_join",
-                         (batch, heads if waves > 1 else -(-heads // 4)),
-                         64 * max(4, waves)))
         workspace = (items + batch) * heads * (dim + 2) * 4 + batch * 8
+        chunks = min(items, -(-most // _MIN_UNITS))
+        launches.append(("ek_paged_attention_join", (batch, heads),
+                         64 * min(16, max(4, -(-chunks // 16)))))
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch, heads,
         group, dim, kc.shape[1], kc.shape[0], capacity, window, *_page_division(kc.shape[1]),
-        items, _MIN_UNITS, waves, int(2 * kc.span() > _STREAM), scale * k_scale * log2e, softcap * log2e, v_scale)
+        items, _MIN_UNITS, int(2 * kc.span() > _STREAM),
+        0 if scale >= 0 else 0x80000000 if qa.kind == "fp32" else 0x80008000,
+        # so small a scale is as good as none, and keeps -inf (no key there) what it is
+        max(abs(scale) * k_scale * log2e, 2.0 ** -126), softcap * log2e, v_scale)
     if not workspace:
         tail = bytes(8) + tail         # the address of the partial results
     return _Plan("paged_attention.hip", macros, launches, arrays, {5, 6}, workspace, tail,
