@@ -650,6 +650,17 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
 _LOGITS = struct.Struct("<12q3i4f4x")
 
 
+MAX_BIASES = 1023                   # per row: 10 bits of a logit's word
+MAX_HISTORY = (1 << 21) - 1         # per row: 21 bits
+
+
+def _stretch(rows: int, vocab: int) -> int:
+    """Logits per workgroup (of 512 threads): the longer stretch, which reads a history fewer
+    times, unless that leaves CUs without a workgroup (256 x 128000 bf16, histories of up to 4096:
+    44 us with 4096, 34 with 8192; one row of 32000 fp32, 20000 tokens: 6.0 and 6.9)."""
+    return 4096 if rows * -(-vocab // 8192) < C.coarsen_cap() else 8192
+
+
 def _per_row(name: str, x, rows: int, default: float):
     """(array or None, number) of a per-row setting given as a number or an array."""
     if x is None:
@@ -676,12 +687,13 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
 
     Args:
         logits: `[rows, vocabulary]`, float32, float16 or bfloat16.
-        tokens: the history, int32 `[rows, length]`; ids outside the vocabulary are ignored.
+        tokens: the history, int32 `[rows, length]`, shorter than 2^21; ids outside the
+            vocabulary are ignored.
         token_lens: how much of each row of `tokens` counts, int32 `[rows]`; all without it.
         prompt_lens: how much of that is the prompt, int32 `[rows]`; none without it.
         repetition, frequency, presence, temperature: a number, or float32 `[rows]`.
-        bias_ids, bias: int32 and float32 `[rows, entries]`; ids outside the vocabulary are
-            ignored, entries with the same id add up in their order.
+        bias_ids, bias: int32 and float32 `[rows, entries]`, at most 1023 entries; ids outside
+            the vocabulary are ignored, entries with the same id add up in their order.
         allowed: int32 `[rows, words]`, 32 tokens to a word: token t is bit t % 32 of word
             t // 32. One mask for all rows is an expanded array.
         out: where the result goes (`logits` itself will do); new without it.
@@ -765,11 +777,13 @@ def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency,
     _need(vocab < 1 << 30 and rows * vocab < 1 << 41,
           f"logits of shape {la.shape} are too large for one call")
     biases = ia.shape[1] if ia else 0
-    n, threads = (2048, 128) if rows * vocab < 1 << 21 else (8192, 256)
-    if la.kind == "fp32" and n == 2048:
-        threads = 256
-    macros = (("EK_Q", _Q[la.kind]), ("EK_N", n), ("EK_THREADS", threads),
-              ("EK_BIAS", int(biases > 0)))
+    _need(biases <= MAX_BIASES, f"at most {MAX_BIASES} biases of a row are supported, got "
+                                f"{biases}")
+    _need(ta is None or ta.shape[1] <= MAX_HISTORY,
+          f"at most {MAX_HISTORY} tokens of history are supported, got "
+          f"{ta.shape[1] if ta else 0}")
+    n = _stretch(rows, vocab)
+    macros = (("EK_Q", _Q[la.kind]), ("EK_N", n))
 
     def step(a):
         return a.strides[0] if a is not None else 0
@@ -778,7 +792,7 @@ def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency,
                         step(pl), step(rep_a), step(freq_a), step(pres_a), step(temp_a), vocab,
                         ta.shape[1] if ta else 0, biases, rep, freq, pres, temp)
     return _Plan("adjust_logits.hip", macros,
-                 [("ek_adjust_logits", (-(-vocab // n) * rows, 1), threads)], arrays, {1}, 0,
+                 [("ek_adjust_logits", (-(-vocab // n) * rows, 1), 512)], arrays, {1}, 0,
                  tail, [(1, 0, True)] + [(1, i, False) for i in range(2, 12)]), out
 
 
@@ -793,7 +807,5 @@ def specializations():
             yield "append_kv.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_V", 8 if q else 4),
                                     ("EK_PAIRS", pairs))
     for q in (0, 1, 2):
-        for n, threads in ((2048, 128 if q else 256), (8192, 256)):
-            for bias in (0, 1):
-                yield "adjust_logits.hip", (("EK_Q", q), ("EK_N", n), ("EK_THREADS", threads),
-                                            ("EK_BIAS", bias))
+        for n in (4096, 8192):
+            yield "adjust_logits.hip", (("EK_Q", q), ("EK_N", n))
