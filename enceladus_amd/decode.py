@@ -200,6 +200,8 @@ class _Cuda:
         if hasattr(torch._C, "_cuda_getDevice") and torch.cuda.is_initialized():
             self.here = torch._C._cuda_getDevice
         self.empty, self.uint8 = torch.empty, torch.uint8
+        self.empty_like, self.dense = torch.empty_like, torch.contiguous_format
+        self.tensor = torch.Tensor
         self.launch_list = hip.load_library().ek_launch_list
         return self.__dict__[name]
 
@@ -220,8 +222,14 @@ def _keep(key, plan) -> None:
 
 
 def _of(x):
-    """What a plan depends on of an optional array."""
-    return None if x is None else (x.dtype, x.shape, x.stride(), x.get_device())
+    """What a plan depends on of an array on a GPU."""
+    return x.dtype, x.shape, x.stride(), x.get_device()
+
+
+def _like(x):
+    """A new dense array of x's kind, shape, type and device."""
+    return _cuda.empty_like(x, memory_format=_cuda.dense) if x.__class__ is _cuda.tensor else \
+        T.new_empty(x)
 
 
 # -- arguments ---------------------------------------------------------------------------
@@ -372,10 +380,8 @@ def _head_dim(dim: int, cache: str) -> None:
           f"{MAX_HEAD_DIM}, got {dim}")
 
 
-def _scale_arg(name: str, x) -> float:
-    x = float(x)
+def _positive(name: str, x: float) -> None:
     _need(math.isfinite(x) and x > 0, f"`{name}` must be a positive number, got {x}")
-    return x
 
 
 # -- appending to the cache ----------------------------------------------------------------
@@ -425,12 +431,21 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     Returns:
         The rotated queries, or None without `q`.
     """
+    # plain numbers from here on: a plan is kept by their values
+    interleaved, k_scale, v_scale = bool(interleaved), float(k_scale), float(v_scale)
     try:
         key = (0, k.dtype, k.shape, k.stride(), k.get_device(), v.dtype, v.shape, v.stride(),
                v.get_device(), k_cache.dtype, k_cache.shape, k_cache.stride(),
                k_cache.get_device(), v_cache.dtype, v_cache.shape, v_cache.stride(),
-               v_cache.get_device(), _of(block_table), _of(seq_lens), _of(cu_tokens), _of(q),
-               _of(q_out), _of(cos), _of(sin), interleaved, k_scale, v_scale)
+               v_cache.get_device(), block_table.dtype, block_table.shape,
+               block_table.stride(), block_table.get_device(), seq_lens.dtype, seq_lens.shape,
+               seq_lens.stride(), seq_lens.get_device(),
+               None if cu_tokens is None else _of(cu_tokens),
+               None if q is None else (q.dtype, q.shape, q.stride(), q.get_device()),
+               None if q_out is None else _of(q_out),
+               None if cos is None else (cos.dtype, cos.shape, cos.stride(), cos.get_device()),
+               None if sin is None else (sin.dtype, sin.shape, sin.stride(), sin.get_device()),
+               interleaved, k_scale, v_scale)
         plan = _plans.get(key)
     except (AttributeError, TypeError):
         key = plan = None              # arrays of another kind, or no arrays
@@ -442,7 +457,7 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
             return q_out
         _keep(key, plan)
     elif q is not None and not given:
-        q_out = T.new_empty(q)
+        q_out = _like(q)
     arrays = [q, k, v, q_out, k_cache, v_cache, block_table, seq_lens, cu_tokens, cos, sin]
     if given:
         plan.check_apart(arrays)
@@ -487,7 +502,8 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         sa = _array("sin", sin, ("fp32",), 2, ca.shape)
         rotary = 2 * ca.shape[1]
         _need(0 < rotary <= dim, f"`cos` rotates {rotary} elements of heads of {dim}")
-    k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
+    _positive("k_scale", k_scale)
+    _positive("v_scale", v_scale)
     arrays = [("q", qa), ("k", ka), ("v", va), ("q_out", qo), ("k_cache", kc), ("v_cache", vc),
               ("block_table", bt), ("seq_lens", sl), ("cu_tokens", cu), ("cos", ca),
               ("sin", sa)]
@@ -559,11 +575,17 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
         The result, `[batch, heads, dim]` of the type of `q`; `(result, lse)` when
         `return_lse`.
     """
+    # plain numbers from here on: a plan is kept by their values
+    scale = None if scale is None else float(scale)
+    window, softcap = operator.index(window), float(softcap)
+    k_scale, v_scale = float(k_scale), float(v_scale)
     try:
         key = (1, q.dtype, q.shape, q.stride(), q.get_device(), k_cache.dtype, k_cache.shape,
                k_cache.stride(), k_cache.get_device(), v_cache.dtype, v_cache.shape,
-               v_cache.stride(), v_cache.get_device(), _of(block_table), _of(seq_lens),
-               _of(out), scale, window, type(window), softcap, k_scale, v_scale)
+               v_cache.stride(), v_cache.get_device(), block_table.dtype, block_table.shape,
+               block_table.stride(), block_table.get_device(), seq_lens.dtype, seq_lens.shape,
+               seq_lens.stride(), seq_lens.get_device(), None if out is None else _of(out),
+               scale, window, softcap, k_scale, v_scale)
         plan = _plans.get(key)
     except (AttributeError, TypeError):
         key = plan = None              # arrays of another kind, or no arrays
@@ -574,7 +596,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
         if plan is not None:
             _keep(key, plan)
     elif not given:
-        out = T.new_empty(q)
+        out = _like(q)
     lse = T.new_empty(q, tuple(q.shape[:2]), np.float32) if return_lse else None
     if plan is not None:
         arrays = [q, k_cache, v_cache, block_table, seq_lens, out, lse]
@@ -598,12 +620,12 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     _need(heads <= 65535, f"at most 65535 query heads are supported, got {heads}")
     bt, sl = _sequences(block_table, seq_lens, batch)
     capacity = _capacity(bt, kc)
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(dim) if scale is None else scale
     _need(math.isfinite(scale), f"`scale` must be finite, got {scale}")
-    softcap, window = float(softcap), operator.index(window)
     _need(math.isfinite(softcap) and softcap >= 0, f"`softcap` must be at least 0, got {softcap}")
     _need(window >= 0, f"`window` must be at least 0, got {window}")
-    k_scale, v_scale = _scale_arg("k_scale", k_scale), _scale_arg("v_scale", v_scale)
+    _positive("k_scale", k_scale)
+    _positive("v_scale", v_scale)
     if out is None:
         out = T.new_empty(q)
     oa = _array("out", out, (qa.kind,), 3, qa.shape)
@@ -629,8 +651,9 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     if most > _MIN_UNITS:              # some sequence may have more than one chunk
         workspace = (items + batch) * heads * (dim + 2) * 4 + batch * 8
         chunks = min(items, -(-most // _MIN_UNITS))
-        launches.append(("ek_paged_attention_join", (batch, heads),
-                         64 * min(16, max(4, -(-chunks // 16)))))
+        # A wave per 16 chunks; where there are many sequences, few of them have many.
+        waves = max(4, min(16, -(-chunks // 16), 8192 // (batch * heads)))
+        launches.append(("ek_paged_attention_join", (batch, heads), 64 * waves))
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], batch, heads,
@@ -702,10 +725,11 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
         The adjusted logits, of the type of `logits`.
     """
     try:
-        key = (2, logits.dtype, logits.shape, logits.stride(), logits.get_device(), _of(tokens),
-               _of(token_lens), _of(prompt_lens), _number_or(repetition), _number_or(frequency),
-               _number_or(presence), _number_or(temperature), _of(bias_ids), _of(bias),
-               _of(allowed), _of(out))
+        key = (2, logits.dtype, logits.shape, logits.stride(), logits.get_device(),
+               *[x if x is None or x.__class__ in _NUMBERS else
+                 (x.dtype, x.shape, x.stride(), x.get_device())
+                 for x in (tokens, token_lens, prompt_lens, repetition, frequency, presence,
+                           temperature, bias_ids, bias, allowed, out)])
         plan = _plans.get(key)
     except (AttributeError, TypeError):
         key = plan = None              # arrays of another kind, or no arrays
@@ -717,10 +741,11 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
             return out
         _keep(key, plan)
     elif not given:
-        out = T.new_empty(logits)
+        out = _like(logits)
     arrays = [logits, out, tokens, token_lens, prompt_lens,
-              *(x if hasattr(x, "shape") else None
-                for x in (repetition, frequency, presence, temperature)),
+              *[None if x is None or x.__class__ in _NUMBERS or not
+                (key is not None or T.is_array_like(x)) else x
+                for x in (repetition, frequency, presence, temperature)],
               bias_ids, bias, allowed]
     if given:
         plan.check_apart(arrays)
@@ -728,8 +753,7 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
     return out
 
 
-def _number_or(x):
-    return _of(x) if hasattr(x, "stride") else x
+_NUMBERS = (float, int)
 
 
 def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency, presence,

@@ -209,3 +209,17 @@ def test_module_is_public():
     assert enceladus.decode is decode
     for name in decode.__all__:
         assert getattr(decode, name).__doc__
+
+
+def test_settings_of_any_number_type():
+    """NumPy scalars and tensors of one value count as numbers; a tensor's later value is seen."""
+    for one in (1, True, np.float32(1.0), torch.tensor(1.0), torch.tensor(0.5)):
+        *args, _ = _attend(q=torch.zeros(3, 7, 64))
+        with pytest.raises(ValueError, match="not a multiple"):
+            decode.paged_attention(*args, scale=one, k_scale=one)
+        with pytest.raises(TypeError, match="`logits`"):
+            decode.adjust_logits(torch.zeros(3, 10, dtype=torch.int8),
+                                 temperature=one if one.__class__ is not torch.Tensor else 1)
+    *args, _ = _attend()
+    with pytest.raises(ValueError, match="k_scale"):
+        decode.paged_attention(*args, k_scale=torch.tensor(-1.0))

@@ -681,3 +681,26 @@ def test_calls_are_timed_and_traced(tmp_path):
     with enceladus.capture(path):
         decode.adjust_logits(**g)
     assert "ek_adjust_logits" in path.read_text()
+
+
+def test_settings_by_their_values():
+    """A setting given as a tensor or a NumPy scalar counts with the value that it has at the
+    call: a plan made before is not taken for the object's sake."""
+    gen = torch.Generator().manual_seed(70)
+    lens = [50, 9]
+    bt, pages = table_for(gen, lens, 16)
+    kc, vc = (cache(gen, pages, 16, 1, 64, F32).cuda() for _ in "kv")
+    q = rand(gen, 2, 2, 64).cuda()
+    args = q, kc, vc, bt.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    scale = torch.tensor(0.25)
+    a = decode.paged_attention(*args, scale=scale)
+    scale.fill_(0.5)
+    b = decode.paged_attention(*args, scale=scale)
+    assert torch.equal(a, decode.paged_attention(*args, scale=0.25))
+    assert torch.equal(b, decode.paged_attention(*args, scale=np.float32(0.5)))
+    assert not torch.equal(a, b)
+    x, tokens = rand(gen, 2, 100).cuda(), torch.tensor([[3, 4], [5, 6]], dtype=torch.int32).cuda()
+    for _ in range(2):
+        a = decode.adjust_logits(x, tokens=tokens, repetition=np.float32(1.5), presence=1)
+        b = decode.adjust_logits(x, tokens=tokens, repetition=1.5, presence=True)
+        assert torch.equal(a, b)
