@@ -51,8 +51,8 @@ struct Params {
 
 extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a) {
   __shared__ __attribute__((aligned(16))) uint32_t s_mark[N];
-  __shared__ int32_t s_id[MOST_BIASES + 1];
-  __shared__ float s_bias[MOST_BIASES + 1];
+  __shared__ __attribute__((aligned(16))) int32_t s_id[MOST_BIASES + 1];
+  __shared__ __attribute__((aligned(16))) float s_bias[MOST_BIASES + 1];
   const int stretches = (a.vocab + N - 1) / N, tid = threadIdx.x;
   const int64_t b = blockIdx.x / stretches;
   const int v0 = (int)(blockIdx.x - b * stretches) * N;
@@ -109,6 +109,7 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
       s_id[tid] = bias_id;
       s_bias[tid] = bias;
     }
+    if (tid < (-a.biases & 3)) s_id[a.biases + tid] = -1;    // up to whole vectors
     for (int i = tid + THREADS; i < a.biases; i += THREADS) {
       s_id[i] = a.bias_ids[b * a.id_row + i];
       s_bias[i] = a.bias[b * a.bias_row + i];
@@ -173,9 +174,21 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
       bool first = true;
       sum[k] = s_bias[i];
       if (entries > 1) {
-        for (int j = 0; j < i; ++j) first &= s_id[j] != s_id[i];
-        for (int j = i + 1; first && j < a.biases; ++j)
-          if (s_id[j] == s_id[i]) sum[k] += s_bias[j];
+        const int32_t id = s_id[i];
+        sum[k] = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < a.biases; j += 4) {
+          int32_t ids4[4];
+          float bias4[4];
+          ek::vload<int32_t, 4>(ids4, s_id + j);
+          ek::vload<float, 4>(bias4, s_bias + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool same = ids4[e] == id;
+            first &= !(same && j + e < i);
+            sum[k] = same ? sum[k] + bias4[e] : sum[k];
+          }
+        }
       }
       if (first) change[k] = ((uint32_t)(i + 1) - entries) << ENTRY;
       else at[k] = ~0u;

@@ -262,6 +262,8 @@ struct Query {
 #endif
 };
 
+__device__ const u32 s_zeros[4] = {0, 0, 0, 0};
+
 struct Tile {
   words<4> k[ST][KL];
   words<VW> v[VR][PANELS];
@@ -334,30 +336,27 @@ extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void
   const char* vbase = a.v + g * a.c_head;
   const int32_t* row = a.table + b * a.table_row;
 
+  // Loads first, without branches between them, then zeros for heads and elements that are not
+  // there: a wait per load would cost a latency each.
   Query q;
   {
-    const T* src = a.q + b * a.q_row + (int64_t)(g * a.group + h0 + r) * a.q_head;
-    const bool head = r < nh;
-#if EK_Q == 0
+    const T* src = a.q + b * a.q_row +
+                   (int64_t)(g * a.group + h0 + (r < nh ? r : 0)) * a.q_head;
+    constexpr int QN = sizeof(q.w) / 16, QE = 16 / sizeof(T);
+    const auto place = [&](int i) {
+      return EK_Q == 0 ? (i * 4 + c) * 4 : (i / (KE / QE) * 4 + c) * KE + i % (KE / QE) * 8;
+    };
+    words<4> x[QN];
 #pragma unroll
-    for (int s = 0; s < KL; ++s)
+    for (int i = 0; i < QN; ++i)
+      x[i] = load_words<4>((const char*)(src + (place(i) < a.dim ? place(i) : 0)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = s * 16 + c * 4 + i;
-        q.w[s][i] = head && d < a.dim ? ek::bits_f32(ek::f32_bits(src[d]) ^ a.q_sign) : 0.0f;
+    for (int i = 0; i < QN; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32 w = r < nh && place(i) < a.dim ? x[i].w[k] ^ a.q_sign : 0;
+        __builtin_memcpy(&q.w[i][k], &w, 4);
       }
-#else
-#pragma unroll
-    for (int s = 0; s < KL; ++s)
-#pragma unroll
-      for (int e = 0; e < KE / 8; ++e) {
-        const int d = (s * 4 + c) * KE + e * 8;
-        words<4> x = {{0, 0, 0, 0}};
-        if (head && d < a.dim) x = load_words<4>((const char*)(src + d));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q.w[s * (KE / 8) + e][i] = x.w[i] ^ a.q_sign;
-      }
-#endif
   }
 
   // what the scores are multiplied by for exp2: positive, since the queries took the sign
@@ -382,6 +381,8 @@ extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void
     live = __builtin_amdgcn_ballot_w64(ok);
     return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : 0;
   };
+  // lanes past the end of a head read zeros: loads without a branch
+  const char* zeros = (const char*)s_zeros;
   const auto load_k = [&](Tile& t, int64_t off) {
     const auto go = [&](auto nt) {
 #pragma unroll
@@ -390,8 +391,7 @@ extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
           const int d = (i * 4 + c) * KE;
-          if (EK_PAD) t.k[s][i] = words<4>{{0, 0, 0, 0}};
-          if (!EK_PAD || d < a.dim) t.k[s][i] = load_words<4, nt.value>(p + d * CS);
+          t.k[s][i] = load_words<4, nt.value>(!EK_PAD || d < a.dim ? p + d * CS : zeros);
         }
       }
     };
@@ -406,8 +406,7 @@ extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void
 #pragma unroll
         for (int i = 0; i < PANELS; ++i) {
           const int d = i * 16 * VE + r * VE;
-          if (EK_PAD) t.v[j][i] = words<VW>{};
-          if (!EK_PAD || d < a.dim) t.v[j][i] = load_words<VW, nt.value>(p + d * CS);
+          t.v[j][i] = load_words<VW, nt.value>(!EK_PAD || d < a.dim ? p + d * CS : zeros);
         }
       }
     };

@@ -163,6 +163,9 @@ LOGITS = [
     (dict(bias=torch.zeros(3, 5)), ValueError, "go together"),
     (dict(bias=torch.zeros(3, 5), bias_ids=torch.zeros(3, 4, dtype=torch.int32)), ValueError,
      "`bias`"),
+    (dict(bias=torch.zeros(3, 1024), bias_ids=torch.zeros(3, 1024, dtype=torch.int32)),
+     ValueError, "at most 1023"),
+    (dict(tokens=torch.zeros(3, 1 << 21, dtype=torch.int32)), ValueError, "at most 2097151"),
     (dict(allowed=torch.zeros(3, 3, dtype=torch.int32)), ValueError, "need 4"),
     (dict(allowed=torch.zeros(3, 4, dtype=torch.int64)), TypeError, "`allowed`"),
     (dict(out=torch.zeros(3, 99)), ValueError, "`out`"),

@@ -451,7 +451,8 @@ def check_logits(d, out=None):
     (1, 1, 3, 0, False), (2, 7, 5, 3, True), (3, 31, 0, 0, True), (3, 32, 9, 2, True),
     (1, 2047, 100, 5, False), (5, 2049, 1, 300, True), (4, 8191, 1000, 17, True),
     (2, 32000, 5000, 0, False), (40, 50001, 260, 20, True), (300, 8193, 33, 0, True),
-    (3, 100003, 0, 0, False), (70000, 3, 2, 1, True),
+    (3, 100003, 0, 0, False), (70000, 3, 2, 1, True), (2, 4097, 30, 1023, False),
+    (2, 9000, 0, 513, False), (1, 20000, 2048, 511, True),
 ])
 def test_logits(dtype, rows, vocab, history, biases, mask):
     gen = torch.Generator().manual_seed(rows + vocab)
