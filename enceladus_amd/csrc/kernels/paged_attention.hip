@@ -41,10 +41,13 @@ typedef ek::bf16 T;
 constexpr int DP = EK_DP;
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
 constexpr float LN2 = 0.69314718055994531f;
-// Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that.
-// (32 x 128 bf16, that is 16 KB, needs 177 registers instead of 125 and gains nothing: 64 ragged
-// sequences, 501 MB: 94.1 us with 16 keys, 94.9 with 32 at their best numbers of waves.)
-constexpr int KT = 4096 / (DP * CS) < 16 ? 16 : 4096 / (DP * CS) > 32 ? 32 : 4096 / (DP * CS);
+// Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that; of an
+// e4m3 cache twice as many, whose conversions and scores cost more per byte than their loads.
+// Measured at their best numbers of waves: 64 ragged sequences, 501 MB of bf16, heads of 128:
+// 16 keys 88.3 us, 32 89.7 (and 177 registers instead of 125), 64 105; 24 ragged sequences,
+// 153 MB of e4m3: 16 keys 50.7 us, 32 46.4, 64 43.4.
+constexpr int KT0 = EK_FP8 ? 8192 / DP : 4096 / (DP * CS);
+constexpr int KT = KT0 < 16 ? 16 : KT0 > (EK_FP8 ? 64 : 32) ? (EK_FP8 ? 64 : 32) : KT0;
 constexpr int ST = KT / 16;                         // score tiles
 constexpr int KE = 16 / CS;                         // elements of a 16-byte key load
 constexpr int KL = DP / (4 * KE);                   // key loads per score tile and lane
@@ -146,6 +149,24 @@ EK_INLINE Item find_item(const Params& a, int item) {
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
   int per = (total + a.items - 1) / a.items;
   per = per < a.min_units ? a.min_units : per;
+  // Each sequence may have a chunk more than its share. If chunks of up to half as many units
+  // again fit all of them into `items`, that saves a last round of few waves.
+  if (a.batch <= HELD * 64) {
+    int try_per = per;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      int all = 0;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (i * 64 < a.batch) all += chunks_of(units_of(n[i]), try_per);
+      all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(all));
+      if (all <= a.items) {
+        per = try_per;
+        break;
+      }
+      try_per += (try_per + 7) >> 3;
+    }
+  }
 
   int before = 0;
   const auto search = [&](int base, int first, int count, Item& it) {

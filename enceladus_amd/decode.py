@@ -538,10 +538,11 @@ _ATTEND = struct.Struct("<9q8iI4iI3f4x")
 _UNIT = 16                          # tokens: what a sequence is split in multiples of
 _MIN_UNITS = 4                      # of a chunk
 _STREAM = 256 << 20                # bytes of caches that do not stay in the last-level cache
-# Chunks of all sequences and key heads, per CU, by the bytes of a cached element: as many as keep
-# 64 KB on their way into a CU at once. More of them leave more partial results (one sequence of
-# 131075, fp16: 94.8 us with 8, 102.3 with 16), fewer leave loads out (100.4 with 6).
-_WAVES = {1: 10, 2: 8, 4: 6}
+# Chunks of all sequences and key heads, per CU: two waves per SIMD. More of them leave more
+# partial results (one sequence of 131075, fp16: 94.8 us with 8, 102.3 with 16), fewer leave loads
+# out (100.4 with 6), and any that do not fit the SIMDs evenly run longer (64 ragged sequences,
+# bf16: 88.3 with 8, 96.2 with 10).
+_WAVES = 8
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float | None = None,
@@ -641,7 +642,7 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     most = -(-(min(window, capacity) if window else capacity) // _UNIT)
     group = heads // kv_heads
     y = kv_heads * (-(-group // 16))
-    items = max(1, min(_WAVES[kc.size] * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
+    items = max(1, min(_WAVES * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
               ("EK_PAD", int(dim != width)))
