@@ -257,11 +257,11 @@ class _Array:
         torch = _torch()
         self.obj = obj
         if torch is not None and isinstance(obj, torch.Tensor):
+            if obj.device.type not in ("cuda", "cpu") or obj.layout is not torch.strided:
+                raise ValueError(f"`{name}` is not a dense tensor on a GPU or the host")
             self.kind = _torch_kinds.get(obj.dtype, str(obj.dtype))
             self.shape, self.strides = tuple(obj.shape), obj.stride()
             self.device = obj.device.index if obj.device.type == "cuda" else -1
-            if obj.device.type not in ("cuda", "cpu") or obj.layout is not torch.strided:
-                raise ValueError(f"`{name}` is not a dense tensor on a GPU or the host")
             if self.device < 0 and self.kind == "fp8":
                 raise ValueError(f"`{name}` holds float8 values on the host: move it to the GPU")
         elif T.is_array_like(obj):
@@ -349,7 +349,9 @@ def _caches(k_cache, v_cache, heads, dim, kinds):
     vc = _array("v_cache", v_cache, (kc.kind,), 4, kc.shape)
     _need(tuple(kc.strides) == tuple(vc.strides), "`k_cache` and `v_cache` must have the same "
           f"strides, got {tuple(kc.strides)} and {tuple(vc.strides)}")
-    _need(kc.shape[1] > 0, "a page of `k_cache` must hold at least one token")
+    _need(0 < kc.shape[1] <= MAX_TOKENS, "a page of `k_cache` must hold at least one token, and "
+          f"at most {MAX_TOKENS}")
+    _need(kc.shape[0] < 1 << 31, f"`k_cache` has {kc.shape[0]} pages: ids are 32-bit")
     return kc, vc
 
 
@@ -380,8 +382,18 @@ def _head_dim(dim: int, cache: str) -> None:
           f"{MAX_HEAD_DIM}, got {dim}")
 
 
+# Scales beyond these have no product or reciprocal in 32 bits.
+_SCALES = 2.0 ** -60, 2.0 ** 60
+
+
 def _positive(name: str, x: float) -> None:
-    _need(math.isfinite(x) and x > 0, f"`{name}` must be a positive number, got {x}")
+    _need(_SCALES[0] <= x <= _SCALES[1],
+          f"`{name}` must be a positive number from 2^-60 to 2^60, got {x}")
+
+
+def _f32(x: float) -> float:
+    """x as far as 32 bits reach: infinite beyond."""
+    return math.copysign(math.inf, x) if abs(x) > 3.4028234e38 else x
 
 
 # -- appending to the cache ----------------------------------------------------------------
@@ -408,8 +420,9 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     `cu_tokens`, row b alone); they are its last ones, so that the i-th of n is at position
     `seq_lens[b] - n + i`. Rows of no sequence (padding behind the last, or before the first),
     and rows whose position is negative, not covered by the block table or not in `cos`, or
-    whose page is not in the cache, are skipped: neither cache nor `q_out` is written for them.
-    Two rows must not share a slot of the cache.
+    whose page is not in the cache, are skipped: neither cache nor `q_out` is written for them
+    (a new `q_out` holds anything there). Two rows must not share a slot of the cache, and the
+    new keys and values must not lie in it.
 
     With `cos` and `sin`, the first R elements of each key and query head are rotated in pairs,
     (j, j + R / 2), or (2 j, 2 j + 1) when `interleaved`: (x, y) becomes
@@ -447,9 +460,11 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
                None if sin is None else (sin.dtype, sin.shape, sin.stride(), sin.get_device()),
                interleaved, k_scale, v_scale)
         plan = _plans.get(key)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):
         key = plan = None              # arrays of another kind, or no arrays
     given = q_out is not None
+    if plan is not None and k_cache.data_ptr() == v_cache.data_ptr():
+        plan = None                    # refused below
     if plan is None:
         plan, q_out = _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q,
                                    q_out, cos, sin, interleaved, k_scale, v_scale)
@@ -470,6 +485,7 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
     """The checked call's plan (None: nothing to do) and its `q_out`."""
     ka = _array("k", k, ("fp32", "fp16", "bf16"), 3)
     tokens, kv_heads, dim = ka.shape
+    _need(tokens <= 1 << 25, f"at most {1 << 25} tokens are supported, got {tokens}")
     va = _array("v", v, (ka.kind,), 3, ka.shape)
     kc, vc = _caches(k_cache, v_cache, kv_heads, dim, (ka.kind, "fp8"))
     _head_dim(dim, kc.kind)
@@ -494,6 +510,7 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         _need(q_out is None, "`q_out` is given without `q`")
     _written("k_cache", kc)
     _written("v_cache", vc)
+    _need(kc.address() != vc.address() or not kc.span(), "`k_cache` and `v_cache` are the same")
     _need((cos is None) == (sin is None), "`cos` and `sin` go together")
     ca = sa = None
     rotary = 0
@@ -529,7 +546,8 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         ca.shape[0] if ca else 0, parts, 1.0 / k_scale, 1.0 / v_scale)
     return _Plan("append_kv.hip", macros,
                  [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
-                 tail, [(3, 0, True), (3, 1, False), (3, 2, False)]), q_out
+                 tail, [(3, 0, True), (3, 1, False), (3, 2, False), (3, 4, False),
+                        (3, 5, False)]), q_out
 
 
 # -- attention over the cache ----------------------------------------------------------------
@@ -588,7 +606,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
                seq_lens.stride(), seq_lens.get_device(), None if out is None else _of(out),
                scale, window, softcap, k_scale, v_scale)
         plan = _plans.get(key)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):
         key = plan = None              # arrays of another kind, or no arrays
     given = out is not None
     if plan is None:
@@ -618,12 +636,14 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     _head_dim(dim, kc.kind)
     _need(kv_heads > 0 and heads % kv_heads == 0,
           f"{heads} query heads are not a multiple of {kv_heads} key heads")
-    _need(heads <= 65535, f"at most 65535 query heads are supported, got {heads}")
+    _need(heads <= 65535 and batch <= 1 << 20,
+          f"at most 65535 query heads and {1 << 20} sequences are supported, got {heads}, {batch}")
     bt, sl = _sequences(block_table, seq_lens, batch)
     capacity = _capacity(bt, kc)
     scale = 1.0 / math.sqrt(dim) if scale is None else scale
-    _need(math.isfinite(scale), f"`scale` must be finite, got {scale}")
-    _need(math.isfinite(softcap) and softcap >= 0, f"`softcap` must be at least 0, got {softcap}")
+    _need(abs(scale) <= _SCALES[1], f"`scale` must be at most 2^60, got {scale}")
+    _need(softcap == 0 or _SCALES[0] <= softcap <= _SCALES[1],
+          f"`softcap` must be 0 or from 2^-60 to 2^60, got {softcap}")
     _need(window >= 0, f"`window` must be at least 0, got {window}")
     _positive("k_scale", k_scale)
     _positive("v_scale", v_scale)
@@ -691,7 +711,7 @@ def _per_row(name: str, x, rows: int, default: float):
         return None, default
     if T.is_array_like(x):
         return _array(name, x, ("fp32",), 1, (rows,), dense=False), default
-    return None, float(x)
+    return None, _f32(float(x))
 
 
 def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
@@ -732,7 +752,7 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
                  for x in (tokens, token_lens, prompt_lens, repetition, frequency, presence,
                            temperature, bias_ids, bias, allowed, out)])
         plan = _plans.get(key)
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):
         key = plan = None              # arrays of another kind, or no arrays
     given = out is not None
     if plan is None:
@@ -799,7 +819,7 @@ def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency,
     _device_of(arrays)
     if rows == 0 or vocab == 0:
         return None, out
-    _need(vocab < 1 << 30 and rows * vocab < 1 << 41,
+    _need(vocab < 1 << 30 and rows * -(-vocab // 4096) < 1 << 22,
           f"logits of shape {la.shape} are too large for one call")
     biases = ia.shape[1] if ia else 0
     _need(biases <= MAX_BIASES, f"at most {MAX_BIASES} biases of a row are supported, got "

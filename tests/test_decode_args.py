@@ -62,6 +62,17 @@ ATTEND = [
     (dict(softcap=float("nan")), ValueError, "softcap"),
     (dict(scale=float("inf")), ValueError, "scale"),
     (dict(k_scale=0.0), ValueError, "k_scale"),
+    (dict(k_scale=1e-30), ValueError, "k_scale"),
+    (dict(scale=1e30), ValueError, "scale"),
+    (dict(scale=float("nan")), ValueError, "scale"),
+    (dict(softcap=1e-30), ValueError, "softcap"),
+    (dict(q=torch.zeros(3, 8, 64, device="meta")), ValueError, "dense tensor"),
+    (dict(q=torch.zeros(3, 8, 64).to_sparse()), ValueError, "dense tensor"),
+    (dict(k_cache=torch.zeros(1, 1, 2, 64).expand(1 << 31, 1, 2, 64),
+          v_cache=torch.zeros(1, 1, 2, 64).expand(1 << 31, 1, 2, 64)), ValueError, "32-bit"),
+    (dict(q=torch.zeros(1, 8, 64).expand(1 << 21, 8, 64),
+          block_table=torch.zeros(1, 4, dtype=torch.int32).expand(1 << 21, 4),
+          seq_lens=torch.zeros(1, dtype=torch.int32).expand(1 << 21)), ValueError, "sequences"),
     (dict(v_scale=float("nan")), ValueError, "v_scale"),
     (dict(out=torch.zeros(3, 8, 32)), ValueError, "`out`"),
     (dict(out=torch.zeros(3, 8, 64).half()), TypeError, "`out`"),
@@ -112,6 +123,7 @@ APPEND = [
     (dict(q_out=torch.zeros(3, 8, 64)), ValueError, "without `q`"),
     (dict(q=torch.zeros(3, 8, 64), q_out=torch.zeros(3, 4, 64)), ValueError, "`q_out`"),
     (dict(k_scale=-1.0), ValueError, "k_scale"),
+    (dict(k=torch.zeros(1, 2, 64).expand(1 << 26, 2, 64)), ValueError, "tokens"),
 ]
 
 
@@ -139,6 +151,13 @@ def test_append_kv_refuses_overlap_and_read_only():
     *args, _ = _append()
     with pytest.raises(ValueError, match="`q_out` overlaps `q`"):
         decode.append_kv(*args, q=rows[:3], q_out=rows[1:])
+    *args, _ = _append()
+    args[3] = args[2]
+    with pytest.raises(ValueError, match="are the same"):
+        decode.append_kv(*args)
+    *args, _ = _append()
+    with pytest.raises(ValueError, match="`q_out` overlaps `v_cache`"):
+        decode.append_kv(*args, q=rows[:3], q_out=args[3].view(-1)[64:64 + 1536].view(3, 8, 64))
     cache = np.zeros((10, 16, 2, 64), np.float32)
     cache.flags.writeable = False
     *args, _ = _append(k_cache=cache)
@@ -169,6 +188,8 @@ LOGITS = [
     (dict(allowed=torch.zeros(3, 3, dtype=torch.int32)), ValueError, "need 4"),
     (dict(allowed=torch.zeros(3, 4, dtype=torch.int64)), TypeError, "`allowed`"),
     (dict(out=torch.zeros(3, 99)), ValueError, "`out`"),
+    (dict(logits=torch.zeros(1, 100).expand(1 << 22, 100),
+          out=torch.zeros(1, 100).expand(1 << 22, 100)), ValueError, "expanded"),
     (dict(out=torch.zeros(3, 1).expand(3, 100)), ValueError, "contiguous|expanded"),
 ]
 
