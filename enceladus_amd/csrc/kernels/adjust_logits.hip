@@ -12,7 +12,8 @@
 // history, from the L2: a longer stretch (EK_N) reads it fewer times, a shorter one gives few
 // rows more workgroups and overlaps one workgroup's counting with another's streaming.
 //
-// Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_N (logits per workgroup).
+// Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_N (logits per workgroup), EK_STREAM
+// (the output is more than the caches keep: stored past them).
 #include "enceladus_cdna4.h"
 
 #if EK_Q == 0
@@ -239,7 +240,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
       y[j] = ek::cvt<T>(ok >> j & 1 ? z : -__builtin_inff());
     }
     if (at + V <= n) {
-      ek::vstore_u<T, V>(dst + at, y);
+      if constexpr (EK_STREAM) ek::vstore_nt_u<T, V>(dst + at, y);
+      else ek::vstore_u<T, V>(dst + at, y);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)

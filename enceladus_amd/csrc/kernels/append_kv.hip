@@ -12,7 +12,8 @@
 // meet in one lane, so that queries can be rotated in place.
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
-// vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS.
+// vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS,
+// EK_STREAM (the rows are more than the caches keep: loaded and stored past them).
 #include "enceladus_cdna4.h"
 
 #if EK_Q == 0
@@ -46,6 +47,11 @@ struct Params {
 
 EK_INLINE float sat8(float x) { return x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x; }
 
+template <int N, typename S> EK_INLINE void put(S* p, const S* w) {
+  if constexpr (EK_STREAM) ek::vstore_nt_u<S, N>(p, w);
+  else ek::vstore_u<S, N>(p, w);
+}
+
 // V floats into the cache at p.
 EK_INLINE void store_cache(char* p, const float* x, float inv) {
 #if EK_FP8
@@ -59,12 +65,12 @@ EK_INLINE void store_cache(char* p, const float* x, float inv) {
     u = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], u, true);
     __builtin_memcpy(w + i, &u, 4);
   }
-  ek::vstore_u<uint8_t, V>((uint8_t*)p, w);
+  put<V>((uint8_t*)p, w);
 #else
   T w[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) w[i] = ek::cvt<T>(x[i] * inv);
-  ek::vstore_u<T, V>((T*)p, w);
+  put<V>((T*)p, w);
 #endif
 }
 
@@ -72,14 +78,17 @@ EK_INLINE void store_out(T* p, const float* x) {
   T w[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) w[i] = ek::cvt<T>(x[i]);
-  ek::vstore_u<T, V>(p, w);
+  put<V>(p, w);
 }
 
-template <typename S> EK_INLINE void load(float* x, const S* p) {
+template <bool NT = false, typename S> EK_INLINE void load(float* x, const S* p) {
   S w[V];
   constexpr int M = sizeof(S) * V > 16 ? 16 / sizeof(S) : V;
 #pragma unroll
-  for (int i = 0; i < V; i += M) ek::vload_u<S, M>(w + i, p + i);
+  for (int i = 0; i < V; i += M) {
+    if constexpr (NT) ek::vload_nt_u<S, M>(w + i, p + i);
+    else ek::vload_u<S, M>(w + i, p + i);
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) x[i] = ek::f32(w[i]);
 }
@@ -140,8 +149,8 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
                       : is_k ? a.k + t * a.k_row + h * a.k_head
                              : a.v + t * a.v_row + h * a.v_head) + d;
       float x[V], y[V];
-      load(x, src);
-      if (two) load(y, src + half);
+      load<EK_STREAM>(x, src);
+      if (two) load<EK_STREAM>(y, src + half);
       if (turn && (is_q || is_k)) {
         if constexpr (EK_PAIRS) {
 #pragma unroll

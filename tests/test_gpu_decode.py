@@ -377,6 +377,27 @@ def test_append_many_tokens():
     check_append(append_case(gen, F16, F16, [9000, 700], [8999, 300], 16, 1, 3, 64, 64))
 
 
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F8), (BF16, BF16)])
+def test_loads_past_the_caches_give_the_same(dtype, cdtype, monkeypatch):
+    """Large rows and caches are loaded with another hint: the same bits."""
+    gen = torch.Generator().manual_seed(12)
+    lens, new = [300, 77], [200, 70]
+    d = append_case(gen, dtype, cdtype, lens, new, 16, 2, 4, 80, 40)
+    got = []
+    for size in (1 << 62, 0):
+        monkeypatch.setattr(decode, "_STREAM", size)
+        monkeypatch.setattr(decode, "_STREAM_ROWS", size)
+        decode._plans.clear()
+        g, q = check_append(d)
+        o = decode.paged_attention(q[[199, 269]], g["k_cache"], g["v_cache"], g["block_table"],
+                                   g["seq_lens"]) if dtype is not F32 or cdtype is F32 else q
+        x = check_logits(logits_case(torch.Generator().manual_seed(13), 9, 9001, 70, 5, True, dtype))
+        got.append((g["k_cache"].view(torch.uint8), g["v_cache"].view(torch.uint8), q, o, x))
+    decode._plans.clear()
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_append_rounds_to_8_bits_as_the_type_says():
     """Every neighbourhood of an e4m3 value: its rounding, ties, zeros, overflow, NaN."""
     grid = torch.arange(256, dtype=torch.uint8).view(F8).float()
