@@ -99,16 +99,21 @@ EK_INLINE int page_of(const Params& a, int key) {
 }
 
 // Keys that sequence b attends to: [first, first + count).
-EK_INLINE void span_of(const Params& a, int b, int& first, int& count) {
-  int n = b < a.batch ? a.lens[b * a.lens_step] : 0;
-  n = n < 0 ? 0 : n > a.capacity ? a.capacity : n;
+EK_INLINE int length_of(const Params& a, int b) {
+  return a.lens[(b < a.batch ? b : a.batch - 1) * a.lens_step];
+}
+EK_INLINE void span_of(const Params& a, int b, int n, int& first, int& count) {
+  n = n < 0 || b >= a.batch ? 0 : n > a.capacity ? a.capacity : n;
   first = a.window > 0 && n > a.window ? n - a.window : 0;
   count = n - first;
+}
+EK_INLINE void span_of(const Params& a, int b, int& first, int& count) {
+  span_of(a, b, length_of(a, b), first, count);
 }
 
 EK_INLINE int units_of(int count) { return (count + UNIT - 1) / UNIT; }
 
-EK_INLINE int chunks_of(int units, int per) { return (units + per - 1) / per; }
+EK_INLINE int chunks_of(int units, int per) { return (u32)(units + per - 1) / (u32)per; }
 
 template <typename OP, typename V> EK_INLINE V wave_all(V x) {
   x = ek::reduce_xor<OP, 1>(x);
@@ -135,19 +140,19 @@ EK_INLINE Item find_item(const Params& a, int item) {
   const int lane = ek::lane_id();
   int f[HELD], n[HELD], total = 0;
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
-    f[i] = n[i] = 0;
-    if (i == 0 || i * 64 < a.batch) span_of(a, i * 64 + lane, f[i], n[i]);
-  }
+  for (int i = 0; i < HELD; ++i) n[i] = length_of(a, i * 64 + lane);   // one wait for all
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) total += units_of(n[i]);
+  for (int i = 0; i < HELD; ++i) {
+    span_of(a, i * 64 + lane, n[i], f[i], n[i]);
+    total += units_of(n[i]);
+  }
   for (int base = HELD * 64; base < a.batch; base += 64) {
     int first, count;
     span_of(a, base + lane, first, count);
     total += units_of(count);
   }
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
-  int per = (total + a.items - 1) / a.items;
+  int per = chunks_of(total, a.items);
   per = per < a.min_units ? a.min_units : per;
   // Each sequence may have a chunk more than its share. If chunks of up to half as many units
   // again fit all of them into `items`, that saves a last round of few waves.
@@ -160,10 +165,8 @@ EK_INLINE Item find_item(const Params& a, int item) {
       for (int i = 0; i < HELD; ++i)
         if (i * 64 < a.batch) all += chunks_of(units_of(n[i]), try_per);
       all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(all));
-      if (all <= a.items) {
-        per = try_per;
-        break;
-      }
+      if (all <= a.items) per = try_per;
+      if (all <= a.items || all > a.items + a.items / 2) break;
       try_per += (try_per + 7) >> 3;
     }
   }

@@ -668,6 +668,8 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
         capacity = 0
     window = min(window, MAX_TOKENS)
     most = -(-(min(window, capacity) if window else capacity) // _UNIT)
+    _need(batch * most < 1 << 31, f"`block_table` covers {batch} sequences of {capacity} tokens: "
+          f"at most {_UNIT << 31} tokens in all are supported")
     group = heads // kv_heads
     y = kv_heads * (-(-group // 16))
     items = max(1, min(_WAVES * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))

@@ -53,6 +53,9 @@ ATTEND = [
     (dict(block_table=torch.zeros(3, 1 << 26, dtype=torch.int32)[:, ::1],
           k_cache=torch.zeros(1, 32, 2, 64), v_cache=torch.zeros(1, 32, 2, 64)), ValueError,
      "at most"),
+    (dict(q=torch.zeros(1, 8, 64).expand(1 << 16, 8, 64),
+          block_table=torch.zeros(1, 1 << 15, dtype=torch.int32).expand(1 << 16, 1 << 15),
+          seq_lens=torch.zeros(1, dtype=torch.int32).expand(1 << 16)), ValueError, "in all"),
     (dict(seq_lens=torch.ones(4, dtype=torch.int32)), ValueError, "`seq_lens`"),
     (dict(seq_lens=np.ones(3, np.float32)), TypeError, "`seq_lens`"),
     (dict(seq_lens=np.ones(3, np.int32)[::-1]), ValueError, "negative strides"),
