@@ -204,7 +204,9 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
   }
   if (marks) __syncthreads();
 
-  const float rrep = 1.0f / rep, rtemp = temp > 0.0f ? 1.0f / temp : 1.0f;
+  // lift: the reciprocal of a temperature below 2^-128 would be infinite, and 0 times that NaN
+  const float lift = temp > 0.0f && temp < 0x1p-100f ? 0x1p60f : 1.0f;
+  const float rrep = 1.0f / rep, rtemp = temp > 0.0f ? 1.0f / (temp * lift) : 1.0f;
   T* dst = a.out + b * a.out_row + v0;
 #pragma unroll
   for (int i = 0; i < VN; ++i) {
@@ -236,7 +238,7 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
     T y[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float z = f[j] * rtemp;
+      const float z = f[j] * lift * rtemp;
       y[j] = ek::cvt<T>(ok >> j & 1 ? z : -__builtin_inff());
     }
     if (at + V <= n) {

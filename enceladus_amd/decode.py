@@ -582,7 +582,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
     `softcap`) when that is above 0; the result is the sum of softmax(s)_j v_j. `heads` is a
     multiple of the key heads: head h reads key head h // (heads / key heads). A sequence
     without tokens gives zeros. Tokens on a page outside the cache count as absent. Cache
-    memory that no sequence's length reaches may hold anything, NaN included.
+    memory that no sequence's length reaches may hold anything, NaN included. A value among a
+    sequence's own that is not finite makes its element of the result infinite or NaN.
 
     Args:
         q: `[batch, heads, dim]`, float32, float16 or bfloat16; `dim` a multiple of 8 up to
@@ -745,7 +746,8 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
             vocabulary are ignored.
         token_lens: how much of each row of `tokens` counts, int32 `[rows]`; all without it.
         prompt_lens: how much of that is the prompt, int32 `[rows]`; none without it.
-        repetition, frequency, presence, temperature: a number, or float32 `[rows]`.
+        repetition, frequency, presence, temperature: a number, or float32 `[rows]`
+            (`repetition` from 2^-60 to 2^60).
         bias_ids, bias: int32 and float32 `[rows, entries]`, at most 1023 entries; ids outside
             the vocabulary are ignored, entries with the same id add up in their order.
         allowed: int32 `[rows, words]`, 32 tokens to a word: token t is bit t % 32 of word
@@ -817,7 +819,10 @@ def _logits_plan(logits, tokens, token_lens, prompt_lens, repetition, frequency,
     freq_a, freq = _per_row("frequency", frequency, rows, 0.0)
     pres_a, pres = _per_row("presence", presence, rows, 0.0)
     temp_a, temp = _per_row("temperature", temperature, rows, 0.0)
-    _need(rep > 0, f"`repetition` must be above 0, got {rep}")
+    _positive("repetition", rep)
+    # others lose digits, or all of them, as 32-bit numbers or in their reciprocals
+    _need(temp <= 0 or 2.0 ** -126 <= temp <= 2.0 ** 126,
+          f"`temperature` must be from 2^-126 to 2^126, or 0 for none, got {temp}")
     if out is None:
         out = T.new_empty(logits)
     oa = _array("out", out, (la.kind,), 2, la.shape)

@@ -179,6 +179,10 @@ LOGITS = [
     (dict(repetition=1.2), ValueError, "need the history"),
     (dict(token_lens=torch.zeros(3, dtype=torch.int32)), ValueError, "need the history"),
     (dict(tokens=torch.zeros(3, 5, dtype=torch.int32), repetition=0.0), ValueError, "repetition"),
+    (dict(tokens=torch.zeros(3, 5, dtype=torch.int32), repetition=1e39), ValueError, "repetition"),
+    (dict(temperature=1e-40), ValueError, "temperature"),
+    (dict(temperature=1e-60), ValueError, "temperature"),
+    (dict(temperature=float("nan")), ValueError, "temperature"),
     (dict(tokens=torch.zeros(3, 5, dtype=torch.int32), repetition=torch.zeros(2)), ValueError,
      "`repetition`"),
     (dict(temperature=torch.zeros(3).half()), TypeError, "`temperature`"),

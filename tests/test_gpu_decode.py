@@ -190,6 +190,24 @@ def test_attention_values_that_are_not_finite():
     check_attention(rand(gen, 4, 4, 64), kc, vc, bt, lens)
 
 
+@pytest.mark.parametrize("dtype,value", [(F16, math.inf), (BF16, -math.inf), (BF16, math.nan)])
+def test_attention_values_that_are_not_finite_stay_in_their_elements(dtype, value):
+    """Infinite or NaN there (a weight is a sum of two 16-bit terms, which may differ in sign),
+    and no other element sees it."""
+    gen = torch.Generator().manual_seed(3)
+    lens = [200, 90]
+    bt, pages = table_for(gen, lens, 16)
+    kc, vc = (only_live(cache(gen, pages, 16, 1, 64, dtype), bt, lens, 16) for _ in "kv")
+    q = rand(gen, 2, 4, 64, dtype=dtype).cuda()
+    rest = kc.cuda(), vc.cuda(), bt.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    want = decode.paged_attention(q, *rest)
+    rest[1][int(bt[0, 3]), 5, 0, 7] = value
+    got = decode.paged_attention(q, *rest)
+    assert not torch.isfinite(got[0, :, 7]).any()
+    got[0, :, 7] = want[0, :, 7]
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("batch", [1, 63, 64, 65, 200])
 def test_attention_of_many_sequences(batch):
     gen = torch.Generator().manual_seed(batch)
@@ -501,6 +519,16 @@ def test_logits_that_are_not_finite():
     d["temperature"] = torch.full((4,), 1.25)
     d["repetition"] = torch.full((4,), 1.0)
     check_logits(d)
+
+
+def test_logits_of_temperatures_near_zero():
+    """Below 2^-128, where the reciprocal is infinite: zeros stay zeros, small logits finite."""
+    gen = torch.Generator().manual_seed(5)
+    x = rand(gen, 5, 300, scale=4.0)
+    x[:, ::7] = 0.0
+    x[:, 1::7] *= 2.0 ** -40
+    check_logits(dict(logits=x, temperature=torch.tensor([1e-40, 2.0 ** -149, 1e-38, 1e-30,
+                                                          2.0 ** -101])))
 
 
 def test_logits_strides_shared_masks_and_places():
