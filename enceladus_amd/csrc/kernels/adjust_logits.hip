@@ -118,38 +118,48 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_adjust_logits(Params a)
     __syncthreads();
   }
   if (a.tokens) {
-    const auto count = [&](int i, int32_t id) {
+    const auto prompted = [&](int32_t id) {
       const uint32_t at = (uint32_t)id - (uint32_t)v0;
-      if (at < (uint32_t)n) {
-        if (i < prompt) atomicOr(&s_mark[at], SEEN);
-        else atomicAdd(&s_mark[at], 1u);
+      if (at < (uint32_t)n) atomicOr(&s_mark[at], SEEN);
+    };
+    const auto generated = [&](int32_t id) {
+      const uint32_t at = (uint32_t)id - (uint32_t)v0;
+      if (at < (uint32_t)n) atomicAdd(&s_mark[at], 1u);
+    };
+    // Tokens `from` to `to`, four vectors of ids on their way at once.
+    const auto each = [&](int from, int to, const auto& count) {
+      constexpr int STEP = THREADS * 4;
+      int i = from + tid * 4;
+      for (; i + 3 * STEP + 4 <= to; i += 4 * STEP) {
+        int32_t id[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ek::vload_u<int32_t, 4>(id[k], row + i + k * STEP);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) count(id[k][j]);
+      }
+      for (; i < to; i += STEP) {
+        if (i + 4 <= to) {
+          int32_t id[4];
+          ek::vload_u<int32_t, 4>(id, row + i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) count(id[j]);
+        } else {
+          for (int j = i; j < to; ++j) count(row[j]);
+        }
       }
     };
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (tid * 4 + j < len) count(tid * 4 + j, ids[j]);
-    // four vectors of ids on their way at once
-    constexpr int STEP = THREADS * 4;
-    int i = tid * 4 + STEP;
-    for (; i + 3 * STEP + 4 <= len; i += 4 * STEP) {
-      int32_t id[4][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ek::vload_u<int32_t, 4>(id[k], row + i + k * STEP);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) count(i + k * STEP + j, id[k][j]);
-    }
-    for (; i < len; i += STEP) {
-      if (i + 4 <= len) {
-        int32_t id[4];
-        ek::vload_u<int32_t, 4>(id, row + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) count(i + j, id[j]);
-      } else {
-        for (int j = i; j < len; ++j) count(j, row[j]);
+      if (tid * 4 + j < len) {
+        if (tid * 4 + j < prompt) prompted(ids[j]);
+        else generated(ids[j]);
       }
-    }
+    constexpr int FIRST = THREADS * 4;
+    const int middle = prompt < FIRST ? FIRST : prompt > len ? len : prompt;
+    each(FIRST, middle, prompted);
+    each(middle, len, generated);
   }
   if (a.biases > 0) {
     // Entries count themselves in first. One that is alone with its id stands for itself; of
