@@ -651,38 +651,39 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
     float mm = -__builtin_inff(), ll = 0.0f;
 #pragma unroll
     for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
+#pragma unroll 1
     for (int i0 = 0; i0 < size; i0 += 16) {
       const int count = size - i0 < 16 ? size - i0 : 16, i = lane & 15;
-      float m = -__builtin_inff(), l = 0.0f;
-      if (i < count) {
-        m = ml[((int64_t)(begin + i0 + i) * a.heads + head) * 2];
-        l = ml[((int64_t)(begin + i0 + i) * a.heads + head) * 2 + 1];
-      }
+      // Loads without branches: lanes and chunks that are not there read the last one, which
+      // then has no weight.
+      const int64_t at = (int64_t)(begin + i0) * a.heads + head;
+      const float* mls = ml + (at + (int64_t)(i < count ? i : count - 1) * a.heads) * 2;
+      float m = mls[0], l = mls[1];
       float v[16][DW][2];
+      const char* base = (const char*)(a.part + at * a.dim);
+      const u32 step = (u32)a.heads * a.dim * 4;   // of 15 at most: below 2^32
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (int j = 0; j < 16; ++j) {
+        const u32 row = (u32)(j < count ? j : count - 1) * step;
 #pragma unroll
         for (int k = 0; k < DW; ++k) {
           const int d = k * 128 + lane * 2;
-          v[j][k][0] = v[j][k][1] = 0.0f;
-          if (j < count && d < a.dim)
-            ek::vload_u<float, 2>(v[j][k],
-                                  a.part + ((int64_t)(begin + i0 + j) * a.heads + head) * a.dim + d);
+          ek::vload_u<float, 2>(v[j][k], (const float*)(base + (row + (d < a.dim ? d : 0) * 4u)));
         }
-      float w = weigh16(m, l), f = 0.0f;
-      if (i0 > 0) {                    // more than 16 chunks: onto what came before
-        const float m_new = __builtin_fmaxf(mm, m);
-        const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-        f = ek::exp2_fast(mm - mu);
-        const float part = ek::exp2_fast(m - mu);
-        w *= part;
-        l = __builtin_fmaf(ll, f, l * part);
-        m = m_new;
-#pragma unroll
-        for (int k = 0; k < DW; ++k) x[k][0] *= f, x[k][1] *= f;
       }
-      mm = m;
-      ll = l;
+      __builtin_amdgcn_sched_barrier(0);           // all of them before the first wait
+      m = i < count ? m : -__builtin_inff();
+      l = i < count ? l : 0.0f;
+      float w = weigh16(m, l);
+      // onto what came before (with more than 16 chunks)
+      const float m_new = __builtin_fmaxf(mm, m);
+      const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+      const float f = ek::exp2_fast(mm - mu), part = ek::exp2_fast(m - mu);
+      w *= part;
+      ll = __builtin_fmaf(ll, f, l * part);
+      mm = m_new;
+#pragma unroll
+      for (int k = 0; k < DW; ++k) x[k][0] *= f, x[k][1] *= f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float y = lane_value(w, j);

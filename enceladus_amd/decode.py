@@ -684,7 +684,7 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
         workspace = (items + batch) * heads * (dim + 2) * 4 + batch * 8
         chunks = min(items, -(-most // _MIN_UNITS))
         # A wave per 16 chunks; where there are many sequences, few of them have many.
-        waves = max(4, min(16, -(-chunks // 16), 8192 // (batch * heads)))
+        waves = max(4, min(16, -(-chunks // 16), 4096 // (batch * heads)))
         launches.append(("ek_paged_attention_join", (batch, heads), 64 * waves))
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
