@@ -152,6 +152,18 @@ def test_attention_window_softcap_scale(dtype, window, softcap, scale):
                     softcap=softcap, scale=scale)
 
 
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128), (BF16, 240)])
+@pytest.mark.parametrize("group", [1, 7, 8, 9, 24])
+@pytest.mark.parametrize("window,softcap,scale", [(0, 30.0, None), (71, 0.0, -0.2), (200, 2.0, -1.0)])
+def test_attention_8_bit_window_softcap_scale(dtype, dim, group, window, softcap, scale):
+    gen = torch.Generator().manual_seed(window + group)
+    bt, pages = table_for(gen, LENS, 16)
+    bt[-1, 3] = -1                                          # a page that is not there
+    kc, vc = (only_live(cache(gen, pages, 16, 2, dim, F8), bt, LENS, 16) for _ in "kv")
+    check_attention(rand(gen, len(LENS), 2 * group, dim, dtype=dtype), kc, vc, bt, LENS,
+                    window=window, softcap=softcap, scale=scale, k_scale=0.5)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_attention_one_large_weight_among_many_small_ones(dtype):
     """One key with nearly all of the weight, thousands that share the rest."""
