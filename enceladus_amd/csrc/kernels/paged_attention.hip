@@ -577,7 +577,7 @@ extern "C" __global__ __launch_bounds__(64, EK_Q == 0 && DP == 256 ? 1 : 2) void
       // e4m3, 64 heads over 8 key heads: with a softcap 39.9 us instead of 41.4, without one
       // the same).
       if (nh <= 8) {
-        ek::f32x4 x[ST / 2];
+        ek::f32x4 x[PACKS ? ST / 2 : 1];
 #pragma unroll
         for (int s = 0; s < ST / 2; ++s)
 #pragma unroll
