@@ -10,7 +10,7 @@
 // takes one token, or a part of its rows (query, key and value heads) when there are few tokens;
 // a lane keeps one place in the head, so its cos and sin are read once for all rows, and pairs
 // meet in one lane, so that queries can be rotated in place.
-// Measured: 21152 tokens of 32 query, 8 key and 8 value heads of 128 in bf16, 531 MB: 92 us, 5.8
+// Measured: 21152 tokens of 32 query, 8 key and 8 value heads of 128 in bf16, 531 MB: 90 us, 5.9
 // TB/s (a copy of 1 GiB: 5.0). One token of such heads: 3.2 us, a launch and a chain of loads.
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
@@ -95,27 +95,41 @@ template <bool NT = false, typename S> EK_INLINE void load(float* x, const S* p)
   for (int i = 0; i < V; ++i) x[i] = ek::f32(w[i]);
 }
 
+__device__ const float s_zeros[8] = {};              // what is no cos or sin
+
 extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
   const int lane = ek::lane_id();
-  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = (int)(id / a.parts), part = (int)(id - (int64_t)t * a.parts);
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = (int)(unit / (uint32_t)a.parts), part = (int)unit - t * a.parts;
   if (t >= a.tokens) return;
 
   int b = t, back = 1;               // the sequence, and how far before its end the token is
   if (a.cu) {
     b = 0;
-    for (int i = 0; i < a.batch; i += 64) {
-      const bool over = i + lane < a.batch && a.cu[(i + lane + 1) * a.cu_step] <= t;
-      b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(over));
+    for (int i = 0; i < a.batch; i += 256) {
+      int end[4];                    // on their way at once
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = i + k * 64 + lane;
+        end[k] = a.cu[((at < a.batch ? at : a.batch - 1) + 1) * a.cu_step];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        b += __builtin_popcountll(
+            __builtin_amdgcn_ballot_w64(i + k * 64 + lane < a.batch && end[k] <= t));
     }
-    if (b >= a.batch || a.cu[b * a.cu_step] > t) return;
-    back = a.cu[(b + 1) * a.cu_step] - t;
+    if (b >= a.batch) return;
   }
-  const int pos = a.lens[b * a.lens_step] - back;
+  int len = a.lens[b * a.lens_step];
+  if (a.cu) {
+    int begin = a.cu[b * a.cu_step], end = a.cu[(b + 1) * a.cu_step];
+    asm volatile("" : "+s"(begin), "+s"(end), "+s"(len));    // one wait for the three
+    if (begin > t) return;
+    back = end - t;
+  }
+  const int pos = len - back;
   if (pos < 0 || pos >= a.capacity || (a.rotary && pos >= a.positions)) return;
-  const int pg = pos / a.page, id_ = a.table[b * a.table_row + pg];
-  if ((uint32_t)id_ >= (uint32_t)a.pages) return;
-  const int64_t slot = id_ * a.c_page + (pos - pg * a.page) * a.c_token;
+  const int pg = pos / a.page, page_id = a.table[b * a.table_row + pg];
 
   // places of a head: `pairs` of two vectors that are rotated together, then single vectors
   const int half = a.rotary / 2;
@@ -131,28 +145,32 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
     const int d = two ? place * V : EK_PAIRS ? place * V : a.rotary + (place - pairs) * V;
     float cs[V], sn[V];
     const bool turn = EK_PAIRS ? d < a.rotary : two;
-    if (turn) {
-      const float* cp = a.cos + pos * a.cos_row + (EK_PAIRS ? d / 2 : d);
-      const float* sp = a.sin + pos * a.sin_row + (EK_PAIRS ? d / 2 : d);
-      if constexpr (EK_PAIRS) {
+    // where nothing turns, zeros, so that no branch has to wait for what it loaded
+    const float* cp = turn ? a.cos + pos * a.cos_row + (EK_PAIRS ? d / 2 : d) : s_zeros;
+    const float* sp = turn ? a.sin + pos * a.sin_row + (EK_PAIRS ? d / 2 : d) : s_zeros;
+    if constexpr (EK_PAIRS) {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) cs[i] = cp[i], sn[i] = sp[i];
-      } else {
-        load(cs, cp);
-        load(sn, sp);
-      }
+      for (int i = 0; i < V / 2; ++i) cs[i] = cp[i], sn[i] = sp[i];
+    } else {
+      load(cs, cp);
+      load(sn, sp);
     }
     for (int row = part * lanes + (places <= 64 ? sub : 0); row < rows;
          row += a.parts * lanes) {
       const bool is_q = row < a.heads, is_k = !is_q && row < a.heads + a.kv_heads;
-      if (is_q && !a.q) continue;
       const int h = is_q ? row : is_k ? row - a.heads : row - a.heads - a.kv_heads;
       const T* src = (is_q ? a.q + t * a.q_row + h * a.q_head
                       : is_k ? a.k + t * a.k_row + h * a.k_head
                              : a.v + t * a.v_row + h * a.v_head) + d;
       float x[V], y[V];
       load<EK_STREAM>(x, src);
-      if (two) load<EK_STREAM>(y, src + half);
+      // without a branch, whose wait for the first load would come before the second
+      if constexpr (!EK_PAIRS) load<EK_STREAM>(y, src + (two ? half : 0));
+      // the page is looked at with the first row on its way (and not moved in front of that)
+      int id;
+      asm volatile("v_mov_b32 %0, %1" : "=v"(id) : "v"(page_id));
+      if ((uint32_t)id >= (uint32_t)a.pages) return;
+      const int64_t slot = id * a.c_page + (pos - pg * a.page) * a.c_token;
       if (turn && (is_q || is_k)) {
         if constexpr (EK_PAIRS) {
 #pragma unroll

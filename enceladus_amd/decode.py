@@ -408,6 +408,12 @@ _APPEND = struct.Struct("<16q11i2f4x")
 _STREAM_ROWS = 32 << 20
 
 
+# Rows that a lane takes one after the other. 265 MB of fp32 tokens of 72 rows of 192, one row at
+# a time: 109 us with all 72, 61 with 8 or 4, 70 with 2; the tokens above 93 us with 6, 90 with 4;
+# 41 MB of 80 rows of 64, many at a time: 11.7 with 4, 13.1 with 3.
+_ROUNDS = 4
+
+
 def _vector(size: int, rotary: int, dim: int, interleaved: bool) -> int:
     """Elements of an access: up to 16 bytes, dividing each part of a head."""
     v = 16 // size
@@ -540,10 +546,11 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
     macros = (("EK_Q", _Q[ka.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_V", vec),
               ("EK_PAIRS", int(interleaved)),
               ("EK_STREAM", int(tokens * rows * dim * ka.size > _STREAM_ROWS)))
-    # One wave per token, unless that leaves CUs without one: then as many as it has rows for.
+    # Waves per token: as many as it has rows for while CUs are without one, then enough for
+    # _ROUNDS rows a lane (2^25 in all: a grid holds fewer than 2^32 threads).
     places = dim // vec if interleaved else (dim - rotary // 2) // vec
     most = -(-rows // max(1, 64 // places))
-    parts = max(1, min(most, 4096 // tokens))
+    parts = max(1, min(most, 4096 // tokens), min(-(-most // _ROUNDS), (1 << 25) // tokens))
     zero = (0, 0, 0)
     qs, os = (a.strides if a is not None else zero for a in (qa, qo))
     tail = _APPEND.pack(

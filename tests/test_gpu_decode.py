@@ -154,7 +154,8 @@ def test_attention_window_softcap_scale(dtype, window, softcap, scale):
 
 @pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128), (BF16, 240)])
 @pytest.mark.parametrize("group", [1, 7, 8, 9, 24])
-@pytest.mark.parametrize("window,softcap,scale", [(0, 30.0, None), (71, 0.0, -0.2), (200, 2.0, -1.0)])
+@pytest.mark.parametrize("window,softcap,scale", [(0, 30.0, None), (71, 0.0, -0.2),
+                                                  (200, 2.0, -1.0)])
 def test_attention_8_bit_window_softcap_scale(dtype, dim, group, window, softcap, scale):
     gen = torch.Generator().manual_seed(window + group)
     bt, pages = table_for(gen, LENS, 16)
@@ -405,6 +406,26 @@ def test_append_many_sequences(batch):
 def test_append_many_tokens():
     gen = torch.Generator().manual_seed(11)
     check_append(append_case(gen, F16, F16, [9000, 700], [8999, 300], 16, 1, 3, 64, 64))
+
+
+@pytest.mark.parametrize("heads,dim,rotary,behind", [(37, 24, 8, 3), (9, 136, 0, 0),
+                                                     (20, 192, 16, 1)])
+def test_append_many_rows_of_many_tokens(heads, dim, rotary, behind):
+    """Several waves per token, the last of them with fewer rows than the others."""
+    gen = torch.Generator().manual_seed(heads)
+    check_append(append_case(gen, F32, F32, [4200, 3, 1], [4199, 1, 0], 16, 3, heads, dim, rotary,
+                             behind=behind))
+
+
+@pytest.mark.parametrize("batch", [256, 257, 600])
+def test_append_single_tokens_of_many_sequences(batch):
+    gen = torch.Generator().manual_seed(batch)
+    new = [1] * batch
+    new[3:40] = [0] * 37
+    lens = [n + int(torch.randint(0, 20, (1,), generator=gen)) for n in new]
+    d = append_case(gen, F16, F8, lens, new, 16, 2, 2, 64, 64, before=2, behind=2)
+    d["block_table"][::5, 0] = -1                              # pages that are not there
+    check_append(d)
 
 
 @pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F8), (BF16, BF16)])
