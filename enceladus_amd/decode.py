@@ -685,7 +685,13 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
               ("EK_PAD", int(dim != width)))
     log2e = 1.4426950408889634
-    launches = [("ek_paged_attention", (items + batch, y), 64)]
+    # Heads whose rows share 128-byte lines go to one XCD, whose L2 then reads them once (workgroups
+    # go round the 8 XCDs): 34 sequences of 16 heads of 80 e4m3, 32.5 us without this and 25.5 with
+    # it. Whole lines: 14 sequences of 16 heads of 128 bf16, 13.9 without and 14.8 with it.
+    x = items + batch
+    if dim * kc.size % 128:
+        x = -(-x // 8) * 8
+    launches = [("ek_paged_attention", (x, y), 64)]
     workspace = 0
     if most > _MIN_UNITS:              # some sequence may have more than one chunk
         workspace = (items + batch) * heads * (dim + 2) * 4 + batch * 8
