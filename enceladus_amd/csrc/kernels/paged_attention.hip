@@ -35,7 +35,8 @@
 // merge in the LDS (they start and end together).
 //
 // Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_FP8 (the cache is e4m3), EK_DP (64, 128 or 256: the
-// head dimension it is compiled for), EK_PAD (the head dimension is smaller than EK_DP).
+// head dimension it is compiled for), EK_PAD (the head dimension is smaller than EK_DP), EK_KT
+// (keys per wave and step: 16, 32 or 64).
 #include "enceladus_cdna4.h"
 
 #if EK_Q == 0
@@ -48,13 +49,7 @@ typedef ek::bf16 T;
 constexpr int DP = EK_DP;
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
 constexpr float LN2 = 0.69314718055994531f;
-// Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that; of an
-// e4m3 cache twice as many, whose conversions and scores cost more per byte than their loads.
-// Measured at their best numbers of waves: 64 ragged sequences, 501 MB of bf16, heads of 128:
-// 16 keys 88.3 us, 32 89.7 (and 177 registers instead of 125), 64 105; 24 ragged sequences,
-// 153 MB of e4m3: 16 keys 50.7 us, 32 46.4, 64 43.4.
-constexpr int KT0 = EK_FP8 ? 8192 / DP : 4096 / (DP * CS);
-constexpr int KT = KT0 < 16 ? 16 : KT0 > (EK_FP8 ? 64 : 32) ? (EK_FP8 ? 64 : 32) : KT0;
+constexpr int KT = EK_KT;                           // keys per wave and step
 constexpr int ST = KT / 16;                         // score tiles
 constexpr int KE = 16 / CS;                         // elements of a 16-byte key load
 constexpr int KL = DP / (4 * KE);                   // key loads per score tile and lane

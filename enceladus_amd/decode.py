@@ -578,6 +578,21 @@ _STREAM = 256 << 20                # bytes of caches that do not stay in the las
 _WAVES = 8
 
 
+def _step(width: int, size: int, short: bool) -> int:
+    """Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that; of
+    an e4m3 cache twice as many, whose conversions and scores cost more per byte than their loads.
+    Measured at their best numbers of waves: 64 ragged sequences, 501 MB of bf16, heads of 128:
+    16 keys 87.7 us, 32 89.8 (and 187 registers instead of 123), 64 118; 24 ragged sequences, 153 MB
+    of e4m3: 16 keys 50.7 us, 32 46.4, 64 43.4. `short`: no wave will have many, so that fewer waits
+    count for more: one sequence of 1999 tokens, bf16 10.7 us with 16 keys, 9.9 with 32, 11.1 with 64;
+    46 sequences of at most 317 12.4, 11.4 and 14.1."""
+    if size == 1:
+        return max(16, min(64, 8192 // width))
+    if short and width * size == 256:
+        return 32
+    return max(16, min(32, 4096 // (width * size)))
+
+
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float | None = None,
                     window: int = 0, softcap: float = 0.0, k_scale: float = 1.0,
                     v_scale: float = 1.0, out=None, return_lse: bool = False):
@@ -683,7 +698,8 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     items = max(1, min(_WAVES * C.coarsen_cap() // y, batch * -(-most // _MIN_UNITS)))
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
     macros = (("EK_Q", _Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
-              ("EK_PAD", int(dim != width)))
+              ("EK_PAD", int(dim != width)),
+              ("EK_KT", _step(width, kc.size, batch * most <= 8 * items)))
     log2e = 1.4426950408889634
     # Heads whose rows share 128-byte lines go to one XCD, whose L2 then reads them once (workgroups
     # go round the 8 XCDs): 34 sequences of 16 heads of 80 e4m3, 32.5 us without this and 25.5 with
@@ -875,8 +891,11 @@ def specializations():
     for q, fp8 in ((2, 0), (1, 0), (0, 0), (2, 1), (1, 1)):
         for width in (64, 128, 256):
             for pad in (0, 1):
-                yield "paged_attention.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_DP", width),
-                                              ("EK_PAD", pad))
+                size = 1 if fp8 else 2 if q else 4
+                for keys in sorted({_step(width, size, short) for short in (False, True)}):
+                    yield "paged_attention.hip", (("EK_Q", q), ("EK_FP8", fp8),
+                                                  ("EK_DP", width), ("EK_PAD", pad),
+                                                  ("EK_KT", keys))
         for pairs in (0, 1):
             for stream in (0, 1):
                 yield "append_kv.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_V", 8 if q else 4),
