@@ -29,7 +29,7 @@
 //
 // Measured, both kernels: 64 ragged sequences, 8 key heads of 128, 32 query heads, bf16, 501 MB: 88
 // us, 5.7 TB/s; one sequence of 131075, fp16, 537 MB: 93 us, 5.8 (a kernel that only reads: 6.0
-// to 6.2). One sequence of 1999: 7.6 + 3.4 us, a chain of lengths, table, keys, then the join's.
+// to 6.2). One sequence of 1999: 6.7 + 3.4 us, a chain of lengths, table, keys, then the join's.
 // Joining in the first kernel, by the last wave of a sequence to arrive, took longer (18 instead
 // of 12 us there: its counters are as far away as memory), and so did workgroups of 4 waves that
 // merge in the LDS (they start and end together).
