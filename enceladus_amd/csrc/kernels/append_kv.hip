@@ -105,19 +105,26 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
 
   int b = t, back = 1;               // the sequence, and how far before its end the token is
   if (a.cu) {
+    // sequences that end before the token: of many, first the stretches whose last one does
+    const auto ends = [&](int i) { return a.cu[((i < a.batch ? i : a.batch - 1) + 1) * a.cu_step]; };
     b = 0;
-    for (int i = 0; i < a.batch; i += 256) {
-      int end[4];                    // on their way at once
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int at = i + k * 64 + lane;
-        end[k] = a.cu[((at < a.batch ? at : a.batch - 1) + 1) * a.cu_step];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        b += __builtin_popcountll(
-            __builtin_amdgcn_ballot_w64(i + k * 64 + lane < a.batch && end[k] <= t));
+    int count = a.batch;
+    while (count > 256) {
+      const int step = (count + 63) / 64, at = (lane + 1) * step - 1;
+      const int over = __builtin_popcountll(
+          __builtin_amdgcn_ballot_w64(ends(b + at) <= t && at < count));
+      b += over * step;
+      count = count - over * step < step ? count - over * step : step;
     }
+    int end[4];                      // on their way at once
+#pragma unroll
+    for (int k = 0; k < 4; ++k) end[k] = ends(b + k * 64 + lane);
+    int over = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      over += __builtin_popcountll(
+          __builtin_amdgcn_ballot_w64(k * 64 + lane < count && end[k] <= t));
+    b += over;
     if (b >= a.batch) return;
   }
   int len = a.lens[b * a.lens_step];

@@ -508,6 +508,7 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         cu = _array("cu_tokens", cu_tokens, ("i32",), 1, dense=False)
         _need(cu.shape[0] > 0, "`cu_tokens` must have one entry more than there are sequences")
         batch = cu.shape[0] - 1
+    _need(batch <= 1 << 25, f"at most {1 << 25} sequences are supported, got {batch}")
     bt, sl = _sequences(block_table, seq_lens, batch)
     capacity = _capacity(bt, kc)
     qa = qo = None
@@ -667,8 +668,8 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, scale, window, s
     _head_dim(dim, kc.kind)
     _need(kv_heads > 0 and heads % kv_heads == 0,
           f"{heads} query heads are not a multiple of {kv_heads} key heads")
-    _need(heads <= 65535 and batch <= 1 << 20,
-          f"at most 65535 query heads and {1 << 20} sequences are supported, got {heads}, {batch}")
+    _need(heads <= 65535 and batch <= 1 << 16,
+          f"at most 65535 query heads and {1 << 16} sequences are supported, got {heads}, {batch}")
     bt, sl = _sequences(block_table, seq_lens, batch)
     capacity = _capacity(bt, kc)
     scale = 1.0 / math.sqrt(dim) if scale is None else scale

@@ -56,6 +56,10 @@ ATTEND = [
     (dict(q=torch.zeros(1, 8, 64).expand(1 << 16, 8, 64),
           block_table=torch.zeros(1, 1 << 15, dtype=torch.int32).expand(1 << 16, 1 << 15),
           seq_lens=torch.zeros(1, dtype=torch.int32).expand(1 << 16)), ValueError, "in all"),
+    (dict(q=torch.zeros(1, 8, 64).expand((1 << 16) + 1, 8, 64),
+          block_table=torch.zeros(1, 4, dtype=torch.int32).expand((1 << 16) + 1, 4),
+          seq_lens=torch.zeros(1, dtype=torch.int32).expand((1 << 16) + 1)), ValueError,
+     "65536 sequences"),
     (dict(seq_lens=torch.ones(4, dtype=torch.int32)), ValueError, "`seq_lens`"),
     (dict(seq_lens=np.ones(3, np.float32)), TypeError, "`seq_lens`"),
     (dict(seq_lens=np.ones(3, np.int32)[::-1]), ValueError, "negative strides"),
@@ -106,6 +110,8 @@ def test_paged_attention_refuses_overlap():
 
 
 APPEND = [
+    (dict(cu_tokens=torch.zeros(1, dtype=torch.int32).expand((1 << 25) + 2)), ValueError,
+     "sequences are supported"),
     (dict(k=torch.zeros(3, 2, 64, dtype=torch.int32)), TypeError, "`k` must hold"),
     (dict(v=torch.zeros(3, 2, 32)), ValueError, "`v` must have shape"),
     (dict(k_cache=torch.zeros(10, 16, 3, 64)), ValueError, "`k_cache`"),

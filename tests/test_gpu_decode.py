@@ -417,11 +417,13 @@ def test_append_many_rows_of_many_tokens(heads, dim, rotary, behind):
                              behind=behind))
 
 
-@pytest.mark.parametrize("batch", [256, 257, 600])
+@pytest.mark.parametrize("batch", [256, 257, 600, 16384, 16385, 20011])
 def test_append_single_tokens_of_many_sequences(batch):
     gen = torch.Generator().manual_seed(batch)
-    new = [1] * batch
+    new = [1] * batch if batch < 1000 else \
+        (torch.rand(batch, generator=gen) < 0.05).int().tolist()
     new[3:40] = [0] * 37
+    new[-1] = 1
     lens = [n + int(torch.randint(0, 20, (1,), generator=gen)) for n in new]
     d = append_case(gen, F16, F8, lens, new, 16, 2, 2, 64, 64, before=2, behind=2)
     d["block_table"][::5, 0] = -1                              # pages that are not there
