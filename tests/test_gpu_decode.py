@@ -290,6 +290,68 @@ def test_attention_of_a_long_sequence_is_split_and_joined():
     assert torch.equal(a, check_attention(q, kc, vc, bt, lens))       # the same bits again
 
 
+def attention_variant(call):
+    """What `call` returns, and the macros of the one attention kernel that it planned."""
+    decode._plans.clear()
+    got = call()
+    plans = [p for p in decode._plans.values() if p.file == "paged_attention.hip"]
+    assert len(plans) == 1
+    return got, dict(plans[0].macros)
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 128), (BF16, 128), (F16, 80), (BF16, 80), (F32, 64),
+                                       (F32, 48)])
+@pytest.mark.parametrize("window,softcap,scale", [(0, 0.0, None), (1200, 0.0, -0.2),
+                                                  (1300, 8.0, 0.3)])
+def test_attention_16_keys_a_step(dtype, dim, window, softcap, scale, monkeypatch):
+    """The step of large calls (here: of a block table far wider than the lengths), with either
+    kind of loads: the same bits."""
+    gen = torch.Generator().manual_seed(dim + window)
+    lens, page, kv = [3000, 0, 1, 777, 64, 2000, 17], 16, 32
+    bt, pages = table_for(gen, lens, page, width=190)
+    bt[3, 5] = -1                                           # a page that is not there
+    kc, vc = (only_live(cache(gen, pages, page, kv, dim, dtype), bt, lens, page) for _ in "kv")
+    q = rand(gen, len(lens), kv, dim, dtype=dtype)
+    got = []
+    for size in (1 << 62, 0):
+        monkeypatch.setattr(decode, "_STREAM", size)
+        x, macros = attention_variant(lambda: check_attention(
+            q, kc, vc, bt, lens, window=window, softcap=softcap, scale=scale))
+        assert macros["EK_KT"] == 16 and macros["EK_PAD"] == (dim in (80, 48))
+        got.append(x)
+    decode._plans.clear()
+    assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("dim", [64, 80, 128, 200])
+@pytest.mark.parametrize("window,softcap,scale", [(1, 0.0, None), (64, 20.0, None),
+                                                  (100, 0.0, -0.2), (1000, 5.0, -1.0),
+                                                  (0, 50.0, 0.0)])
+def test_attention_fp16_window_softcap_scale(dim, window, softcap, scale):
+    gen = torch.Generator().manual_seed(window + dim)
+    bt, pages = table_for(gen, LENS, 16)
+    kc, vc = (only_live(cache(gen, pages, 16, 2, dim, F16), bt, LENS, 16) for _ in "kv")
+    check_attention(rand(gen, len(LENS), 8, dim, dtype=F16), kc, vc, bt, LENS, window=window,
+                    softcap=softcap, scale=scale)
+
+
+@pytest.mark.parametrize("batch", [256, 257, 320, 1000])
+@pytest.mark.parametrize("empty", ["none", "first", "last", "some", "all"])
+def test_attention_beyond_256_sequences(batch, empty):
+    """With sequences of several chunks among them, and empty ones in the first 256, behind
+    them, in both."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(1, 80, (batch,), generator=gen).tolist()
+    lens[7::60] = [900] * len(lens[7::60])
+    none = {"none": range(0), "first": range(3, 250, 2), "last": range(251, batch),
+            "some": range(0, batch, 3), "all": range(batch)}[empty]
+    for b in none:
+        lens[b] = 0
+    bt, pages = table_for(gen, lens, 16)
+    kc, vc = (only_live(cache(gen, pages, 16, 1, 64, BF16), bt, lens, 16) for _ in "kv")
+    check_attention(rand(gen, batch, 2, 64, dtype=BF16), kc, vc, bt, lens)
+
+
 # -- appending ------------------------------------------------------------------------------
 
 def append_case(gen, dtype, cdtype, lens, new, page, kv, heads, dim, rotary, layout="token",
