@@ -61,7 +61,8 @@ constexpr int VR = KT / 4;                          // value rows per lane
 constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value load
 constexpr bool PACKS = EK_FP8 && ST > 1;            // see the softmax of few heads
 constexpr int UNIT = 16;                            // keys: what chunks are multiples of
-// Weights are exp2(s - m + LIFT). Fp16 has no more than 24 binary places below 1: lifted to
+// Weights are exp2(s - m + LIFT), with the difference taken of the scores as the product gave them
+// (or capped) and scaled after that: the largest is 2^LIFT exactly, however large the scores are. Fp16 has no more than 24 binary places below 1: lifted to
 // 2^14, a weight keeps them down to 2^-39 of the largest one (131072 keys of a weight of 2^-26
 // each are 0.2% of the sum). bf16 and fp32 have the exponents for it.
 constexpr float LIFT = EK_Q == 1 ? 14.0f : 0.0f;
@@ -85,8 +86,9 @@ struct Params {
   const int32_t* lens;
   T* out;
   float* lse;
-  float* part;   // [item][head][dim]: O; then [item][head][2]: m, l; then [sequence][2] words:
-                 // its first item and how many; or null: no sequence has two chunks
+  float* part;   // [item][head][dim]: O; then [item][head][2]: m (not scaled), l; then
+                 // [sequence][2] words: its first item and how many; or null: no sequence has
+                 // two chunks
   int64_t q_row, q_head, out_row, out_head;   // elements
   int64_t c_page, c_token, c_head;   // bytes
   int64_t table_row, lens_step;      // elements
@@ -318,19 +320,22 @@ EK_INLINE int group_of(int chunks) {
 // A head's value: o f, rounded once to T.
 EK_INLINE T result(float o, float f, bool any) { return ek::cvt<T>(any ? o * f : 0.0f); }
 
+// What differences of the running maxima are multiplied by for exp2: capped scores are in log2 units.
+EK_INLINE float scale_of(const Params& a) { return a.cap > 0.0f ? 1.0f : a.scale; }
+
 EK_INLINE float* part_ml(const Params& a) {
   return a.part + (int64_t)(a.items + a.batch) * a.heads * a.dim;
 }
 
 // The weights of up to 16 parts (m, l) of a head, one in each lane of a group of 16 (m -inf
 // where there is none): m and l become the whole's, in all 16 lanes.
-EK_INLINE float weigh16(float& m, float& l) {
+EK_INLINE float weigh16(float& m, float& l, float scale) {
   const float mine = m;
   m = ek::reduce_xor<ek::Max, 1>(m);
   m = ek::reduce_xor<ek::Max, 2>(m);
   m = ek::reduce_xor<ek::Max, 4>(m);
   m = ek::reduce_xor<ek::Max, 8>(m);
-  const float w = ek::exp2_fast(mine - (m == -__builtin_inff() ? 0.0f : m));
+  const float w = ek::exp2_fast((mine - (m == -__builtin_inff() ? 0.0f : m)) * scale);
   l *= w;
   l = ek::reduce_xor<ek::Sum, 1>(l);
   l = ek::reduce_xor<ek::Sum, 2>(l);
@@ -403,7 +408,7 @@ ek_paged_attention(Params a) {
 
   // what the scores are multiplied by for exp2: positive, since the queries took the sign
   const float to_cap = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
-  const float scale = a.cap > 0.0f ? 1.0f : a.scale;
+  const float scale = scale_of(a);
   float m = -__builtin_inff(), l = 0.0f;
   ek::f32x4 o[PANELS][VE];
 #pragma unroll
@@ -493,8 +498,7 @@ ek_paged_attention(Params a) {
       id = page_id(next + KT);
       load_k(t, off);
     }
-    // softmax: scores stay as the product gave them (or capped, in log2 units) until exp2, whose
-    // argument is one fma of them; m is in log2 units
+    // softmax: scores and m stay as the product gave them (or capped, in log2 units) until exp2
     const bool full = live == ~0ull;
     const auto soften = [&](auto& x, const auto& key_of) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
@@ -518,10 +522,10 @@ ek_paged_attention(Params a) {
         for (int i = 0; i < 4; ++i) mt = __builtin_fmaxf(mt, x[s][i]);
       if constexpr (N < ST) mt = __builtin_fmaxf(mt, half_row(mt));
       mt = ek::reduce_xor<ek::Max, 16>(mt);
-      mt = ek::reduce_xor<ek::Max, 32>(mt) * scale;
+      mt = ek::reduce_xor<ek::Max, 32>(mt);
       const float m_new = __builtin_fmaxf(m, mt);
       const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-      const float alpha = ek::exp2_fast(m - m_use);
+      const float alpha = ek::exp2_fast((m - m_use) * scale);
       m = m_new;
       // most steps raise no head's maximum
       if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
@@ -535,7 +539,7 @@ ek_paged_attention(Params a) {
       for (int s = 0; s < N; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[s][i] = ek::exp2_fast(__builtin_fmaf(x[s][i], scale, LIFT - m_use));
+          x[s][i] = ek::exp2_fast(__builtin_fmaf(x[s][i] - m_use, scale, LIFT));
           l += x[s][i];
         }
     };
@@ -665,7 +669,7 @@ ek_paged_attention(Params a) {
       }
     if (a.lse && c == 0)
       a.lse[(int64_t)b * a.heads + head] =
-          any ? (m - LIFT + __builtin_log2f(l)) * LN2 : -__builtin_inff();
+          any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
   } else {
     const int64_t at = (int64_t)blockIdx.x * a.heads + head;
     float* dst = a.part + at * a.dim;
@@ -684,7 +688,7 @@ ek_paged_attention(Params a) {
       }
     if (c == 0) {
       float* ml = part_ml(a) + at * 2;
-      ml[0] = m - LIFT;
+      ml[0] = m;
       ml[1] = l;
     }
   }
@@ -704,6 +708,7 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
   const int32_t* info = (const int32_t*)(ml + (int64_t)(a.items + a.batch) * a.heads * 2);
   const int start = info[2 * b], chunks = info[2 * b + 1];
   if (chunks <= 1) return;
+  const float scale = scale_of(a);
   const int gs = group_of(chunks), groups = (chunks + gs - 1) / gs;
   float x[DW][2];
   for (int group = wave; group < groups; group += waves) {
@@ -735,11 +740,11 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
       __builtin_amdgcn_sched_barrier(0);           // all of them before the first wait
       m = i < count ? m : -__builtin_inff();
       l = i < count ? l : 0.0f;
-      float w = weigh16(m, l);
+      float w = weigh16(m, l, scale);
       // onto what came before (with more than 16 chunks)
       const float m_new = __builtin_fmaxf(mm, m);
       const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-      const float f = ek::exp2_fast(mm - mu), part = ek::exp2_fast(m - mu);
+      const float f = ek::exp2_fast((mm - mu) * scale), part = ek::exp2_fast((m - mu) * scale);
       w *= part;
       ll = __builtin_fmaf(ll, f, l * part);
       mm = m_new;
@@ -773,7 +778,7 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
   float m = (lane & 15) < groups ? s_m[lane & 15] : -__builtin_inff();
   float l = (lane & 15) < groups ? s_l[lane & 15] : 0.0f;
   if (groups > 1) {
-    const float w = weigh16(m, l);
+    const float w = weigh16(m, l, scale);
 #pragma unroll
     for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
     for (int j = 0; j < groups; ++j) {
@@ -803,5 +808,5 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
   }
   if (a.lse && lane == 0)
     a.lse[(int64_t)b * a.heads + head] =
-        any ? (m + __builtin_log2f(l)) * LN2 : -__builtin_inff();
+        any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
 }

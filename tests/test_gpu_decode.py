@@ -352,6 +352,35 @@ def test_attention_beyond_256_sequences(batch, empty):
     check_attention(rand(gen, batch, 2, 64, dtype=BF16), kc, vc, bt, lens)
 
 
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F16), (BF16, BF16), (F16, F8),
+                                          (BF16, F8)])
+@pytest.mark.parametrize("dim", [16, 128])
+@pytest.mark.parametrize("scale", [1e6, 1e8, -1e10, 2.0 ** 40, 2.0 ** 60])
+def test_attention_of_large_scores(dtype, cdtype, dim, scale):
+    """Scores far apart in sequences of one chunk and of several: the largest ones, which are
+    equal, share the weight. Products of small whole numbers are exact and differ by 1 at least,
+    so every weight is 2^0 or 0: what is left to round are the sums over the keys, the division
+    and a few products, and in the lse a product."""
+    gen = torch.Generator().manual_seed(dim)
+    lens, kv = [1, 50, 64, 65, 700, 1500], 2
+    bt, pages = table_for(gen, lens, 16)
+
+    def whole(*shape):
+        x = torch.randint(-1, 2, shape, generator=gen).float()
+        x[..., 16:] = 0
+        return x
+    kc = only_live(whole(pages, 16, kv, dim).to(cdtype), bt, lens, 16)
+    vc = only_live(cache(gen, pages, 16, kv, dim, cdtype), bt, lens, 16)
+    q = whole(len(lens), kv * 3, dim).to(dtype)
+    kw = dict(scale=scale, k_scale=0.5 if cdtype is F8 else 1.0)
+    want, lse, mag, _ = R.paged_attention(q, kc, vc, bt, lens, **kw)
+    got, got_lse = decode.paged_attention(on_gpu(q), on_gpu(kc), on_gpu(vc), bt.cuda(),
+                                          torch.tensor(lens, dtype=torch.int32).cuda(),
+                                          return_lse=True, **kw)
+    close(got, want, half_step(dtype) * want.abs() + mag * 2 * (1500 + 16) * U + SUB[dtype], "out")
+    close(got_lse, lse, 8 * U * lse.abs() + (1500 + 64) * U, "lse")
+
+
 # -- appending ------------------------------------------------------------------------------
 
 def append_case(gen, dtype, cdtype, lens, new, page, kv, heads, dim, rotary, layout="token",
