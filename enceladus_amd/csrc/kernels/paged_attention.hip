@@ -19,8 +19,10 @@
 //   elements of those keys' values from element VE r on; the m-th product takes element VE r + m
 //   of them, so that the VE products cover 16 VE elements of the head without any transpose
 //   through the LDS (a register permute pairs the keys).
-// - The weights are split into two terms of the 16-bit type (p = hi + lo), two products each:
-//   the matrix units idle anyway, and the output keeps the accuracy of 32-bit weights.
+// - The weights are split into terms of the values' 16-bit type, a product each (the matrix units
+//   idle anyway), so that they are rounded about as 32-bit ones are (2^-24): three bf16 terms leave
+//   2^-24 of a weight, two fp16 terms 2^-22. e4m3 values are exact in fp16, whose two terms take
+//   bf16 queries' weights as well.
 //
 // Work: a chunk of one sequence is an item; one wave takes an item of one key head, by itself.
 // The chunks' length comes from all sequences' lengths, on the device, so that ragged batches
@@ -61,11 +63,14 @@ constexpr int VR = KT / 4;                          // value rows per lane
 constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value load
 constexpr bool PACKS = EK_FP8 && ST > 1;            // see the softmax of few heads
 constexpr int UNIT = 16;                            // keys: what chunks are multiples of
-// Weights are exp2(s - m + LIFT), with the difference taken of the scores as the product gave them
-// (or capped) and scaled after that: the largest is 2^LIFT exactly, however large the scores are. Fp16 has no more than 24 binary places below 1: lifted to
-// 2^14, a weight keeps them down to 2^-39 of the largest one (131072 keys of a weight of 2^-26
-// each are 0.2% of the sum). bf16 and fp32 have the exponents for it.
-constexpr float LIFT = EK_Q == 1 ? 14.0f : 0.0f;
+// Weights are exp2(s - m), with the difference taken of the scores as the product gave them (or
+// capped) and scaled after that: the largest is 1 exactly, however large the scores are. Fp16 has
+// no more than 24 binary places below 1: terms lifted by 2^14 keep a weight down to 2^-39 of the
+// largest one (131072 keys of a weight of 2^-26 each are 0.2% of the sum). bf16 and fp32 have the
+// exponents for it.
+constexpr bool HALF = EK_Q == 1 || EK_FP8;          // the weights' terms are fp16
+constexpr int TERMS = HALF ? 2 : 3;
+constexpr float LIFT = HALF ? 0x1p14f : 1.0f;
 
 typedef uint32_t u32;
 template <int W> struct words { u32 w[W]; };
@@ -86,7 +91,7 @@ struct Params {
   const int32_t* lens;
   T* out;
   float* lse;
-  float* part;   // [item][head][dim]: O; then [item][head][2]: m (not scaled), l; then
+  float* part;   // [item][head][dim]: O (lifted); then [item][head][2]: m (not scaled), l; then
                  // [sequence][2] words: its first item and how many; or null: no sequence has
                  // two chunks
   int64_t q_row, q_head, out_row, out_head;   // elements
@@ -236,46 +241,31 @@ EK_INLINE float tanh_f(float x) {
 }
 
 #if EK_FP8
-// Four e4m3 values as four 16-bit ones (exact).
-EK_INLINE void widen4(u32 w, u32* lo, u32* hi) {
-#if EK_Q == 1
-  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
-  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
-#else
-  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
-  const auto b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
-#endif
-  *lo = __builtin_bit_cast(u32, a);
-  *hi = __builtin_bit_cast(u32, b);
+// Four e4m3 values as four fp16 ones, or bf16 ones (exact).
+template <bool FP16> EK_INLINE void widen4(u32 w, u32* lo, u32* hi) {
+  if constexpr (FP16) {
+    *lo = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    *hi = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  } else {
+    *lo = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    *hi = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+  }
 }
 #endif
 
 #if EK_Q != 0
 // acc += a b over 32 k values: four words of 16-bit pairs per lane and operand.
-EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32* b) {
-#if EK_Q == 1
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ek::pack<ek::f16x8>(a), ek::pack<ek::f16x8>(b),
-                                               acc, 0, 0, 0);
-#else
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ek::pack<ek::bf16x8>(a), ek::pack<ek::bf16x8>(b),
-                                                acc, 0, 0, 0);
-#endif
+template <bool FP16> EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32* b) {
+  if constexpr (FP16)
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ek::pack<ek::f16x8>(a), ek::pack<ek::f16x8>(b),
+                                                 acc, 0, 0, 0);
+  else
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ek::pack<ek::bf16x8>(a),
+                                                  ek::pack<ek::bf16x8>(b), acc, 0, 0, 0);
 }
-// The same over 16 k values: two words per lane and operand.
-EK_INLINE void mma16(ek::f32x4& acc, const u32* a, const u32* b) {
-#if EK_Q == 1
-  acc = __builtin_amdgcn_mfma_f32_16x16x16f16(ek::pack<ek::f16x4>(a), ek::pack<ek::f16x4>(b),
-                                              acc, 0, 0, 0);
-#else
-  acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(ek::pack<ek::s16x4>(a), ek::pack<ek::s16x4>(b),
-                                                  acc, 0, 0, 0);
-#endif
-}
-#if EK_Q == 1
-typedef _Float16 half_t;
-#else
-typedef __bf16 half_t;
-#endif
+template <bool FP16> struct half_of { typedef __bf16 type; };
+template <> struct half_of<true> { typedef _Float16 type; };
+typedef half_of<HALF>::type half_t;                 // of the weights' terms
 EK_INLINE u32 pack2(half_t a, half_t b) {
   return (u32)__builtin_bit_cast(uint16_t, a) | (u32)__builtin_bit_cast(uint16_t, b) << 16;
 }
@@ -485,11 +475,11 @@ ek_paged_attention(Params a) {
 #elif EK_FP8
         u32 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) widen4(t.k[s][i].w[e], &x[2 * e], &x[2 * e + 1]);
-        mma(acc[s], x, q.w[2 * i]);
-        mma(acc[s], x + 4, q.w[2 * i + 1]);
+        for (int e = 0; e < 4; ++e) widen4<EK_Q == 1>(t.k[s][i].w[e], &x[2 * e], &x[2 * e + 1]);
+        mma<EK_Q == 1>(acc[s], x, q.w[2 * i]);
+        mma<EK_Q == 1>(acc[s], x + 4, q.w[2 * i + 1]);
 #else
-        mma(acc[s], t.k[s][i].w, q.w[i]);
+        mma<EK_Q == 1>(acc[s], t.k[s][i].w, q.w[i]);
 #endif
       }
     }
@@ -539,7 +529,7 @@ ek_paged_attention(Params a) {
       for (int s = 0; s < N; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[s][i] = ek::exp2_fast(__builtin_fmaf(x[s][i] - m_use, scale, LIFT));
+          x[s][i] = ek::exp2_fast((x[s][i] - m_use) * scale);
           l += x[s][i];
         }
     };
@@ -569,13 +559,19 @@ ek_paged_attention(Params a) {
                                                          acc[j / 4][j & 3], o[p][e], 0, 0, 0);
 #else
     constexpr int SS = ST == 1 ? 1 : 2;            // score tiles of a product
-    u32 hi_p[ST / SS][2 * SS], lo_p[ST / SS][2 * SS];
-    const auto split = [&](const ek::f32x4& x, u32* ph, u32* pl) {
+    u32 w_p[TERMS][ST / SS][2 * SS];
+    // the weights' terms from word `at` on: each is what the ones before it leave, rounded
+    const auto split = [&](const ek::f32x4& x, int at) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const half_t h0 = (half_t)x[2 * i], h1 = (half_t)x[2 * i + 1];
-        ph[i] = pack2(h0, h1);
-        pl[i] = pack2((half_t)(x[2 * i] - (float)h0), (half_t)(x[2 * i + 1] - (float)h1));
+        float x0 = x[2 * i] * LIFT, x1 = x[2 * i + 1] * LIFT;
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+          const half_t h0 = (half_t)x0, h1 = (half_t)x1;
+          w_p[k][at / (2 * SS)][at % (2 * SS) + i] = pack2(h0, h1);
+          x0 -= (float)h0;
+          x1 -= (float)h1;
+        }
       }
     };
     if constexpr (PACKS) {
@@ -592,25 +588,22 @@ ek_paged_attention(Params a) {
         soften(x, [&](int s) { return s * 32 + (r >> 3) * 16 + c * 4; });
 #pragma unroll
         for (int s = 0; s < ST / 2; ++s) {
-          split(x[s], hi_p[s], lo_p[s]);
+          split(x[s], s * 4);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            hi_p[s][2 + i] = to_lower_half(hi_p[s][i]);
-            lo_p[s][2 + i] = to_lower_half(lo_p[s][i]);
-          }
+          for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w_p[k][s][2 + i] = to_lower_half(w_p[k][s][i]);
         }
       }
     }
     if (!PACKS || nh > 8) {
       soften(acc, own);
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
-        split(acc[s], hi_p[s / SS] + s % SS * 2, lo_p[s / SS] + s % SS * 2);
+      for (int s = 0; s < ST; ++s) split(acc[s], s * 2);
     }
     clear_absent();
 #pragma unroll
     for (int s = 0; s < ST; s += SS) {
-      const u32 *ph = hi_p[s / SS], *pl = lo_p[s / SS];
 #pragma unroll
       for (int p = 0; p < PANELS; ++p) {
         // 4 SS keys' VE elements, 16 bits each
@@ -620,7 +613,7 @@ ek_paged_attention(Params a) {
           const words<VW>& v = t.v[s * 4 + j][p];
 #if EK_FP8
 #pragma unroll
-          for (int w = 0; w < VW; ++w) widen4(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
+          for (int w = 0; w < VW; ++w) widen4<HALF>(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
 #else
 #pragma unroll
           for (int w = 0; w < VW; ++w) x[j][w] = v.w[w];
@@ -634,11 +627,19 @@ ek_paged_attention(Params a) {
             w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
                                          e & 1 ? 0x07060302u : 0x05040100u);
           if constexpr (SS == 2) {
-            mma(o[p][e], w, ph);
-            mma(o[p][e], w, pl);
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) mma<HALF>(o[p][e], w, w_p[k][s / SS]);
           } else {
-            mma16(o[p][e], w, ph);
-            mma16(o[p][e], w, pl);
+            // 16 keys: a product over 32 for the first term and one for the others, which next to
+            // the first would lose digits in the product's own sum (64 ragged sequences, bf16: off
+            // from 32-bit sums by 4.0e-5 of the result's norm with the first two together, 2.6e-5 so)
+            const u32 twice[4] = {w[0], w[1], w[0], w[1]};
+            const u32 first[4] = {w_p[0][s][0], w_p[0][s][1], 0, 0};
+            const u32 rest[4] = {w_p[1][s][0], w_p[1][s][1],
+                                 TERMS > 2 ? w_p[TERMS - 1][s][0] : 0,
+                                 TERMS > 2 ? w_p[TERMS - 1][s][1] : 0};
+            mma<HALF>(o[p][e], twice, first);
+            mma<HALF>(o[p][e], twice, rest);
           }
         }
       }
@@ -655,7 +656,7 @@ ek_paged_attention(Params a) {
   const int head = g * a.group + h0 + r;
   if (chunks == 1) {
     const bool any = l > 0.0f || l != l;
-    const float f = any ? a.v_scale / l : 0.0f;
+    const float f = any ? a.v_scale / LIFT / l : 0.0f;
     T* dst = a.out + b * a.out_row + head * a.out_head;
 #pragma unroll
     for (int p = 0; p < PANELS; ++p)
@@ -669,7 +670,7 @@ ek_paged_attention(Params a) {
       }
     if (a.lse && c == 0)
       a.lse[(int64_t)b * a.heads + head] =
-          any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
+          any ? (m * scale + __builtin_log2f(l)) * LN2 : -__builtin_inff();
   } else {
     const int64_t at = (int64_t)blockIdx.x * a.heads + head;
     float* dst = a.part + at * a.dim;
@@ -796,7 +797,7 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
   m = lane_value(m, 0);
   l = lane_value(l, 0);
   const bool any = l > 0.0f || l != l;
-  const float f = any ? a.v_scale / l : 0.0f;
+  const float f = any ? a.v_scale / LIFT / l : 0.0f;
   T* dst = a.out + b * a.out_row + head * a.out_head;
 #pragma unroll
   for (int k = 0; k < DW; ++k) {
@@ -808,5 +809,5 @@ extern "C" __global__ __launch_bounds__(1024) void ek_paged_attention_join(Param
   }
   if (a.lse && lane == 0)
     a.lse[(int64_t)b * a.heads + head] =
-        any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
+        any ? (m * scale + __builtin_log2f(l)) * LN2 : -__builtin_inff();
 }

@@ -381,6 +381,37 @@ def test_attention_of_large_scores(dtype, cdtype, dim, scale):
     close(got_lse, lse, 8 * U * lse.abs() + (1500 + 64) * U, "lse")
 
 
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F16), (BF16, BF16), (F16, F8),
+                                          (BF16, F8)])
+@pytest.mark.parametrize("group", [4, 16])
+def test_attention_weights_keep_32_bits(dtype, cdtype, group):
+    """Two nearly equal weights w1, w2 of 0.37 to 0.61 whose values are 1 and -1, beside a weight
+    of 1 whose value is 0: the result, (w1 - w2) / (1 + w1 + w2), is about 2^-16, so that it shows
+    the weights' errors of 2^-24 and not its own rounding.
+
+    In units of U = 2^-24: the scores are exact; their product with the scale, and that one's
+    own rounding, put 2 U of up to 0.73 into the exponent, exp2 is off by at most 2 U of the
+    weight: 0.61 (0.73 * 2 + 2) = 2.2 U for each weight, 4.4 U for both. fp16's two terms add
+    2^-22 = 4 U of it, 4.9 U for both. The two products' sums are below 1, their terms (up to 6)
+    are added with 1 U each or, if the matrix unit cuts off, 2 U: 12 U. All that is divided by
+    1 + w1 + w2 >= 1.73: 12.4 U. Errors of the divisor count by the result, 2^-16."""
+    gen = torch.Generator().manual_seed(group)
+    batch, dim = 64, 16
+    kc, vc = (torch.zeros(1, 16, 1, dim) for _ in "kv")
+    kc[0, 1, 0, 0] = kc[0, 2, 0, 0] = kc[0, 2, 0, 1] = 1.0
+    vc[0, 1], vc[0, 2] = 1.0, -1.0
+    kc, vc = kc.to(cdtype), vc.to(cdtype)
+    q = torch.zeros(batch, group, dim)
+    q[..., 0] = -torch.rand(batch, group, generator=gen) / 2 - 0.5
+    q[..., 1] = -torch.rand(batch, group, generator=gen) * 2.0 ** -14
+    q = q.to(dtype)
+    bt, lens = torch.zeros(batch, 1, dtype=torch.int32), [3] * batch
+    want, _, _, _ = R.paged_attention(q, kc, vc, bt, lens, scale=1.0)
+    got = decode.paged_attention(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(),
+                                 torch.tensor(lens, dtype=torch.int32).cuda(), scale=1.0)
+    close(got, want, half_step(dtype) * want.abs() + 12.5 * U, "out")
+
+
 # -- appending ------------------------------------------------------------------------------
 
 def append_case(gen, dtype, cdtype, lens, new, page, kv, heads, dim, rotary, layout="token",
