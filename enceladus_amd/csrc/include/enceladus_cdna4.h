@@ -187,6 +187,13 @@ EK_INLINE float erf_as(float x) {
 
 // 2^x with the hardware v_exp_f32 (1 ulp; results below 2^-126 flush to zero).
 EK_INLINE float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// x / t with one rounding (of quotients above 2^-100), from r = 1 / t, rounded: the remainder of
+// x r corrects it (Markstein 1990). What is not a number other than 0 stays as x r is.
+EK_INLINE float quotient(float x, float t, float r) {
+  const float q = x * r;
+  const float y = __builtin_fmaf(__builtin_fmaf(-q, t, x), r, q);
+  return __builtin_amdgcn_classf(q, 0x198) ? y : q;    // normal or subnormal
+}
 
 // ---------------------------------------------------------------------------
 // Raw vector moves. N is the byte count (1, 2, 4, 8 or 16).

@@ -4,7 +4,7 @@
 // slot is token p % page of page table[b][p / page]. Rotation of the first `rotary` elements of
 // a head, in pairs (x, y) = (j, j + rotary / 2), or (2 j, 2 j + 1) when EK_PAIRS:
 // (x cos - y sin, y cos + x sin) with cos, sin at [p, j]. Cached values are divided by the
-// cache's scale and rounded once (e4m3: saturated to +-448, NaN stays NaN).
+// cache's scale in 32 bits and rounded to its type (e4m3: saturated to +-448, NaN stays NaN).
 //
 // A handful of flops per element: the time is the bytes over the HBM rate, or a launch. A wave
 // takes one token, or a part of its rows (query, key and value heads) when there are few tokens;
@@ -44,7 +44,7 @@ struct Params {
   int64_t table_row, lens_step, cu_step, cos_row, sin_row;
   int32_t tokens, batch, heads, kv_heads, dim, rotary, page, pages, capacity, positions;
   int32_t parts;                     // waves per token
-  float k_inv, v_inv;                // 1 / scale
+  float k_scale, v_scale, k_inv, v_inv;   // and 1 / scale
 };
 
 EK_INLINE float sat8(float x) { return x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x; }
@@ -55,14 +55,14 @@ template <int N, typename S> EK_INLINE void put(S* p, const S* w) {
 }
 
 // V floats into the cache at p.
-EK_INLINE void store_cache(char* p, const float* x, float inv) {
+EK_INLINE void store_cache(char* p, const float* x, float scale, float inv) {
 #if EK_FP8
   uint8_t w[V < 4 ? 4 : V];
 #pragma unroll
   for (int i = 0; i < V; i += 4) {
     float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = i + j < V ? sat8(x[i + j] * inv) : 0.0f;
+    for (int j = 0; j < 4; ++j) y[j] = i + j < V ? sat8(ek::quotient(x[i + j], scale, inv)) : 0.0f;
     int u = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     u = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], u, true);
     __builtin_memcpy(w + i, &u, 4);
@@ -71,7 +71,7 @@ EK_INLINE void store_cache(char* p, const float* x, float inv) {
 #else
   T w[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) w[i] = ek::cvt<T>(x[i] * inv);
+  for (int i = 0; i < V; ++i) w[i] = ek::cvt<T>(ek::quotient(x[i], scale, inv));
   put<V>((T*)p, w);
 #endif
 }
@@ -202,9 +202,9 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
       } else {
         char* dst = (is_k ? a.k_cache : a.v_cache) + slot + h * a.c_head +
                     (int64_t)d * (EK_FP8 ? 1 : sizeof(T));
-        const float inv = is_k ? a.k_inv : a.v_inv;
-        store_cache(dst, x, inv);
-        if (two) store_cache(dst + (int64_t)half * (EK_FP8 ? 1 : sizeof(T)), y, inv);
+        const float scale = is_k ? a.k_scale : a.v_scale, inv = is_k ? a.k_inv : a.v_inv;
+        store_cache(dst, x, scale, inv);
+        if (two) store_cache(dst + (int64_t)half * (EK_FP8 ? 1 : sizeof(T)), y, scale, inv);
       }
     }
   }

@@ -396,9 +396,13 @@ def _f32(x: float) -> float:
     return math.copysign(math.inf, x) if abs(x) > 3.4028234e38 else x
 
 
+def _round32(x: float) -> float:
+    return struct.unpack("<f", struct.pack("<f", x))[0]
+
+
 # -- appending to the cache ----------------------------------------------------------------
 
-_APPEND = struct.Struct("<16q11i2f4x")
+_APPEND = struct.Struct("<16q11i4f4x")
 
 
 # Bytes of rows, more than the L2s hold together, from which on they move past the caches: 21152
@@ -559,7 +563,8 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0],
         cu.strides[0] if cu else 0, ca.strides[0] if ca else 0, sa.strides[0] if sa else 0,
         tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
-        ca.shape[0] if ca else 0, parts, 1.0 / k_scale, 1.0 / v_scale)
+        ca.shape[0] if ca else 0, parts, k_scale, v_scale, 1.0 / _round32(k_scale),
+        1.0 / _round32(v_scale))
     return _Plan("append_kv.hip", macros,
                  [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
                  tail, [(3, 0, True), (3, 1, False), (3, 2, False), (3, 4, False),

@@ -594,6 +594,42 @@ def test_append_rounds_to_8_bits_as_the_type_says():
         assert torch.equal(got.signbit()[~want.isnan()], (sign * want).signbit()[~want.isnan()])
 
 
+@pytest.mark.parametrize("cdtype", [F32, F16, BF16, F8])
+@pytest.mark.parametrize("scale", [0.3, 0.7, 1.9, 2.0 - 2.0 ** -23, 2.0 ** -30 * 1.1, 0.25])
+def test_append_divides_by_the_scale(cdtype, scale):
+    """Cached values are the 32-bit quotients, rounded to the cache's type: around ties, where a
+    product with the reciprocal may fall on the other side."""
+    gen = torch.Generator().manual_seed(8)
+    s = np.float32(scale)
+    dtype = F32 if cdtype is F8 else cdtype
+    if cdtype is F8:
+        grid = torch.arange(256, dtype=torch.uint8).view(F8).float()
+        grid = grid[~grid.isnan()].sort().values
+        mid = ((grid[1:] + grid[:-1]) / 2).numpy() * s
+        x = np.concatenate([mid, np.nextafter(mid, np.float32(1e9)),
+                            np.nextafter(mid, np.float32(-1e9))])
+    else:
+        x = (rand(gen, 64 * 64) * float(s)).to(dtype).float().numpy()
+    x = np.concatenate([x, np.float32([math.inf, -math.inf, math.nan, 0.0, -0.0])])
+    x = np.concatenate([x, np.zeros(-len(x) % 64, np.float32)]).reshape(-1, 1, 64)
+    x = torch.from_numpy(x).to(dtype)
+    n = x.shape[0]
+    kc, vc = (torch.zeros(n, 1, 1, 64, device="cuda").to(cdtype) for _ in "kv")
+    decode.append_kv(x.cuda(), (-x).cuda(), kc, vc,
+                     torch.arange(n, dtype=torch.int32)[:, None].cuda(),
+                     torch.ones(n, dtype=torch.int32).cuda(), k_scale=float(s),
+                     v_scale=float(s))
+    want = torch.from_numpy(x.float().numpy() / s)
+    if cdtype is F8:
+        want = want.clamp(-448, 448)
+    want = want.to(cdtype).float().view(n, 64)
+    for got, sign in ((kc, 1), (vc, -1)):
+        got = got.float().cpu().view(n, 64)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(9, 1e30, -1e30),
+                           (sign * want).nan_to_num(9, 1e30, -1e30))
+
+
 # -- logits ---------------------------------------------------------------------------------
 
 def logits_case(gen, rows, vocab, history=0, biases=0, mask=False, dtype=F32, numbers=False):
