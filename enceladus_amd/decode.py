@@ -764,7 +764,8 @@ def adjust_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None,
                   repetition=None, frequency=None, presence=None, bias_ids=None, bias=None,
                   allowed=None, temperature=None, out=None):
     """Penalties for repeated tokens, biases, a temperature and a mask on rows of logits, in
-    this order, computed in 32 bits and rounded once:
+    this order, computed in 32 bits (where 16-bit logits are divided, by the divisor's 32-bit
+    reciprocal) and rounded once to their type:
 
     1. tokens that occur in the row's history: x / `repetition` where x > 0, else
        x * `repetition`;

@@ -724,6 +724,27 @@ def test_logits_of_temperatures_near_zero():
                                                           2.0 ** -101])))
 
 
+@pytest.mark.parametrize("lift", [0, 60])
+def test_logits_quotients_are_rounded_once(lift):
+    """x / temperature, and x / repetition of positive logits, are the 32-bit quotients."""
+    gen = torch.Generator().manual_seed(7)
+    rows, vocab = 200, 3001
+    x = rand(gen, rows, vocab, scale=4.0)
+    by = torch.rand(rows, generator=gen) * 1.5 + 0.25
+    by[0], by[1], by[2] = 2.0 - 2.0 ** -23, 1.0 + 2.0 ** -23, 1.0
+    x[:, 0], x[:, 1], x[:, 2] = math.inf, -math.inf, 0.0
+    t = (by.double() * 2.0 ** -lift).float()
+    got = decode.adjust_logits(x.cuda(), temperature=t.cuda()).cpu()
+    assert torch.equal(got, (x.double() / t.double()[:, None]).float())
+    tokens = torch.arange(vocab, dtype=torch.int32).expand(rows, -1).contiguous()
+    prompt = torch.full((rows,), vocab, dtype=torch.int32)
+    got = decode.adjust_logits(x.cuda(), tokens=tokens.cuda(), prompt_lens=prompt.cuda(),
+                               repetition=t.cuda()).cpu()
+    r = t.double()[:, None]
+    want = torch.where(x > 0, x.double() / r, x.double() * r).float()
+    assert torch.equal(got, want)
+
+
 def test_logits_strides_shared_masks_and_places():
     gen = torch.Generator().manual_seed(3)
     d = logits_case(gen, 6, 4099, 77, 5, True, F16)
