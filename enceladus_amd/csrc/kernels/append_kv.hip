@@ -134,7 +134,7 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
     if (begin > t) return;
     back = end - t;
   }
-  const int pos = len - back;
+  const int pos = (len > 0 ? len : 0) - back;      // a negative length is none: no wrapping round
   if (pos < 0 || pos >= a.capacity || (a.rotary && pos >= a.positions)) return;
   const int pg = pos / a.page, page_id = a.table[b * a.table_row + pg];
 

@@ -630,6 +630,15 @@ def test_append_divides_by_the_scale(cdtype, scale):
                            (sign * want).nan_to_num(9, 1e30, -1e30))
 
 
+def test_append_far_below_the_first_position():
+    """A length of -2^31 with an end of 2^31 - 1: every position is negative, none wraps round."""
+    gen = torch.Generator().manual_seed(14)
+    d = append_case(gen, F32, F32, [20, 20], [2, 2], 16, 1, 2, 64, 0)
+    d["cu_tokens"] = torch.tensor([0, 2, 2 ** 31 - 1], dtype=torch.int32)
+    d["seq_lens"] = torch.tensor([20, -2 ** 31], dtype=torch.int32)
+    check_append(d)
+
+
 # -- logits ---------------------------------------------------------------------------------
 
 def logits_case(gen, rows, vocab, history=0, biases=0, mask=False, dtype=F32, numbers=False):
