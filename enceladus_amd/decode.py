@@ -336,6 +336,28 @@ def _apart(name: str, out: _Array, other: str, a: _Array, same_ok: bool = True) 
     raise ValueError(f"`{name}` overlaps `{other}`")
 
 
+def _steps(a: _Array) -> list:
+    """(stride, extent, bytes behind it: of the further dimensions and an element, less one) of
+    a's dimensions in bytes, the widest stride first."""
+    dims = sorted(((s * a.size, n) for n, s in zip(a.shape, a.strides) if n > 1), reverse=True)
+    rest = a.size - 1 + sum((n - 1) * s for s, n in dims)
+    found = []
+    for s, n in dims:
+        rest -= (n - 1) * s
+        found.append((s, n, rest))
+    return found
+
+
+def _meet(steps: list, size: int, gap: int) -> bool:
+    """Whether an array of such `_steps` shares bytes with its like `gap` bytes further on: a
+    difference of two of its elements' places is within an element of that."""
+    gaps = [gap]
+    for s, n, rest in steps:
+        gaps = [g - i * s for g in gaps
+                for i in range(max(1 - n, -((rest - g) // s)), min(n - 1, (g + rest) // s) + 1)]
+    return any(abs(g) < size for g in gaps)
+
+
 def _device_of(arrays) -> int:
     """The GPU that the arrays are on: torch's, or -1 where none says one. Refuses two."""
     found = {a.device for _, a in arrays if a is not None and a.device >= 0}
@@ -439,7 +461,8 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     and rows whose position is negative, not covered by the block table or not in `cos`, or
     whose page is not in the cache, are skipped: neither cache nor `q_out` is written for them
     (a new `q_out` holds anything there). Two rows must not share a slot of the cache, and the
-    new keys and values must not lie in it.
+    new keys and values must not lie in it. The caches may lie in one array, as long as they
+    share no element.
 
     With `cos` and `sin`, the first R elements of each key and query head are rotated in pairs,
     (j, j + R / 2), or (2 j, 2 j + 1) when `interleaved`: (x, y) becomes
@@ -480,8 +503,10 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     except (AttributeError, TypeError, RuntimeError):
         key = plan = None              # arrays of another kind, or no arrays
     given = q_out is not None
-    if plan is not None and k_cache.data_ptr() == v_cache.data_ptr():
-        plan = None                    # refused below
+    if plan is not None:
+        gap = v_cache.data_ptr() - k_cache.data_ptr()
+        if abs(gap) < plan.cache_span and _meet(plan.cache_steps, plan.cache_size, gap):
+            plan = None                # refused below
     if plan is None:
         plan, q_out = _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q,
                                    q_out, cos, sin, interleaved, k_scale, v_scale)
@@ -528,7 +553,10 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         _need(q_out is None, "`q_out` is given without `q`")
     _written("k_cache", kc)
     _written("v_cache", vc)
-    _need(kc.address() != vc.address() or not kc.span(), "`k_cache` and `v_cache` are the same")
+    gap, steps = vc.address() - kc.address(), _steps(kc)
+    if abs(gap) < kc.span():
+        _need(gap != 0, "`k_cache` and `v_cache` are the same")
+        _need(not _meet(steps, kc.size, gap), "`k_cache` overlaps `v_cache`")
     _need((cos is None) == (sin is None), "`cos` and `sin` go together")
     ca = sa = None
     rotary = 0
@@ -565,10 +593,12 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
         ca.shape[0] if ca else 0, parts, k_scale, v_scale, 1.0 / _round32(k_scale),
         1.0 / _round32(v_scale))
-    return _Plan("append_kv.hip", macros,
+    plan = _Plan("append_kv.hip", macros,
                  [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
                  tail, [(3, 0, True), (3, 1, False), (3, 2, False), (3, 4, False),
-                        (3, 5, False)]), q_out
+                        (3, 5, False)])
+    plan.cache_span, plan.cache_steps, plan.cache_size = kc.span(), steps, kc.size
+    return plan, q_out
 
 
 # -- attention over the cache ----------------------------------------------------------------

@@ -174,6 +174,52 @@ def test_append_kv_refuses_overlap_and_read_only():
         decode.append_kv(*args)
 
 
+@pytest.mark.parametrize("views,apart", [
+    (lambda x: (x[:, 0], x[:, 1]), True),                      # [pages, 2, page, heads, dim]
+    (lambda x: (x[:, 1], x[:, 0]), True),
+    (lambda x: (x[0::2, 0], x[1::2, 0]), True),
+    (lambda x: (x.view(10, 16, 2, 2, 64)[:, :, 0], x.view(10, 16, 2, 2, 64)[:, :, 1]), True),
+    (lambda x: (x.view(10, 16, 2, 128)[..., 64:], x.view(10, 16, 2, 128)[..., :64]), True),
+    (lambda x: (x.view(10, 16, 4, 64)[:, :, ::2], x.view(10, 16, 4, 64)[:, :, 1::2]), True),
+    (lambda x: (x[:, 0], x[:, 0]), False),
+    (lambda x: (x[:-1, 0], x[1:, 0]), False),
+    (lambda x: (x[:-1, 1], x[1:, 0]), True),
+    (lambda x: (x[:, 0, :, :1], x[:, 0, :, 1:]), True),
+    (lambda x: (x[:, 0, :-1], x[:, 0, 1:]), False),
+    (lambda x: (x[:, 0, :8], x[:, 0, 8:]), True),
+    (lambda x: (x.view(10, 16, 2, 128)[..., :64], x.view(10, 16, 2, 128)[..., 63:127]), False),
+    (lambda x: (x.view(10, 16, 2, 128)[..., 8:72], x.view(10, 16, 2, 128)[..., :64]), False),
+])
+@pytest.mark.parametrize("kind", ["torch", "numpy"])
+def test_append_kv_refuses_caches_that_share_memory(views, apart, kind):
+    """Caches inside one array: taken where no element is both's. (A `q` without work: nothing is
+    launched.)"""
+    k, v = views(torch.zeros(10, 2, 16, 2, 64))
+    if kind == "numpy":
+        k, v = k.numpy(), v.numpy()
+    heads = k.shape[2]
+    new = torch.zeros(0, heads, 64)
+    args = (new, new, k, v, torch.zeros(0, 4, dtype=torch.int32), torch.zeros(0, dtype=torch.int32))
+    if apart:
+        assert decode.append_kv(*args) is None
+    else:
+        with pytest.raises(ValueError, match="overlaps `v_cache`|are the same"):
+            decode.append_kv(*args)
+
+
+def test_arrays_that_meet_by_their_strides():
+    """Against the sets of their elements' places."""
+    rng = np.random.default_rng(1)
+    for _ in range(300):
+        shape = tuple(int(n) for n in rng.integers(1, 5, 3))
+        strides = [int(s) for s in rng.integers(1, 30, 3)]
+        a = decode._Array("a", torch.zeros(300).as_strided(shape, strides))
+        places = {int(np.dot(i, strides)) for i in np.ndindex(*shape)}
+        for gap in range(-60, 61, 7):
+            want = any(p + gap in places for p in places)
+            assert decode._meet(decode._steps(a), 4, 4 * gap) == want, (shape, strides, gap)
+
+
 LOGITS = [
     (dict(logits=torch.zeros(3, 100, dtype=torch.int32)), TypeError, "`logits`"),
     (dict(logits=torch.zeros(300)), ValueError, "2 dimensions"),

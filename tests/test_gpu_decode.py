@@ -573,6 +573,32 @@ def test_loads_past_the_caches_give_the_same(dtype, cdtype, monkeypatch):
         assert torch.equal(x, y)
 
 
+def test_append_into_caches_of_one_array():
+    """Keys and values of a page side by side, call after call; shifted by a page, so that they
+    share memory, they are refused also where the plan is known."""
+    gen = torch.Generator().manual_seed(15)
+    d = append_case(gen, BF16, BF16, [20, 33], [1, 1], 16, 2, 4, 64, 64)
+    pages = d["k_cache"].shape[0]
+    both = torch.zeros(pages + 1, 2, 16, 2, 64, dtype=BF16)
+    d["k_cache"], d["v_cache"] = both[:-1, 0], both[:-1, 1]
+    want = [x.clone() for x in R.append_kv(*(d[n] for n in ("k", "v", "k_cache", "v_cache",
+                                                            "block_table", "seq_lens")),
+                                           q=d["q"], cos=d["cos"], sin=d["sin"])[1:3]]
+    g = {n: x.cuda() for n, x in d.items() if "cache" not in n}
+    room = both.cuda()
+    kw = dict(q=g["q"], cos=g["cos"], sin=g["sin"])
+    rest = g["block_table"], g["seq_lens"]
+    for _ in range(2):
+        room.zero_()
+        decode.append_kv(g["k"], g["v"], room[:-1, 0], room[:-1, 1], *rest, **kw)
+        for i, w in enumerate(want):
+            close(room[:-1, i], w, half_step(BF16) * w.abs() + 8 * U * 5)
+    before = room.clone()
+    with pytest.raises(ValueError, match="`k_cache` overlaps `v_cache`"):
+        decode.append_kv(g["k"], g["v"], room[:-1, 0], room[1:, 0], *rest, **kw)
+    assert torch.equal(room, before)
+
+
 def test_append_rounds_to_8_bits_as_the_type_says():
     """Every neighbourhood of an e4m3 value: its rounding, ties, zeros, overflow, NaN."""
     grid = torch.arange(256, dtype=torch.uint8).view(F8).float()
