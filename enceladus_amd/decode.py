@@ -505,8 +505,11 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
     given = q_out is not None
     if plan is not None:
         gap = v_cache.data_ptr() - k_cache.data_ptr()
-        if abs(gap) < plan.cache_span and _meet(plan.cache_steps, plan.cache_size, gap):
-            plan = None                # refused below
+        if abs(gap) < plan.cache_span:
+            if plan.cache_steps is None:
+                plan.cache_steps = _steps(_Array("k_cache", k_cache))
+            if _meet(plan.cache_steps, k_cache.element_size(), gap):
+                plan = None            # refused below
     if plan is None:
         plan, q_out = _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q,
                                    q_out, cos, sin, interleaved, k_scale, v_scale)
@@ -553,9 +556,10 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         _need(q_out is None, "`q_out` is given without `q`")
     _written("k_cache", kc)
     _written("v_cache", vc)
-    gap, steps = vc.address() - kc.address(), _steps(kc)
+    gap, steps = vc.address() - kc.address(), None
     if abs(gap) < kc.span():
         _need(gap != 0, "`k_cache` and `v_cache` are the same")
+        steps = _steps(kc)
         _need(not _meet(steps, kc.size, gap), "`k_cache` overlaps `v_cache`")
     _need((cos is None) == (sin is None), "`cos` and `sin` go together")
     ca = sa = None
@@ -597,7 +601,7 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
                  [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
                  tail, [(3, 0, True), (3, 1, False), (3, 2, False), (3, 4, False),
                         (3, 5, False)])
-    plan.cache_span, plan.cache_steps, plan.cache_size = kc.span(), steps, kc.size
+    plan.cache_span, plan.cache_steps = kc.span(), steps
     return plan, q_out
 
 
