@@ -20,9 +20,9 @@
 //   of them, so that the VE products cover 16 VE elements of the head without any transpose
 //   through the LDS (a register permute pairs the keys).
 // - The weights are split into terms of the values' 16-bit type, a product each (the matrix units
-//   idle anyway), so that they are rounded about as 32-bit ones are (2^-24): three bf16 terms leave
-//   2^-24 of a weight, two fp16 terms 2^-22. e4m3 values are exact in fp16, whose two terms take
-//   bf16 queries' weights as well.
+//   idle anyway), so that little is lost of their 32 bits: three bf16 terms hold a weight exactly,
+//   two fp16 terms are off by 2^-22 of it at most. e4m3 values are exact in fp16, whose two terms
+//   take bf16 queries' weights as well.
 //
 // Work: a chunk of one sequence is an item; one wave takes an item of one key head, by itself.
 // The chunks' length comes from all sequences' lengths, on the device, so that ragged batches
@@ -263,11 +263,23 @@ template <bool FP16> EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32*
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ek::pack<ek::bf16x8>(a),
                                                   ek::pack<ek::bf16x8>(b), acc, 0, 0, 0);
 }
-template <bool FP16> struct half_of { typedef __bf16 type; };
-template <> struct half_of<true> { typedef _Float16 type; };
-typedef half_of<HALF>::type half_t;                 // of the weights' terms
-EK_INLINE u32 pack2(half_t a, half_t b) {
+EK_INLINE u32 pack2(_Float16 a, _Float16 b) {
   return (u32)__builtin_bit_cast(uint16_t, a) | (u32)__builtin_bit_cast(uint16_t, b) << 16;
+}
+// The next term of two weights: x0 and x1 become what it leaves. bf16 cuts off, so that three terms
+// are the 24 bits of a weight exactly, and that no conversion is waited for.
+EK_INLINE u32 next_term(float& x0, float& x1) {
+  if constexpr (HALF) {
+    const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
+    x0 -= (float)h0;
+    x1 -= (float)h1;
+    return pack2(h0, h1);
+  } else {
+    const u32 u0 = ek::f32_bits(x0), u1 = ek::f32_bits(x1);
+    x0 -= ek::bits_f32(u0 & 0xFFFF0000u);
+    x1 -= ek::bits_f32(u1 & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+  }
 }
 #endif
 
@@ -560,18 +572,14 @@ ek_paged_attention(Params a) {
 #else
     constexpr int SS = ST == 1 ? 1 : 2;            // score tiles of a product
     u32 w_p[TERMS][ST / SS][2 * SS];
-    // the weights' terms from word `at` on: each is what the ones before it leave, rounded
+    // the weights' terms from word `at` on: each is what the ones before it leave
     const auto split = [&](const ek::f32x4& x, int at) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float x0 = x[2 * i] * LIFT, x1 = x[2 * i + 1] * LIFT;
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          const half_t h0 = (half_t)x0, h1 = (half_t)x1;
-          w_p[k][at / (2 * SS)][at % (2 * SS) + i] = pack2(h0, h1);
-          x0 -= (float)h0;
-          x1 -= (float)h1;
-        }
+        for (int k = 0; k < TERMS; ++k)
+          w_p[k][at / (2 * SS)][at % (2 * SS) + i] = next_term(x0, x1);
       }
     };
     if constexpr (PACKS) {
