@@ -29,9 +29,9 @@
 // give items of about one size. Sequences of one chunk are finished here; the others leave
 // (O, m, l) per chunk to the second kernel.
 //
-// Measured, both kernels: 64 ragged sequences, 8 key heads of 128, 32 query heads, bf16, 501 MB: 88
-// us, 5.7 TB/s; one sequence of 131075, fp16, 537 MB: 93 us, 5.8 (a kernel that only reads: 6.0
-// to 6.2). One sequence of 1999: 6.7 + 3.4 us, a chain of lengths, table, keys, then the join's.
+// Measured, both kernels: 64 ragged sequences, 8 key heads of 128, 32 query heads, bf16, 501 MB: 89
+// us, 5.6 TB/s; one sequence of 131075, fp16, 537 MB: 94 us, 5.7 (a kernel that only reads: 6.0
+// to 6.2). One sequence of 1999: 6.9 + 3.6 us, a chain of lengths, table, keys, then the join's.
 // Joining in the first kernel, by the last wave of a sequence to arrive, took longer (18 instead
 // of 12 us there: its counters are as far away as memory), and so did workgroups of 4 waves that
 // merge in the LDS (they start and end together).
@@ -585,8 +585,7 @@ ek_paged_attention(Params a) {
     if constexpr (PACKS) {
       // A key head of at most 8 query heads leaves lanes 8 to 15 of a row without one: they take
       // the scores of every second tile, and give the weights back (24 sequences, 153 MB of
-      // e4m3, 64 heads over 8 key heads: with a softcap 39.9 us instead of 41.4, without one
-      // the same).
+      // e4m3, 64 heads over 8 key heads: with a softcap 40.4 us instead of 42.1).
       if (nh <= 8) {
         ek::f32x4 x[PACKS ? ST / 2 : 1];
 #pragma unroll

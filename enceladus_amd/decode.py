@@ -622,7 +622,7 @@ def _step(width: int, size: int, short: bool) -> int:
     """Keys per wave and step: 8 KB of keys and values, where there are 16 to 32 keys in that; of
     an e4m3 cache twice as many, whose conversions and scores cost more per byte than their loads.
     Measured at their best numbers of waves: 64 ragged sequences, 501 MB of bf16, heads of 128:
-    16 keys 87.7 us, 32 89.8 (and 187 registers instead of 123), 64 118; 24 ragged sequences, 153 MB
+    16 keys 87.7 us, 32 89.8 (and 187 registers instead of 128), 64 118; 24 ragged sequences, 153 MB
     of e4m3: 16 keys 50.7 us, 32 46.4, 64 43.4. `short`: no wave will have many, so that fewer waits
     count for more: one sequence of 1999 tokens, bf16 10.7 us with 16 keys, 9.9 with 32, 11.1 with 64;
     46 sequences of at most 317 12.4, 11.4 and 14.1."""
@@ -643,13 +643,14 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: float 
     which only the last `window` count when that is above 0, made `softcap` * tanh(s_j /
     `softcap`) when that is above 0; the result is the sum of softmax(s)_j v_j. `heads` is a
     multiple of the key heads: head h reads key head h // (heads / key heads). A sequence
-    without tokens gives zeros. Tokens on a page outside the cache count as absent. Cache
+    without tokens, or with no score above -inf, gives zeros. Tokens on a page outside the cache count as absent. Cache
     memory that no sequence's length reaches may hold anything, NaN included. A value among a
     sequence's own that is not finite makes its element of the result infinite or NaN.
 
     Args:
         q: `[batch, heads, dim]`, float32, float16 or bfloat16; `dim` a multiple of 8 up to
-            256 (of 16 with a float8 cache).
+            256 (of 16 with a float8 cache); at most 65536 sequences (every wave looks for its
+            own among them, which is most of the time from some thousand short ones on).
         k_cache, v_cache: `[pages, page size, key heads, dim]` of the type of `q`, or
             float8_e4m3fn (not with float32).
         block_table: int32 `[batch, pages of a sequence]`.
