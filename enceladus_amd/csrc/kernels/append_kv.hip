@@ -11,7 +11,8 @@
 // a lane keeps one place in the head, so its cos and sin are read once for all rows, and pairs
 // meet in one lane, so that queries can be rotated in place.
 // Measured: 21152 tokens of 32 query, 8 key and 8 value heads of 128 in bf16, 531 MB: 90 us, 5.9
-// TB/s (the framework's own copies: 6.4). One token of such heads: 3.2 us, a launch and a chain of loads.
+// TB/s (the framework's own copies: 6.4). One token of such heads: 3.2 us, a launch and a chain of
+// loads.
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
 // vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS,
