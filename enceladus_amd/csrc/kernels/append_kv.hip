@@ -16,8 +16,13 @@
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
 // vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS,
-// EK_STREAM (the rows are more than the caches keep: loaded and stored past them).
+// EK_STREAM (the rows are more than the caches keep: loaded and stored past them), EK_AXES (0: tokens
+// turn by their slots' positions; else by positions of their own, up to four of them, of which each
+// pair has one: 1 where the pairs of a vector have the same, 2 where they may differ).
 #include "enceladus_cdna4.h"
+#ifndef EK_AXES
+#define EK_AXES 0
+#endif
 
 #if EK_Q == 0
 typedef float T;
@@ -40,12 +45,20 @@ struct Params {
   const int32_t* cu;                 // [batch + 1], or null: one token of each sequence
   const float* cos;
   const float* sin;
+#if EK_AXES
+  const int32_t* turns;              // [axes][tokens]: the positions that tokens turn by
+#endif
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
   int64_t c_page, c_token, c_head;   // bytes
   int64_t table_row, lens_step, cu_step, cos_row, sin_row;
   int32_t tokens, batch, heads, kv_heads, dim, rotary, page, pages, capacity, positions;
   int32_t parts;                     // waves per token
   float k_scale, v_scale, k_inv, v_inv;   // and 1 / scale
+#if EK_AXES
+  int32_t axes;
+  int64_t turn_axis, turn_step;
+  uint64_t pair_axes[4];             // two bits a pair
+#endif
 };
 
 EK_INLINE float sat8(float x) { return x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x; }
@@ -136,7 +149,26 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
     back = end - t;
   }
   const int pos = (len > 0 ? len : 0) - back;      // a negative length is none: no wrapping round
+#if EK_AXES
+  if (pos < 0 || pos >= a.capacity) return;
+  // its places in cos and sin: all four on their way at once, those of no axis the first's
+  int turn_of[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    turn_of[x] = a.turns[(x < a.axes ? x : 0) * a.turn_axis + t * a.turn_step];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if ((uint32_t)turn_of[x] >= (uint32_t)a.positions) return;
+  // of pair j
+  const auto turn_at = [&](int j) {
+    const uint64_t w = j < 64 ? j < 32 ? a.pair_axes[0] : a.pair_axes[1]
+                              : j < 96 ? a.pair_axes[2] : a.pair_axes[3];
+    const int x = (int)(w >> 2 * (j & 31)) & 3;
+    return x < 2 ? x < 1 ? turn_of[0] : turn_of[1] : x < 3 ? turn_of[2] : turn_of[3];
+  };
+#else
   if (pos < 0 || pos >= a.capacity || (a.rotary && pos >= a.positions)) return;
+#endif
   const int pg = pos / a.page, page_id = a.table[b * a.table_row + pg];
 
   // places of a head: `pairs` of two vectors that are rotated together, then single vectors
@@ -154,8 +186,22 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
     float cs[V], sn[V];
     const bool turn = EK_PAIRS ? d < a.rotary : two;
     // where nothing turns, zeros, so that no branch has to wait for what it loaded
-    const float* cp = turn ? a.cos + pos * a.cos_row + (EK_PAIRS ? d / 2 : d) : s_zeros;
-    const float* sp = turn ? a.sin + pos * a.sin_row + (EK_PAIRS ? d / 2 : d) : s_zeros;
+    const int j0 = EK_PAIRS ? d / 2 : d;               // the vector's first pair
+#if EK_AXES == 2
+#pragma unroll
+    for (int i = 0; i < (EK_PAIRS ? V / 2 : V); ++i) {
+      const int at = turn_at(turn ? j0 + i : 0);
+      cs[i] = turn ? a.cos[at * a.cos_row + j0 + i] : 0.0f;
+      sn[i] = turn ? a.sin[at * a.sin_row + j0 + i] : 0.0f;
+    }
+#else
+#if EK_AXES
+    const int at = turn_at(turn ? j0 : 0);
+#else
+    const int at = pos;
+#endif
+    const float* cp = turn ? a.cos + at * a.cos_row + j0 : s_zeros;
+    const float* sp = turn ? a.sin + at * a.sin_row + j0 : s_zeros;
     if constexpr (EK_PAIRS) {
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) cs[i] = cp[i], sn[i] = sp[i];
@@ -163,6 +209,7 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
       load(cs, cp);
       load(sn, sp);
     }
+#endif
     for (int row = part * lanes + (places <= 64 ? sub : 0); row < rows;
          row += a.parts * lanes) {
       const bool is_q = row < a.heads, is_k = !is_q && row < a.heads + a.kv_heads;

@@ -71,7 +71,7 @@ def _function(file: str, macros: tuple, name: str, device: int):
     f = _functions.get((file, macros, name, device))
     if f is not None:
         return f
-    if file == "paged_attention.hip":
+    if file in ("paged_attention.hip", "tree_attention.hip"):
         check_mfma_layout()
     with _lock:
         mod = _modules.get((file, macros, device))
@@ -425,6 +425,8 @@ def _round32(x: float) -> float:
 # -- appending to the cache ----------------------------------------------------------------
 
 _APPEND = struct.Struct("<16q11i4f4x")
+_TURNS = struct.Struct("<i2q4Q")       # after its last number: see `_append_plan`
+MAX_AXES = 4
 
 
 # Bytes of rows, more than the L2s hold together, from which on they move past the caches: 21152
@@ -451,7 +453,7 @@ def _vector(size: int, rotary: int, dim: int, interleaved: bool) -> int:
 
 def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, q=None,
               q_out=None, cos=None, sin=None, interleaved: bool = False, k_scale: float = 1.0,
-              v_scale: float = 1.0):
+              v_scale: float = 1.0, positions=None, pair_axes=None):
     """Writes new keys and values into a paged cache, the keys rotated by their positions,
     and returns the queries rotated likewise.
 
@@ -466,7 +468,10 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
 
     With `cos` and `sin`, the first R elements of each key and query head are rotated in pairs,
     (j, j + R / 2), or (2 j, 2 j + 1) when `interleaved`: (x, y) becomes
-    (x cos - y sin, y cos + x sin).
+    (x cos - y sin, y cos + x sin). They are those of the row's position, or, with `positions`, of
+    positions of its own, wherever its slot is: one (the depth of a drafted token), or one on each
+    of several axes (the time, height and width of a part of a picture or a video), of which pair
+    j turns by the one on axis `pair_axes[j]`.
 
     Args:
         k, v: `[tokens, key heads, dim]`, float32, float16 or bfloat16; `dim` a multiple of 8
@@ -480,12 +485,19 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
         q_out: where the rotated queries go (`q` itself will do); new without it.
         cos, sin: float32 `[positions, R / 2]`.
         k_scale, v_scale: cached values are divided by these (float8: then saturated to +-448).
+        positions: int32 `[tokens]`, or `[axes, tokens]` with at most 4 axes: rows of `cos` and
+            `sin`. A row with a position that is not in them is skipped.
+        pair_axes: R / 2 numbers, each pair's axis; needed with more than one. Where the axes of
+            neighbouring pairs are equal in whole vectors (8 16-bit elements, 4 of 32), cos and
+            sin are read in vectors too.
 
     Returns:
         The rotated queries, or None without `q`.
     """
     # plain numbers from here on: a plan is kept by their values
     interleaved, k_scale, v_scale = bool(interleaved), float(k_scale), float(v_scale)
+    if pair_axes is not None:
+        pair_axes = tuple(map(operator.index, pair_axes))
     try:
         key = (0, k.dtype, k.shape, k.stride(), k.get_device(), v.dtype, v.shape, v.stride(),
                v.get_device(), k_cache.dtype, k_cache.shape, k_cache.stride(),
@@ -499,6 +511,8 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
                None if cos is None else (cos.dtype, cos.shape, cos.stride(), cos.get_device()),
                None if sin is None else (sin.dtype, sin.shape, sin.stride(), sin.get_device()),
                interleaved, k_scale, v_scale)
+        if positions is not None or pair_axes is not None:
+            key += None if positions is None else _of(positions), pair_axes
         plan = _plans.get(key)
     except (AttributeError, TypeError, RuntimeError):
         key = plan = None              # arrays of another kind, or no arrays
@@ -512,21 +526,47 @@ def append_kv(k, v, k_cache, v_cache, block_table, seq_lens, *, cu_tokens=None, 
                 plan = None            # refused below
     if plan is None:
         plan, q_out = _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q,
-                                   q_out, cos, sin, interleaved, k_scale, v_scale)
+                                   q_out, cos, sin, interleaved, k_scale, v_scale, positions,
+                                   pair_axes)
         if plan is None:
             return q_out
         _keep(key, plan)
     elif q is not None and not given:
         q_out = _like(q)
     arrays = [q, k, v, q_out, k_cache, v_cache, block_table, seq_lens, cu_tokens, cos, sin]
+    if positions is not None:
+        arrays.append(positions)
     if given:
         plan.check_apart(arrays)
     plan.run(arrays)
     return q_out
 
 
+def _turns(positions, pair_axes, tokens: int, pairs: int, vec: int):
+    """(positions' array, macro, the numbers that the kernel has of them) for `pairs` rotated
+    pairs, `vec` of them to a vector."""
+    _need(positions is not None, "`pair_axes` is given without `positions`")
+    _need(pairs > 0, "`positions` need `cos` and `sin`")
+    a = _Array("positions", positions)
+    one = len(a.shape) == 1
+    a = _array("positions", positions, ("i32",), 1, (tokens,), dense=False) if one else \
+        _array("positions", positions, ("i32",), 2, (None, tokens), dense=False)
+    axes = 1 if one else a.shape[0]
+    _need(0 < axes <= MAX_AXES, f"`positions` may have 1 to {MAX_AXES} axes, got {axes}")
+    _need(pair_axes is not None or axes == 1, f"`positions` of {axes} axes need `pair_axes`")
+    if pair_axes is None:
+        pair_axes = (0,) * pairs
+    _need(len(pair_axes) == pairs, f"`pair_axes` must have {pairs} entries, got {len(pair_axes)}")
+    _need(all(0 <= x < axes for x in pair_axes), f"`pair_axes` must be from 0 to {axes - 1}")
+    words = [sum(x << 2 * i for i, x in enumerate(pair_axes[w * 32:w * 32 + 32]))
+             for w in range(4)]
+    same = all(len(set(pair_axes[i:i + vec])) == 1 for i in range(0, pairs, vec))
+    step = a.strides[0] if one else a.strides[1]
+    return a, 1 if same else 2, (axes, 0 if one else a.strides[0], step, *words)
+
+
 def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_out, cos, sin,
-                 interleaved, k_scale, v_scale):
+                 interleaved, k_scale, v_scale, positions, pair_axes):
     """The checked call's plan (None: nothing to do) and its `q_out`."""
     ka = _array("k", k, ("fp32", "fp16", "bf16"), 3)
     tokens, kv_heads, dim = ka.shape
@@ -574,15 +614,22 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
     arrays = [("q", qa), ("k", ka), ("v", va), ("q_out", qo), ("k_cache", kc), ("v_cache", vc),
               ("block_table", bt), ("seq_lens", sl), ("cu_tokens", cu), ("cos", ca),
               ("sin", sa)]
+    interleaved = bool(interleaved) and rotary > 0
+    vec = _vector(ka.size, rotary, dim, interleaved)
+    turned = None
+    if positions is not None or pair_axes is not None:
+        turned = _turns(positions, pair_axes, tokens, rotary // 2,
+                        max(1, vec // 2) if interleaved else vec)
+        arrays.append(("positions", turned[0]))
     _device_of(arrays)
     if tokens == 0 or batch == 0 or kv_heads + heads == 0 or capacity == 0 or kc.shape[0] == 0:
         return None, q_out
-    interleaved = bool(interleaved) and rotary > 0
-    vec = _vector(ka.size, rotary, dim, interleaved)
     rows = heads + 2 * kv_heads
     macros = (("EK_Q", _Q[ka.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_V", vec),
               ("EK_PAIRS", int(interleaved)),
               ("EK_STREAM", int(tokens * rows * dim * ka.size > _STREAM_ROWS)))
+    if turned:
+        macros += (("EK_AXES", turned[1]),)
     # Waves per token: as many as it has rows for while CUs are without one, then enough for
     # _ROUNDS rows a lane (2^25 in all: a grid holds fewer than 2^32 threads).
     places = dim // vec if interleaved else (dim - rotary // 2) // vec
@@ -597,10 +644,12 @@ def _append_plan(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens, q, q_
         tokens, batch, heads, kv_heads, dim, rotary, kc.shape[1], kc.shape[0], capacity,
         ca.shape[0] if ca else 0, parts, k_scale, v_scale, 1.0 / _round32(k_scale),
         1.0 / _round32(v_scale))
+    if turned:
+        tail = tail[:-4] + _TURNS.pack(*turned[2])
     plan = _Plan("append_kv.hip", macros,
                  [("ek_append_kv", (-(-tokens * parts // 4), 1), 256)], arrays, {3, 4, 5}, 0,
                  tail, [(3, 0, True), (3, 1, False), (3, 2, False), (3, 4, False),
-                        (3, 5, False)])
+                        (3, 5, False)] + ([(3, 11, False)] if turned else []))
     plan.cache_span, plan.cache_steps = kc.span(), steps
     return plan, q_out
 
