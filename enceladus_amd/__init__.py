@@ -23,11 +23,11 @@ from enceladus_amd.runtime.tensor import (  # noqa: F401
 
 MetalError = HipError  # the reference's runtime error name, kept for drop-in code
 
-_LAZY = ("configs", "testing", "decode", "autotune", "Config", "heuristics")
+_LAZY = ("configs", "testing", "decode", "draft", "pages", "autotune", "Config", "heuristics")
 
 
 def __getattr__(name):
-    if name in ("configs", "testing", "decode"):
+    if name in ("configs", "testing", "decode", "draft", "pages"):
         import importlib
         return importlib.import_module(f"enceladus_amd.{name}")
     if name in ("autotune", "Config", "heuristics"):

@@ -5,7 +5,7 @@ GPU runs start without compile latency; it is also the compile-only coverage che
 list is every variant of the benchmark's workload table (`examples/workloads.py`, with
 torch "meta" tensors standing in for the full-size buffers: same shapes, dtypes and
 argument facts, no memory), the example wrappers' own default launches, and the hand-written
-kernels of `enceladus.decode`.
+kernels of `enceladus.decode`, `enceladus.draft` and `enceladus.pages`.
 """
 
 from __future__ import annotations
@@ -113,8 +113,8 @@ def compile_all(verbose: bool = False) -> int:
         kern, types, facts, consts, nw, dw = job
         return kern._compile_for(types, facts, consts, nw, dw).ck
 
-    from enceladus_amd import decode
-    hand = list(decode.specializations())
+    from enceladus_amd import decode, draft, pages
+    hand = [x for module in (decode, draft, pages) for x in module.specializations()]
 
     def one_hand(spec):
         decode._code(*spec)
