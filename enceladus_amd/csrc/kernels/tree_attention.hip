@@ -8,31 +8,34 @@
 // it sees, lse = log sum_j exp(s_j). Nothing seen: out = 0, lse = -inf.
 //
 // The (token, query head) pairs of a key head are the columns of every product: rows * heads per
-// key head of them share each key and value. A wave takes CT tiles of 16 columns through a chunk of
-// the keys, reads them straight into the registers that feed the matrix instructions and uses them
-// for all of its tiles, so that few columns take the cache's bytes over the HBM rate and many the
-// matrix products' time. The W waves of a workgroup take neighbouring columns of the same chunk: what
-// one reads the others find in the CU's cache.
+// key head of them share each key and value. Few columns take the cache's bytes over the HBM rate;
+// many take the products and, as long, the VALU's softmax. So each key and value is read once for
+// all columns of a workgroup: its waves copy KT keys at a time into the LDS, straight from memory and
+// a stage ahead, and WC of them take CT tiles of 16 columns each. Where that leaves waves without
+// columns, WK waves share the columns and split a stage's keys; they join in the LDS at the end.
 //
-// Layout (16x16 MFMA, lane l, r = l % 16, c = l / 16), as for one token per sequence:
+// Layout (16x16 MFMA, lane l, r = l % 16, c = l / 16):
 // - S^T = K Q^T: lane l reads a chunk of key r; its accumulator holds keys 4 c + i of column r.
 // - O^T = V^T P^T: the product over 32 keys gives lane l's slot j the key 4 c + j (j < 4) of the
-//   first and of the second 16 keys, so that P is where S left it. Lane l reads VE consecutive
-//   elements of those keys' values from element VE r on; the m-th product takes element VE r + m
-//   of them (a register permute pairs the keys).
+//   first and of the second 16 keys, so that P is where S left it. 16-bit values come transposed
+//   out of the LDS (tr_read4: 4 keys of one element); of others lane l reads VE consecutive elements
+//   of those keys from element VE r on, and the m-th product takes element VE r + m of them.
 // - A weight is two terms of the values' 16-bit type, a product each: 2^-17 of it is left out in
 //   bf16 and 2^-22 in fp16 and e4m3 (whose values are exact in fp16). One term would be half a
 //   step of the output's own type off in every weight, as much again as its rounding.
+// - In the LDS a row's 16-byte chunks are swapped by its key's number, so that no two lanes of a
+//   pass (256 bytes) meet in a bank: chunk x of key k is at x ^ k_swap(k) or x ^ v_swap(k). The
+//   copy does it for nothing: each lane picks the chunk that belongs at its place.
 //
-// Work: the (chunk, block of W CT 16 columns) pairs of all sequences are items, a workgroup each, of
+// Work: the (chunk, block of WC CT 16 columns) pairs of all sequences are items, a workgroup each, of
 // one key head. The chunks' length comes from all sequences' lengths and rows, on the device.
 // Sequences of one chunk are finished here; the others leave (O, m, l) per chunk and column to the
 // second kernel.
 //
 // Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_FP8 (the cache is e4m3), EK_DP (64, 128 or 256: the
-// head dimension it is compiled for), EK_PAD (the head dimension is smaller), EK_KT (keys per wave
-// and step: 16 or 32), EK_CT (column tiles of a wave), EK_W (waves of a workgroup), EK_OCC (waves
-// per SIMD that registers are left for).
+// head dimension it is compiled for), EK_KT (keys of a stage: 16, 32 or 64), EK_CT (column tiles of
+// a wave), EK_WC, EK_WK (waves over columns and over a stage's keys), EK_OCC (waves per SIMD that
+// registers are left for).
 #include "enceladus_cdna4.h"
 
 #if EK_Q == 0
@@ -42,20 +45,26 @@ typedef _Float16 T;
 #else
 typedef ek::bf16 T;
 #endif
-constexpr int DP = EK_DP, KT = EK_KT, CT = EK_CT, W = EK_W;
-constexpr int COLS = W * CT * 16;                   // columns of a workgroup
+constexpr int DP = EK_DP, KT = EK_KT, CT = EK_CT, WC = EK_WC, WK = EK_WK, W = WC * WK;
+constexpr int COLS = WC * CT * 16;                  // columns of a workgroup
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
 constexpr float LN2 = 0.69314718055994531f;
-constexpr int ST = KT / 16;                         // score tiles
-constexpr int KE = 16 / CS;                         // elements of a 16-byte key load
-constexpr int KL = DP / (4 * KE);                   // key loads per score tile and lane
-// Elements of a value load: 16 lanes cover at most the whole head.
-constexpr int VE0 = EK_Q == 0 ? 4 : 8;
-constexpr int VE = VE0 * 16 > DP ? DP / 16 : VE0;
-constexpr int PANELS = DP / (16 * VE);
-constexpr int VR = KT / 4;                          // value rows per lane
-constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value load
-constexpr int UNIT = 16;                            // keys: what chunks are multiples of
+constexpr int NK = KT / 16 / WK;                    // score tiles of a wave and stage
+constexpr int KE = 16 / CS;                         // elements of a chunk of 16 bytes
+constexpr int KL = DP / (4 * KE);                   // key chunks per score tile and lane
+constexpr bool TR = CS == 2;                        // values come transposed out of the LDS
+// Elements of a value read: 16 lanes cover at most the whole head.
+constexpr int VE0 = EK_FP8 ? 8 : 4;
+constexpr int VE = TR ? 1 : VE0 * 16 > DP ? DP / 16 : VE0;
+constexpr int NP = DP / 16;                         // output tiles, VE of them from one value read
+constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value read
+constexpr int CPR = DP * CS / 16;                   // chunks of a row in the LDS
+constexpr int ROW = CPR * 16, PART = KT * ROW, STAGE = 2 * PART;   // bytes: keys, then values
+constexpr int LOADS = KT * CPR / (64 * W);          // of a lane and stage, of keys and of values
+constexpr int UNIT = 64;                            // keys: what chunks are multiples of
+constexpr int PARTS = (WK - 1) * WC * CT * (NP * 1024 + 512);    // what waves leave each other
+constexpr int LDS = 2 * STAGE > PARTS ? 2 * STAGE : PARTS;
+static_assert(KT * CPR % (64 * W) == 0 && KT % (16 * WK) == 0, "a stage is shared evenly");
 // Weights are exp2(s - m), with the difference taken of the scores as the product gave them (or
 // capped) and scaled after that: the largest is 1 exactly, however large the scores are. fp16 terms
 // are lifted by 2^14: they keep a weight down to 2^-39 of the largest one.
@@ -68,6 +77,11 @@ template <int N> struct words { u32 w[N]; };
 template <int N> EK_INLINE words<N> load_words(const char* p) {
   words<N> r;
   ek::vload_u<uint8_t, N * 4>((uint8_t*)r.w, (const uint8_t*)p);
+  return r;
+}
+template <int N> EK_INLINE words<N> lds_words(const char* p) {
+  words<N> r;
+  ek::vload<uint8_t, N * 4>((uint8_t*)r.w, (const uint8_t*)p);
   return r;
 }
 
@@ -235,6 +249,15 @@ template <bool FP16> EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32*
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ek::pack<ek::bf16x8>(a),
                                                   ek::pack<ek::bf16x8>(b), acc, 0, 0, 0);
 }
+// acc += a b over 16 k values.
+template <bool FP16> EK_INLINE void mma16(ek::f32x4& acc, const u32* a, const u32* b) {
+  if constexpr (FP16)
+    acc = __builtin_amdgcn_mfma_f32_16x16x16f16(ek::pack<ek::f16x4>(a), ek::pack<ek::f16x4>(b),
+                                                acc, 0, 0, 0);
+  else
+    acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(ek::pack<ek::s16x4>(a),
+                                                    ek::pack<ek::s16x4>(b), acc, 0, 0, 0);
+}
 EK_INLINE u32 pack2(_Float16 a, _Float16 b) {
   return (u32)__builtin_bit_cast(uint16_t, a) | (u32)__builtin_bit_cast(uint16_t, b) << 16;
 }
@@ -267,23 +290,27 @@ EK_INLINE bool odd_word(u32 w) {
   return ((w & X) + ONE & 0x80008000u) != 0;
 #endif
 }
-// Element e of a load of values.
-EK_INLINE float element(const u32* w, int e) {
+// A word with 0 for each value that is not finite.
+EK_INLINE u32 finite_of(u32 w) {
+  constexpr int BITS = CS * 8;
+  u32 y = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += BITS) {
+    const u32 one = w & (BITS == 32 ? ~0u : (1u << (BITS & 31)) - 1 << i);
+    y |= odd_word(one) ? 0 : one;
+  }
+  return y;
+}
+// The value at p.
+EK_INLINE float element(const char* p) {
 #if EK_FP8
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  const f2 y = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w[e / 4], true)
-                       : __builtin_amdgcn_cvt_pk_f32_fp8((int)w[e / 4], false);
-  return e & 1 ? y[1] : y[0];
-#elif EK_Q == 0
-  return ek::bits_f32(w[e]);
+  return __builtin_amdgcn_cvt_f32_fp8((int)*(const uint8_t*)p, 0);
 #else
-  const uint16_t h = (uint16_t)(w[e / 2] >> (e & 1) * 16);
-  if constexpr (EK_Q == 1) return (float)__builtin_bit_cast(_Float16, h);
-  else return ek::bits_f32((u32)h << 16);
+  return ek::f32(*(const T*)p);
 #endif
 }
 
-// The query columns as the products' operand: element chunk (s, c) of column r, in the order in
+// The query columns as the products' operand: element chunk (i, c) of column r, in the order in
 // which a lane reads its keys.
 struct Query {
 #if EK_Q == 0
@@ -295,10 +322,19 @@ struct Query {
 
 __device__ const u32 s_zeros[4] = {0, 0, 0, 0};
 
-struct Tile {
-  words<4> k[ST][KL];
-  words<VW> v[VR][PANELS];
-};
+EK_INLINE int k_swap(int key) {
+  return CPR >= 16 ? key & 15 : CPR == 8 ? key >> 1 & 7 : key >> 2 & 3;
+}
+EK_INLINE int v_swap(int key) {
+  return !TR ? 0 : CPR >= 16 ? (key & 7) << 1 : (key >> 1 & 3) << 1;
+}
+
+// 16 bytes from `from` of each lane to LDS byte `lds` + 16 * lane. The compiler does not see the
+// copy: whoever reads waits for vmcnt and a barrier.
+EK_INLINE void copy16(u32 lds, const char* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               ::"s"(lds), "v"(from) : "memory", "m0");
+}
 
 // Word x of a row of the tree: what lies before the new tokens is seen, behind the mask nothing.
 EK_INLINE u32 tree_word(const Params& a, const u32* row, int x) {
@@ -328,32 +364,29 @@ EK_INLINE T result(float o, float f, bool any) { return ek::cvt<T>(any ? o * f :
 EK_INLINE float scale_of(const Params& a) { return a.cap > 0.0f ? 1.0f : a.scale; }
 
 extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(Params a) {
+  __shared__ __attribute__((aligned(1024))) char s_stage[LDS];
   const int lane = ek::lane_id(), r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wc = wave % WC, wk = wave / WC;
   const int g = blockIdx.y;
   Seq sq;
   const Item it = find_item(a, blockIdx.x, sq);
   if (it.b < 0) return;
   const int all = sq.rows * a.group;                          // columns of the sequence
-  const int col0 = it.block * COLS + wave * CT * 16;          // this wave's first
-  if (col0 >= all) return;
+  const int block0 = it.block * COLS, col0 = block0 + wc * CT * 16;   // this wave's first
 
-  // this lane's column of each tile: its token and head
-  int index[CT], head[CT];
-  bool valid[CT];
+  // this lane's column of each tile: its token, and its head of those of the key head
+  const auto valid = [&](int t) { return col0 + t * 16 + r < all; };
+  const auto column = [&](int t) { return valid(t) ? col0 + t * 16 + r : all - 1; };
+  int index[CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    const int col = col0 + t * 16 + r;
-    valid[t] = col < all;
-    const int x = valid[t] ? col : all - 1;
-    index[t] = (int)((u32)x / (u32)a.group);
-    head[t] = g * a.group + x - index[t] * a.group;
-  }
-  if (a.part && it.chunk == 0 && g == 0 && c == 0) {
+  for (int t = 0; t < CT; ++t) index[t] = (int)((u32)column(t) / (u32)a.group);
+  const auto head = [&](int t) { return column(t) - index[t] * a.group; };
+  if (a.part && it.chunk == 0 && g == 0 && wk == 0 && c == 0) {
     // for the second kernel, by the column of each token's first head
 #pragma unroll
     for (int t = 0; t < CT; ++t)
-      if (valid[t] && head[t] == 0)
+      if (valid(t) && head(t) == 0)
         part_rows(a)[sq.begin + index[t]] = {index[t], it.slot, it.chunks, it.blocks};
   }
 
@@ -364,7 +397,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   int lo = sq.first + lo_u * UNIT;
   int hi = hi_u >= units ? sq.end : sq.first + hi_u * UNIT;
   // where each column's keys begin, and (a tree) whether its window ends among the new tokens
-  int from[CT], from_most = 0;
+  int from[CT];
   bool deep = false;
   const u32* row[CT];
 #pragma unroll
@@ -376,20 +409,20 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       if (a.tree) seen = tree_count(a, row[t], sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
       from[t] = sq.past + seen - a.window;
       deep |= a.tree && seen > a.window;
-      from_most = from[t] > from_most ? from[t] : from_most;
     }
   }
-  if (a.window > 0) {
-    from_most = __builtin_amdgcn_readfirstlane(wave_all<ek::Max>(from_most));
-    deep = __builtin_amdgcn_ballot_w64(deep) != 0;
-  }
+  deep = __builtin_amdgcn_ballot_w64(deep) != 0;
+  // Whether a column may not see a key before `next` from `base` on that is there: new ones, and
+  // where windows begin (one for all waves: no column's begins behind this).
+  const int from_most = a.window > 0 ? sq.past + sq.rows - a.window : 0;
+  const auto edge = [&](int base) { return base + KT > sq.past || base < from_most; };
   if (!a.tree) {
-    // a chain's wave: no key behind its last token, none before the window of its first
-    const int last = col0 + CT * 16 < all ? col0 + CT * 16 : all;
+    // a block of a chain: no key behind its last token, none before the window of its first
+    const int last = block0 + COLS < all ? block0 + COLS : all;
     const int stop = sq.past + (last - 1) / a.group + 1;
     hi = hi < stop ? hi : stop;
     if (a.window > 0) {
-      const int begin = sq.past + col0 / a.group + 1 - a.window;
+      const int begin = sq.past + block0 / a.group + 1 - a.window;
       if (begin > lo) lo += (begin - lo) / UNIT * UNIT;
     }
   }
@@ -397,13 +430,48 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const char* kbase = a.k + g * a.c_head;
   const char* vbase = a.v + g * a.c_head;
   const int32_t* table = a.table + it.b * a.table_row;
+  const char* zeros = (const char*)s_zeros;
+  const u32 lds = ek::lds_addr(s_stage);
+  const int row_bytes = a.dim * CS;
 
-  // Loads first, without branches between them, then zeros for columns and elements that are not
-  // there: a wait per load would cost a latency each.
+  // The page of key base + lane of a stage, read one stage before its keys; -1: none.
+  const auto page_id = [&](int base) -> int {
+    const int key = base + (lane & (KT - 1));
+    return key < hi ? table[page_of(a, key)] : -1;
+  };
+  // This lane's key's offset in the cache (-1 where there is none), and which keys there are.
+  const auto offset = [&](int base, int id, uint64_t& live) -> int64_t {
+    const int key = base + (lane & (KT - 1));
+    const bool ok = (u32)id < (u32)a.pages;
+    live = __builtin_amdgcn_ballot_w64(ok);
+    return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : -1;
+  };
+  // A stage's keys and values on their way: zeros where there is no key, or no element of it.
+  const auto fetch = [&](int stage, int64_t off) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int first = (k * W + wave) * 64, key = (first + lane) / CPR;
+      const int chunk = (first + lane) % CPR;
+      const int64_t o = ek::shfl(off, key);
+      const int kc = (chunk ^ k_swap(key)) * 16, vc = (chunk ^ v_swap(key)) * 16;
+      const u32 to = lds + stage * STAGE + first * 16;
+      copy16(to, o >= 0 && kc < row_bytes ? kbase + o + kc : zeros);
+      copy16(to + PART, o >= 0 && vc < row_bytes ? vbase + o + vc : zeros);
+    }
+  };
+
+  uint64_t live = 0;
+  int id = -1;
+  if (lo < hi) {
+    const int64_t off = offset(lo, page_id(lo), live);
+    fetch(0, off);
+    id = page_id(lo + KT);
+  }
+
   Query q[CT];
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    const T* src = a.q + (sq.begin + index[t]) * a.q_row + head[t] * a.q_head;
+    const T* src = a.q + (sq.begin + index[t]) * a.q_row + (g * a.group + head(t)) * a.q_head;
     constexpr int QN = sizeof(q[0].w) / 16, QE = 16 / sizeof(T);
     const auto place = [&](int i) {
       return EK_Q == 0 ? (i * 4 + c) * 4 : (i / (KE / QE) * 4 + c) * KE + i % (KE / QE) * 8;
@@ -416,7 +484,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     for (int i = 0; i < QN; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const u32 w = valid[t] && place(i) < a.dim ? x[i].w[k] ^ a.q_sign : 0;
+        const u32 w = valid(t) && place(i) < a.dim ? x[i].w[k] ^ a.q_sign : 0;
         __builtin_memcpy(&q[t].w[i][k], &w, 4);
       }
   }
@@ -425,88 +493,67 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const float to_cap = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
   const float scale = scale_of(a);
   float m[CT], l[CT];
-  ek::f32x4 o[CT][PANELS][VE];
+  ek::f32x4 o[CT][NP];
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
     m[t] = -__builtin_inff(), l[t] = 0.0f;
 #pragma unroll
-    for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) o[t][p][e] = ek::f32x4{0, 0, 0, 0};
+    for (int p = 0; p < NP; ++p) o[t][p] = ek::f32x4{0, 0, 0, 0};
   }
-
-  // The page of key base + lane of a step, read one step before its keys; -1: none.
-  const auto page_id = [&](int base) -> int {
-    const int key = base + (lane & (KT - 1));
-    return key < hi ? table[page_of(a, key)] : -1;
-  };
-  // This lane's key's offset in the cache (0 where there is none), and which keys there are.
-  const auto offset = [&](int base, int id, uint64_t& live) -> int64_t {
-    const int key = base + (lane & (KT - 1));
-    const bool ok = (u32)id < (u32)a.pages;
-    live = __builtin_amdgcn_ballot_w64(ok);
-    return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : 0;
-  };
-  // lanes past the end of a head read zeros: loads without a branch
-  const char* zeros = (const char*)s_zeros;
-  const auto load_k = [&](Tile& t, int64_t off) {
-#pragma unroll
-    for (int s = 0; s < ST; ++s) {
-      const char* p = kbase + ek::shfl(off, s * 16 + r);
-#pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int d = (i * 4 + c) * KE;
-        t.k[s][i] = load_words<4>(!EK_PAD || d < a.dim ? p + d * CS : zeros);
-      }
-    }
-  };
-  const auto load_v = [&](Tile& t, int64_t off) {
-#pragma unroll
-    for (int j = 0; j < VR; ++j) {
-      const char* p = vbase + ek::shfl(off, (j / 4) * 16 + c * 4 + (j & 3));
-#pragma unroll
-      for (int i = 0; i < PANELS; ++i) {
-        const int d = i * 16 * VE + r * VE;
-        t.v[j][i] = load_words<VW>(!EK_PAD || d < a.dim ? p + d * CS : zeros);
-      }
-    }
+  // the element of the head that o[t][p][i] is
+  const auto element_of = [&](int p, int i) {
+    return p / VE * 16 * VE + (c * 4 + i) * VE + p % VE;
   };
 
-  Tile tile;
-  uint64_t live = 0;
-  int64_t off = 0;
-  int id = -1;
-  if (lo < hi) {
-    off = offset(lo, page_id(lo), live);
-    load_k(tile, off);
-    load_v(tile, off);
-    id = page_id(lo + KT);
-  }
-  for (int base = lo; base < hi; base += KT) {
+  // (all waves: the loads of this stage have arrived, and are seen by the others)
+  const auto arrive = [&] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  arrive();
+  int stage = 0;
+  bool some_odd = false;
+  for (int base = lo; base < hi; base += KT, stage ^= 1) {
     const int next = base + KT;
-    const int64_t here = off;
     uint64_t live_next = 0;
-    // scores of KT keys: acc[t][s][i] is key 16 s + 4 c + i of tile t's column r
-    ek::f32x4 acc[CT][ST];
+    if (next < hi) {
+      fetch(stage ^ 1, offset(next, id, live_next));
+      id = page_id(next + KT);
+    }
+    const char* keys = s_stage + stage * STAGE;
+    const char* values = keys + PART;
+    constexpr int K0 = 16;                            // keys of a tile
+    const int tile0 = wk * NK;                        // this wave's first
+
+    // scores: acc[t][s][i] is key 16 (tile0 + s) + 4 c + i of tile t's column r
+    ek::f32x4 acc[CT][NK];
+    words<4> kf[2][KL];                               // a tile's chunks, read a tile ahead
+    const auto read_keys = [&](int s) {
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+      for (int i = 0; i < KL; ++i)
+        kf[s & 1][i] = lds_words<4>(keys + ((tile0 + s) * K0 + r) * ROW +
+                                    ((i * 4 + c) ^ k_swap(r)) * 16);
+    };
+    read_keys(0);
 #pragma unroll
-      for (int s = 0; s < ST; ++s) acc[t][s] = ek::f32x4{0, 0, 0, 0};
+    for (int s = 0; s < NK; ++s) {
+      if (s + 1 < NK) read_keys(s + 1);
 #pragma unroll
-    for (int s = 0; s < ST; ++s)
+      for (int t = 0; t < CT; ++t) acc[t][s] = ek::f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
+        const words<4>& k = kf[s & 1][i];
 #if EK_Q == 0
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int t = 0; t < CT; ++t)
-            acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(tile.k[s][i].w[e]),
-                                                             q[t].w[i][e], acc[t][s], 0, 0, 0);
+            acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(ek::bits_f32(k.w[e]), q[t].w[i][e],
+                                                             acc[t][s], 0, 0, 0);
 #elif EK_FP8
         u32 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) widen4<EK_Q == 1>(tile.k[s][i].w[e], &x[2 * e], &x[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) widen4<EK_Q == 1>(k.w[e], &x[2 * e], &x[2 * e + 1]);
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
           mma<EK_Q == 1>(acc[t][s], x, q[t].w[2 * i]);
@@ -514,31 +561,28 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
         }
 #else
 #pragma unroll
-        for (int t = 0; t < CT; ++t) mma<EK_Q == 1>(acc[t][s], tile.k[s][i].w, q[t].w[i]);
+        for (int t = 0; t < CT; ++t) mma<EK_Q == 1>(acc[t][s], k.w, q[t].w[i]);
 #endif
       }
-    if (next < hi) {
-      off = offset(next, id, live_next);
-      id = page_id(next + KT);
-      load_k(tile, off);
+      __builtin_amdgcn_sched_barrier(0);              // no tile further ahead: registers
     }
+
     // softmax: scores and m stay as the product gave them (or capped, in log2 units) until exp2
     const bool full = live == ~0ull;
-    // whether a column may not see a key of this step that is there
-    const bool masks = next > sq.past || base < from_most;
+    const bool masks = edge(base);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       if (a.cap > 0.0f) {
 #pragma unroll
-        for (int s = 0; s < ST; ++s)
+        for (int s = 0; s < NK; ++s)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[t][s][i] = a.cap * tanh_f(acc[t][s][i] * to_cap);
       }
       if (!full || masks) {
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-          const int key = base + s * 16 + c * 4, j = key - sq.past;
-          u32 ok = (u32)(live >> (s * 16 + c * 4)) & 15u;
+        for (int s = 0; s < NK; ++s) {
+          const int at = (tile0 + s) * K0 + c * 4, key = base + at, j = key - sq.past;
+          u32 ok = (u32)(live >> at) & 15u;
           if (masks) {
             if (a.tree) {
               if (next > sq.past) {
@@ -567,7 +611,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       }
       float mt = -__builtin_inff();
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
+      for (int s = 0; s < NK; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mt = __builtin_fmaxf(mt, acc[t][s][i]);
       mt = ek::reduce_xor<ek::Max, 16>(mt);
@@ -576,94 +620,94 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
       const float alpha = ek::exp2_fast((m[t] - m_use) * scale);
       m[t] = m_new;
-      // most steps raise no column's maximum
+      // most stages raise no column's maximum
       if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
         l[t] *= alpha;
 #pragma unroll
-        for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) o[t][p][e] *= alpha;
+        for (int p = 0; p < NP; ++p) o[t][p] *= alpha;
       }
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
+      for (int s = 0; s < NK; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           acc[t][s][i] = ek::exp2_fast((acc[t][s][i] - m_use) * scale);
           l[t] += acc[t][s][i];
         }
     }
-    // values without a key are taken as zeros: their memory may hold anything
-    if (!full) {
-#pragma unroll
-      for (int j = 0; j < VR; ++j) {
-        const bool ok = live >> ((j / 4) * 16 + c * 4 + (j & 3)) & 1;
-#pragma unroll
-        for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-          for (int w = 0; w < VW; ++w) tile.v[j][p].w[w] = ok ? tile.v[j][p].w[w] : 0;
-      }
-    }
+
     // A value that is not finite must not reach the columns that don't see its key, whose weight
-    // is 0: its key is left out of the products and added by itself below.
-    uint64_t odd = 0;
+    // is 0: it becomes 0, and what sees it NaN behind the loop.
     if (masks) {
+      bool bad = false;
+      char* at = s_stage + stage * STAGE + PART + (lane & (KT - 1)) * ROW;
+#pragma unroll 4
+      for (int i = 0; i < CPR; ++i) {
+        const words<4> v = lds_words<4>(at + (i ^ k_swap(lane)) * 16);
 #pragma unroll
-      for (int j = 0; j < VR; ++j) {
-        bool bad = false;
-#pragma unroll
-        for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-          for (int w = 0; w < VW; ++w) bad |= odd_word(tile.v[j][p].w[w]);
-        const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
-        if (any == 0) continue;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (any >> (x * 16) & 0xFFFF) odd |= 1ull << ((j / 4) * 16 + x * 4 + (j & 3));
-        const bool out = any >> (c * 16) & 0xFFFF;
-#pragma unroll
-        for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-          for (int w = 0; w < VW; ++w) tile.v[j][p].w[w] = out ? 0 : tile.v[j][p].w[w];
+        for (int w = 0; w < 4; ++w) bad |= odd_word(v.w[w]);
+      }
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) {    // all waves see the same
+        some_odd = true;
+        __syncthreads();
+        if (bad && wave == 0)
+#pragma unroll 1
+          for (int i = 0; i < ROW / 4; ++i) {
+            u32* w = (u32*)(at + i * 4);
+            *w = finite_of(*w);
+          }
+        __syncthreads();
       }
     }
+
 #if EK_Q == 0
 #pragma unroll
-    for (int j = 0; j < VR; ++j)
+    for (int s = 0; s < NK; ++s)
 #pragma unroll
-      for (int p = 0; p < PANELS; ++p)
+      for (int j = 0; j < 4; ++j) {
+        const int key = (tile0 + s) * K0 + c * 4 + j;
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
+        for (int p = 0; p < NP; p += VE) {
+          const words<VW> v = lds_words<VW>(values + key * ROW + (p * 16 + r * VE) * CS);
 #pragma unroll
-          for (int t = 0; t < CT; ++t)
-            o[t][p][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                ek::bits_f32(tile.v[j][p].w[e]), acc[t][j / 4][j & 3], o[t][p][e], 0, 0, 0);
+          for (int e = 0; e < VE; ++e)
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+              o[t][p + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  ek::bits_f32(v.w[e]), acc[t][s][j], o[t][p + e], 0, 0, 0);
+        }
+      }
 #else
-    constexpr int SS = ST == 1 ? 1 : 2;            // score tiles of a product
-    u32 w_p[CT][TERMS][ST / SS][2 * SS];
+    constexpr int SS = NK == 1 ? 1 : 2;               // score tiles of a product
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+    for (int s = 0; s < NK; s += SS) {
+      u32 w_p[CT][TERMS][2 * SS];
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
+      for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          split(acc[t][s][2 * i] * LIFT, acc[t][s][2 * i + 1] * LIFT,
-                w_p[t][0][s / SS][s % SS * 2 + i], w_p[t][1][s / SS][s % SS * 2 + i]);
+        for (int i = 0; i < 2 * SS; ++i) {
+          const ek::f32x4& x = acc[t][s + i / 2];
+          split(x[i % 2 * 2] * LIFT, x[i % 2 * 2 + 1] * LIFT, w_p[t][0][i], w_p[t][1][i]);
+        }
+      const auto take = [&](int p, const u32* w) {
 #pragma unroll
-    for (int s = 0; s < ST; s += SS) {
+        for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int p = 0; p < PANELS; ++p) {
+          for (int k = 0; k < TERMS; ++k) {
+            if constexpr (SS == 1) mma16<HALF>(o[t][p], w, w_p[t][k]);
+            else mma<HALF>(o[t][p], w, w_p[t][k]);
+          }
+      };
+#if EK_FP8
+#pragma unroll
+      for (int p = 0; p < NP; p += VE) {
         // 4 SS keys' VE elements, 16 bits each
         u32 x[4 * SS][VE / 2];
 #pragma unroll
         for (int j = 0; j < 4 * SS; ++j) {
-          const words<VW>& v = tile.v[s * 4 + j][p];
-#if EK_FP8
+          const int key = (tile0 + s + j / 4) * K0 + c * 4 + (j & 3);
+          const words<VW> v = lds_words<VW>(values + key * ROW + p * 16 + r * VE);
 #pragma unroll
           for (int w = 0; w < VW; ++w) widen4<HALF>(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
-#else
-#pragma unroll
-          for (int w = 0; w < VW; ++w) x[j][w] = v.w[w];
-#endif
         }
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -672,101 +716,152 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
           for (int i = 0; i < 2 * SS; ++i)
             w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
                                          e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            if constexpr (SS == 2) {
-#pragma unroll
-              for (int k = 0; k < TERMS; ++k) mma<HALF>(o[t][p][e], w, w_p[t][k][s / SS]);
-            } else {
-              // 16 keys: a product over 32 for each term, which next to each other would lose
-              // digits in the product's own sum
-              const u32 twice[4] = {w[0], w[1], w[0], w[1]};
-#pragma unroll
-              for (int k = 0; k < TERMS; ++k) {
-                const u32 one[4] = {w_p[t][k][s][0], w_p[t][k][s][1], 0, 0};
-                mma<HALF>(o[t][p][e], twice, one);
-              }
-            }
-          }
+          take(p + e, w);
         }
       }
+#else
+      const int key = (tile0 + s) * K0 + c * 4 + (lane >> 2 & 3);
+      const char* at = values + key * ROW + (lane & 1) * 8;
+      const int chunk = lane >> 1 & 1, swap = v_swap(key);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        u32 w[2 * SS];
+#pragma unroll
+        for (int i = 0; i < SS; ++i) {               // v_swap goes by the key within 8
+          uint16_t x[4];
+          ek::tr_read4(x, (const uint16_t*)(at + i * K0 * ROW + ((2 * p + chunk) ^ swap) * 16));
+          __builtin_memcpy(&w[2 * i], x, 8);
+        }
+        take(p, w);
+      }
+#endif
     }
 #endif
-    // keys with values that are not finite: each lane's elements of the head, for its columns
+    live = live_next;
+    arrive();
+  }
+
+  // The same stages' keys once more, one at a time: the elements of their values that are not finite.
+  if (some_odd) {
 #pragma unroll 1
-    while (odd != 0) {
-      const int k = __builtin_ctzll(odd);
-      odd &= odd - 1;
-      const char* v = vbase + ek::shfl(here, k);
-      float weight[CT];
+    for (int key = lo; key < hi; ++key) {
+      const int base = lo + (key - lo) / KT * KT, tile = (key - base) / 16;
+      if (!edge(base) || tile / NK != wk) continue;
+      const int page = table[page_of(a, key)], j = key - sq.past;
+      if ((u32)page >= (u32)a.pages) continue;
+      const char* v = vbase + page * a.c_page + (key - page_of(a, key) * a.page) * a.c_token;
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        float x = 0.0f;
+        bool sees = key >= from[t] && j <= index[t];
+        if (a.tree)
+          sees = j < 0 ? key >= from[t]
+                       : (tree_bits(a, row[t], j) & 1) &&
+                             (!deep || tree_count(a, row[t], j, sq.end - sq.past) <= a.window);
+        if (!sees) continue;
 #pragma unroll
-        for (int s = 0; s < ST; ++s)
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x = k >> 4 == s && (k & 3) == i ? acc[t][s][i] : x;
-        weight[t] = ek::shfl(x, (k >> 2 & 3) * 16 + r) * LIFT;
+          for (int i = 0; i < 4; ++i) {
+            const int d = element_of(p, i);
+            if (d < a.dim && !(__builtin_fabsf(element(v + d * CS)) < __builtin_inff()))
+              o[t][p][i] = __builtin_nanf("");
+          }
       }
-#pragma unroll
-      for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = p * 16 * VE + (c * 4 + i) * VE;
-          const words<VW> y = load_words<VW>(!EK_PAD || d < a.dim ? v + d * CS : zeros);
-#pragma unroll
-          for (int e = 0; e < VE; ++e)
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-              if (weight[t] != 0.0f) o[t][p][e][i] += weight[t] * element(y.w, e);
-        }
     }
-    if (next < hi) load_v(tile, off);
-    live = live_next;
   }
 
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
     l[t] = ek::reduce_xor<ek::Sum, 16>(l[t]);
     l[t] = ek::reduce_xor<ek::Sum, 32>(l[t]);
-    if (!valid[t]) continue;
+  }
+  if constexpr (WK > 1) {
+    // the waves of the same columns: to the first of them, in the order in which it holds its own
+    float* part = (float*)s_stage;
+    constexpr int SIZE = CT * (NP * 256 + 128);
+    float* mine = part + ((wk - 1) * WC + wc) * SIZE;
+    if (wk > 0) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          *(ek::f32x4*)(mine + (t * NP + p) * 256 + lane * 4) = o[t][p];
+        mine[CT * NP * 256 + t * 128 + lane] = m[t];
+        mine[CT * NP * 256 + t * 128 + 64 + lane] = l[t];
+      }
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int k = 0; k < WK - 1; ++k) {
+      const float* other = part + (k * WC + wc) * SIZE;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        const float mo = other[CT * NP * 256 + t * 128 + lane];
+        const float lo = other[CT * NP * 256 + t * 128 + 64 + lane];
+        const float top = __builtin_fmaxf(m[t], mo), use = top == -__builtin_inff() ? 0.0f : top;
+        const float f = ek::exp2_fast((m[t] - use) * scale), fo = ek::exp2_fast((mo - use) * scale);
+        m[t] = top;
+        l[t] = l[t] * f + lo * fo;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const ek::f32x4 y = *(const ek::f32x4*)(other + (t * NP + p) * 256 + lane * 4);
+          o[t][p] = o[t][p] * f + y * fo;
+        }
+      }
+    }
+  }
+
+  // rows of VE or (transposed) 4 adjacent elements
+  constexpr int OUT = TR ? 4 : VE;
+  const auto each_run = [&](int t, const auto& put) {
+    if constexpr (TR) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const float y[4] = {o[t][p][0], o[t][p][1], o[t][p][2], o[t][p][3]};
+        put(p * 16 + c * 4, y);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < NP; p += VE)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float y[VE];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) y[e] = o[t][p + e][i];
+          put(p * 16 + (c * 4 + i) * VE, y);
+        }
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    if (!valid(t)) continue;
     const int64_t token = sq.begin + index[t];
+    const int h = g * a.group + head(t);
     if (it.chunks == 1) {
       const bool any = l[t] > 0.0f || l[t] != l[t];
       const float f = any ? a.v_scale / LIFT / l[t] : 0.0f;
-      T* dst = a.out + token * a.out_row + head[t] * a.out_head;
+      T* dst = a.out + token * a.out_row + h * a.out_head;
+      each_run(t, [&](int d, const float* x) {
+        T y[OUT];
 #pragma unroll
-      for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = p * 16 * VE + (c * 4 + i) * VE;
-          T y[VE];
-#pragma unroll
-          for (int e = 0; e < VE; ++e) y[e] = result(o[t][p][e][i], f, any);
-          if (!EK_PAD || d < a.dim) ek::vstore_u<T, VE>(dst + d, y);
-        }
+        for (int e = 0; e < OUT; ++e) y[e] = result(x[e], f, any);
+        if (d < a.dim) ek::vstore_u<T, OUT>(dst + d, y);
+      });
       if (a.lse && c == 0)
-        a.lse[token * a.heads + head[t]] =
+        a.lse[token * a.heads + h] =
             any ? (m[t] * scale + __builtin_log2f(l[t])) * LN2 : -__builtin_inff();
     } else {
       const int slot = it.slot + it.chunk * it.blocks + it.block;
       if (!a.part || slot < 0 || slot >= a.slots) continue;
-      const int64_t at = ((int64_t)slot * a.kv_heads + g) * COLS + wave * CT * 16 + t * 16 + r;
+      const int64_t at = ((int64_t)slot * a.kv_heads + g) * COLS + wc * CT * 16 + t * 16 + r;
       float* dst = a.part + at * a.dim;
+      each_run(t, [&](int d, const float* y) {
+        if (d < a.dim) {
 #pragma unroll
-      for (int p = 0; p < PANELS; ++p)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = p * 16 * VE + (c * 4 + i) * VE;
-          float y[VE];
-#pragma unroll
-          for (int e = 0; e < VE; ++e) y[e] = o[t][p][e][i];
-          if (!EK_PAD || d < a.dim) {
-#pragma unroll
-            for (int e = 0; e < VE; e += 4) ek::vstore_u<float, 4>(dst + d + e, y + e);
-          }
+          for (int e = 0; e < OUT; e += 4) ek::vstore_u<float, 4>(dst + d + e, y + e);
         }
+      });
       if (c == 0) {
         float* ml = part_ml(a) + at * 2;
         ml[0] = m[t];

@@ -51,9 +51,9 @@ def _tree(tree, tokens: int):
 # -- attention -------------------------------------------------------------------------------
 
 _ATTEND = struct.Struct("<11q11iI4iI3f")
-_UNIT = 16                          # tokens: what a sequence is split in multiples of
-_MIN_UNITS = 4                      # of a chunk
-_WAVES = 8                          # chunks of all sequences, key heads and columns, per CU
+_UNIT = 64                          # tokens: what a sequence is split in multiples of
+_MIN_UNITS = 1                      # of a chunk
+_GROUPS = 2                         # workgroups per CU
 
 
 def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tree=None,
@@ -123,11 +123,15 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
     return (out, lse) if return_lse else out
 
 
-def _shape(columns: float, width: int, size: int) -> tuple[int, int, int]:
-    """(column tiles of a wave, waves of a workgroup, keys of a step) for sequences of so many
-    columns of a key head."""
-    waves = 1 if columns <= 16 else 2 if columns <= 32 else 4
-    return 1, waves, 16
+def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int]:
+    """(keys of a stage, column tiles of a wave, waves over columns, waves over keys) for sequences
+    of so many columns of a key head, in heads of `width` cached elements of `size` bytes."""
+    keys = max(16, min(64, 16384 // (width * size)))
+    tiles = 2 if width <= 128 and size <= 2 and columns > 16 else 1
+    over = 1
+    while over < 4 and (columns > 16 * tiles * over or keys < 64 // over):
+        over *= 2
+    return keys, tiles, over, 4 // over
 
 
 def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree, scale, window,
@@ -173,21 +177,22 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
         capacity = 0
     window = min(window, _d.MAX_TOKENS)
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
-    tiles, waves, step = _shape(tokens / batch * group, width, kc.size)
-    cols = 16 * tiles * waves
+    keys, tiles, over, split = _shape(tokens / batch * group, width, kc.size)
+    cols = 16 * tiles * over
+    waves = over * split
     # blocks of columns: each sequence may have one that is not whole
     blocks = -(-tokens * group // cols) if batch == 1 else tokens * group // cols + \
         min(batch, tokens)
     most = -(-capacity // _UNIT)
     need(blocks * max(most, 1) < 1 << 31, f"{tokens} tokens over tables of {capacity} tokens are "
                                           "too many for one call")
-    items = max(1, _WAVES * C.coarsen_cap() // (kv_heads * waves))
+    items = max(1, _GROUPS * C.coarsen_cap() // kv_heads)
     x = items + blocks
     need(x * 64 * waves < 1 << 32 and kv_heads <= 65535, f"{tokens} tokens are too many for one "
                                                          "call")
     macros = (("EK_Q", _d._Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
-              ("EK_PAD", int(dim != width)), ("EK_KT", step), ("EK_CT", tiles), ("EK_W", waves),
-              ("EK_OCC", 1 if width == 256 or kc.size == 4 else 2))
+              ("EK_KT", keys), ("EK_CT", tiles), ("EK_WC", over), ("EK_WK", split),
+              ("EK_OCC", 1 if width * kc.size == 1024 else 2))
     launches = [("ek_tree_attention", (x, kv_heads), 64 * waves)]
     slots = workspace = 0
     # one sequence of as many blocks as there are items has one chunk
