@@ -33,7 +33,8 @@
 // second kernel.
 //
 // Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_FP8 (the cache is e4m3), EK_DP (64, 128 or 256: the
-// head dimension it is compiled for), EK_KT (keys of a stage: 16, 32 or 64), EK_CT (column tiles of
+// head dimension it is compiled for), EK_PAD (the head dimension is smaller), EK_KT (keys of a
+// stage: 16, 32 or 64), EK_TILE (16 or 32: columns of a tile), EK_CT (tiles of
 // a wave), EK_WC, EK_WK (waves over columns and over a stage's keys), EK_OCC (waves per SIMD that
 // registers are left for).
 #include "enceladus_cdna4.h"
@@ -45,34 +46,42 @@ typedef _Float16 T;
 #else
 typedef ek::bf16 T;
 #endif
-constexpr int DP = EK_DP, KT = EK_KT, CT = EK_CT, WC = EK_WC, WK = EK_WK, W = WC * WK;
-constexpr int COLS = WC * CT * 16;                  // columns of a workgroup
+constexpr int DP = EK_DP, KT = EK_KT, TILE = EK_TILE, CT = EK_CT, WC = EK_WC, WK = EK_WK;
+constexpr int W = WC * WK;
+constexpr int COLS = WC * CT * TILE;                // columns of a workgroup
+constexpr int NC = 64 / TILE;                       // lanes of a column
 constexpr int CS = EK_FP8 ? 1 : sizeof(T);          // bytes of a cache element
 constexpr float LN2 = 0.69314718055994531f;
-constexpr int NK = KT / 16 / WK;                    // score tiles of a wave and stage
+constexpr int NK = KT / TILE / WK;                  // score tiles of a wave and stage
+constexpr int RA = TILE * TILE / 256;               // runs of four keys of a lane in a tile
+constexpr int RUNS = NK * RA;
 constexpr int KE = 16 / CS;                         // elements of a chunk of 16 bytes
-constexpr int KL = DP / (4 * KE);                   // key chunks per score tile and lane
+constexpr int KL = DP / (NC * KE);                  // key chunks per score tile and lane
 constexpr bool TR = CS == 2;                        // values come transposed out of the LDS
-// Elements of a value read: 16 lanes cover at most the whole head.
+// Elements of a value read: the lanes of a tile's rows cover at most the whole head.
 constexpr int VE0 = EK_FP8 ? 8 : 4;
-constexpr int VE = TR ? 1 : VE0 * 16 > DP ? DP / 16 : VE0;
-constexpr int NP = DP / 16;                         // output tiles, VE of them from one value read
+constexpr int VE = TR ? 1 : VE0 * TILE > DP ? DP / TILE : VE0;
+constexpr int NP = DP / TILE;                       // output tiles, VE of them from one value read
 constexpr int VW = VE * CS / 4 < 1 ? 1 : VE * CS / 4;  // words of a value read
 constexpr int CPR = DP * CS / 16;                   // chunks of a row in the LDS
 constexpr int ROW = CPR * 16, PART = KT * ROW, STAGE = 2 * PART;   // bytes: keys, then values
 constexpr int LOADS = KT * CPR / (64 * W);          // of a lane and stage, of keys and of values
 constexpr int UNIT = 64;                            // keys: what chunks are multiples of
-constexpr int PARTS = (WK - 1) * WC * CT * (NP * 1024 + 512);    // what waves leave each other
+constexpr int PARTS = (WK - 1) * WC * CT * (NP * RA * 1024 + 512);   // what waves leave each other
 constexpr int LDS = 2 * STAGE > PARTS ? 2 * STAGE : PARTS;
-static_assert(KT * CPR % (64 * W) == 0 && KT % (16 * WK) == 0, "a stage is shared evenly");
+static_assert(KT * CPR % (64 * W) == 0 && KT % (TILE * WK) == 0, "a stage is shared evenly");
+static_assert(TR || VE * CS >= 4, "values are read in words");
 // Weights are exp2(s - m), with the difference taken of the scores as the product gave them (or
 // capped) and scaled after that: the largest is 1 exactly, however large the scores are. fp16 terms
 // are lifted by 2^14: they keep a weight down to 2^-39 of the largest one.
 constexpr bool HALF = EK_Q == 1 || EK_FP8;          // the weights' terms are fp16
 constexpr int TERMS = 2;
-constexpr float LIFT = HALF ? 0x1p14f : 1.0f;
+constexpr float LIFT = HALF ? 14.0f : 0.0f;        // log2, in the exponents: l is lifted too
+
+#define EK_HERE __attribute__((always_inline))      // of a lambda: what it captures stays in registers
 
 typedef uint32_t u32;
+typedef float Acc __attribute__((ext_vector_type(RA * 4)));    // of a tile
 template <int N> struct words { u32 w[N]; };
 template <int N> EK_INLINE words<N> load_words(const char* p) {
   words<N> r;
@@ -102,7 +111,7 @@ struct Params {
   int64_t table_row, lens_step, cu_step, tree_row;      // elements
   int32_t tokens, batch, heads, kv_heads, group, dim, page, pages, capacity, window, words;
   uint32_t page_mul;
-  int32_t page_shift, items, slots, min_units;
+  int32_t page_shift, items, slots, min_units, join;
   uint32_t q_sign;                   // the sign bits of the queries' words, if scale is negative
   float scale, cap, v_scale;         // scale > 0, with log2(e); cap in the same unit, or 0
 };
@@ -180,19 +189,34 @@ EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
   }
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
   int per = (int)((u32)(total + a.items - 1) / (u32)a.items);
+  per = per < a.min_units ? a.min_units : per;
+  // Each sequence may have a chunk more than its share for each of its blocks. If chunks of up to
+  // half as many units again fit all of them into `items`, that saves a last round of few waves.
+  if (a.batch <= 64) {
+    int try_per = per;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const int all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(
+          blocks_of(a, s0) * chunks_of(units_of(s0), try_per)));
+      if (all <= a.items) per = try_per;
+      if (all <= a.items || all > a.items + a.items / 2) break;
+      try_per += (try_per + 7) >> 3;
+    }
+  }
   // without room for parts each has one chunk, as when rows enough for all items are there
-  per = !a.part ? 1 << 30 : per < a.min_units ? a.min_units : per;
+  if (!a.part) per = 1 << 30;
   Item it = {-1, 0, 0, 0, 0, 0};
   int before = 0, slots = 0;
   for (int base = 0; base < a.batch; base += 64) {
-    const Seq s = base == 0 ? s0 : seq_of(a, base + lane);
+    Seq s = s0;
+    if (base > 0) s = seq_of(a, base + lane);
     const int blocks = blocks_of(a, s), chunks = chunks_of(units_of(s), per);
     const int mine = blocks * chunks, held = chunks > 1 ? mine : 0;
     const int end = before + ek::wave_prefix_sum(mine), slot = slots + ek::wave_prefix_sum(held);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item < end);
     if (hit != 0) {
       const int at = __builtin_ctzll(hit);
-      const auto get = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+      const auto get = [&](int x) EK_HERE { return __builtin_amdgcn_readlane(x, at); };
       it.blocks = get(blocks);
       it.chunks = get(chunks);
       const int local = item - (get(end) - get(mine));
@@ -211,19 +235,21 @@ EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
   return it;
 }
 
-EK_INLINE float tanh_f(float x) {
-  const float y = __builtin_fabsf(x);
-  // below 0.35 the odd series (Taylor, to x^11: off by less than 2e-8 of it), above it
-  // (1 - e) / (1 + e), e = exp(-2 y), whose difference keeps its digits there
+// tanh below 0.35: the odd series (Taylor, to x^11: off by less than 2e-8 of it).
+EK_INLINE float tanh_small(float y) {
   const float z = y * y;
   float s = __builtin_fmaf(z, -1382.0f / 155925.0f, 62.0f / 2835.0f);
   s = __builtin_fmaf(z, s, -17.0f / 315.0f);
   s = __builtin_fmaf(z, s, 2.0f / 15.0f);
   s = __builtin_fmaf(z, s, -1.0f / 3.0f);
-  s = __builtin_fmaf(z * s, y, y);
-  const float e = ek::exp2_fast(y * -2.8853900817779268f);
+  return __builtin_fmaf(z * s, y, y);
+}
+constexpr float SMALL = 0.35f;
+// Above it (1 - e) / (1 + e), e = exp(-2 y), whose difference keeps its digits there.
+EK_INLINE float tanh_f(float x) {
+  const float y = __builtin_fabsf(x), e = ek::exp2_fast(y * -2.8853900817779268f);
   const float r = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-  return __builtin_copysignf(y < 0.35f ? s : r, x);
+  return __builtin_copysignf(y < SMALL ? tanh_small(y) : r, x);
 }
 
 #if EK_FP8
@@ -240,17 +266,20 @@ template <bool FP16> EK_INLINE void widen4(u32 w, u32* lo, u32* hi) {
 #endif
 
 #if EK_Q != 0
-// acc += a b over 32 k values: four words of 16-bit pairs per lane and operand.
-template <bool FP16> EK_INLINE void mma(ek::f32x4& acc, const u32* a, const u32* b) {
+// acc += a b: four words of 16-bit pairs per lane and operand, 32 (16x16) or 16 (32x32) k values.
+#if EK_TILE == 32
+#define EK_MFMA(type) __builtin_amdgcn_mfma_f32_32x32x16_##type
+#else
+#define EK_MFMA(type) __builtin_amdgcn_mfma_f32_16x16x32_##type
+#endif
+template <bool FP16> EK_INLINE void mma(Acc& acc, const u32* a, const u32* b) {
   if constexpr (FP16)
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ek::pack<ek::f16x8>(a), ek::pack<ek::f16x8>(b),
-                                                 acc, 0, 0, 0);
-  else
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ek::pack<ek::bf16x8>(a),
-                                                  ek::pack<ek::bf16x8>(b), acc, 0, 0, 0);
+    acc = EK_MFMA(f16)(ek::pack<ek::f16x8>(a), ek::pack<ek::f16x8>(b), acc, 0, 0, 0);
+  else acc = EK_MFMA(bf16)(ek::pack<ek::bf16x8>(a), ek::pack<ek::bf16x8>(b), acc, 0, 0, 0);
 }
-// acc += a b over 16 k values.
-template <bool FP16> EK_INLINE void mma16(ek::f32x4& acc, const u32* a, const u32* b) {
+// The same over 16 k values of 16x16 tiles: two words.
+template <bool FP16, typename A> EK_INLINE void mma_short(A& acc, const u32* a, const u32* b) {
+  static_assert(sizeof(A) == 16);
   if constexpr (FP16)
     acc = __builtin_amdgcn_mfma_f32_16x16x16f16(ek::pack<ek::f16x4>(a), ek::pack<ek::f16x4>(b),
                                                 acc, 0, 0, 0);
@@ -258,22 +287,23 @@ template <bool FP16> EK_INLINE void mma16(ek::f32x4& acc, const u32* a, const u3
     acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(ek::pack<ek::s16x4>(a),
                                                     ek::pack<ek::s16x4>(b), acc, 0, 0, 0);
 }
-EK_INLINE u32 pack2(_Float16 a, _Float16 b) {
-  return (u32)__builtin_bit_cast(uint16_t, a) | (u32)__builtin_bit_cast(uint16_t, b) << 16;
-}
+typedef float f2 __attribute__((ext_vector_type(2)));
 // The two terms of two weights. bf16: the first is cut off, the second rounded.
 EK_INLINE void split(float x0, float x1, u32& first, u32& second) {
   if constexpr (HALF) {
-    const _Float16 h0 = (_Float16)x0, h1 = (_Float16)x1;
-    first = pack2(h0, h1);
-    second = pack2((_Float16)(x0 - (float)h0), (_Float16)(x1 - (float)h1));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 y = __builtin_convertvector((f2{x0, x1}), h2);
+    first = __builtin_bit_cast(u32, y);
+    second = __builtin_bit_cast(
+        u32, __builtin_convertvector((f2{__builtin_fmaf((float)y[0], -1.0f, x0),
+                                         __builtin_fmaf((float)y[1], -1.0f, x1)}), h2));
   } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     const u32 u0 = ek::f32_bits(x0), u1 = ek::f32_bits(x1);
     first = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 y = {(__bf16)(x0 - ek::bits_f32(u0 & 0xFFFF0000u)),
-                  (__bf16)(x1 - ek::bits_f32(u1 & 0xFFFF0000u))};
-    second = __builtin_bit_cast(u32, y);
+    second = __builtin_bit_cast(
+        u32, __builtin_convertvector((f2{x0 - ek::bits_f32(u0 & 0xFFFF0000u),
+                                         x1 - ek::bits_f32(u1 & 0xFFFF0000u)}), b2));
   }
 }
 #endif
@@ -296,7 +326,7 @@ EK_INLINE u32 finite_of(u32 w) {
   u32 y = 0;
 #pragma unroll
   for (int i = 0; i < 32; i += BITS) {
-    const u32 one = w & (BITS == 32 ? ~0u : (1u << (BITS & 31)) - 1 << i);
+    const u32 one = w & (BITS == 32 ? ~0u : ((1u << (BITS & 31)) - 1) << i);
     y |= odd_word(one) ? 0 : one;
   }
   return y;
@@ -326,22 +356,34 @@ EK_INLINE int k_swap(int key) {
   return CPR >= 16 ? key & 15 : CPR == 8 ? key >> 1 & 7 : key >> 2 & 3;
 }
 EK_INLINE int v_swap(int key) {
-  return !TR ? 0 : CPR >= 16 ? (key & 7) << 1 : (key >> 1 & 3) << 1;
+  if (!TR) return 0;
+  if (TILE == 32) return CPR >= 16 ? (key & 3) << 2 : (key >> 1 & 1) << 2;
+  return CPR >= 16 ? (key & 7) << 1 : (key >> 1 & 3) << 1;
 }
 
-// 16 bytes from `from` of each lane to LDS byte `lds` + 16 * lane. The compiler does not see the
-// copy: whoever reads waits for vmcnt and a barrier.
-EK_INLINE void copy16(u32 lds, const char* from) {
+// 16 (or 4) bytes from `from` of each lane to LDS byte `lds` + 16 (or 4) * lane. The compiler does
+// not see the copy: whoever reads waits for it.
+EK_INLINE void copy16(u32 lds, const void* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                ::"s"(lds), "v"(from) : "memory", "m0");
+}
+EK_INLINE void copy4(u32 lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               ::"s"(lds), "v"(from) : "memory", "m0");
+}
+// Until at most the last N copies are on their way (copies arrive in order).
+template <int N> EK_INLINE void wait_for() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // Word x of a row of the tree: what lies before the new tokens is seen, behind the mask nothing.
 EK_INLINE u32 tree_word(const Params& a, const u32* row, int x) {
   return x < 0 ? ~0u : x < a.words ? row[x] : 0u;
 }
-// Bits [j, j + 4) of a row.
-EK_INLINE u32 tree_bits(const Params& a, const u32* row, int j) {
+// Bits [j, j + 4) of a row, of which `first` holds the first 64.
+EK_INLINE u32 tree_bits(const Params& a, const u32* row, uint64_t first, int j) {
+  if (j < 0) return j <= -4 ? 15u : (u32)(first << -j | ((1u << -j) - 1)) & 15u;
+  if (a.words <= 2) return j < 64 ? (u32)(first >> j) & 15u : 0u;
   const int x = j >> 5;
   const uint64_t w = (uint64_t)tree_word(a, row, x + 1) << 32 | tree_word(a, row, x);
   return (u32)(w >> (j & 31)) & 15u;
@@ -365,7 +407,8 @@ EK_INLINE float scale_of(const Params& a) { return a.cap > 0.0f ? 1.0f : a.scale
 
 extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(Params a) {
   __shared__ __attribute__((aligned(1024))) char s_stage[LDS];
-  const int lane = ek::lane_id(), r = lane & 15, c = lane >> 4;
+  __shared__ int32_t s_ids[W][2][64];
+  const int lane = ek::lane_id(), r = lane % TILE, c = lane / TILE;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wc = wave % WC, wk = wave / WC;
   const int g = blockIdx.y;
@@ -373,20 +416,22 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const Item it = find_item(a, blockIdx.x, sq);
   if (it.b < 0) return;
   const int all = sq.rows * a.group;                          // columns of the sequence
-  const int block0 = it.block * COLS, col0 = block0 + wc * CT * 16;   // this wave's first
+  const int block0 = it.block * COLS, col0 = block0 + wc * CT * TILE;   // this wave's first
 
-  // this lane's column of each tile: its token, and its head of those of the key head
-  const auto valid = [&](int t) { return col0 + t * 16 + r < all; };
-  const auto column = [&](int t) { return valid(t) ? col0 + t * 16 + r : all - 1; };
-  int index[CT];
+  // this lane's column of each tile, its token and its head (those of no column take the last)
+  int index[CT], head[CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) index[t] = (int)((u32)column(t) / (u32)a.group);
-  const auto head = [&](int t) { return column(t) - index[t] * a.group; };
+  for (int t = 0; t < CT; ++t) {
+    const int col = col0 + t * TILE + r, x = col < all ? col : all - 1;
+    index[t] = (int)((u32)x / (u32)a.group);
+    head[t] = g * a.group + x - index[t] * a.group;
+  }
+#define valid(t) (col0 + (t) * TILE + r < all)
   if (a.part && it.chunk == 0 && g == 0 && wk == 0 && c == 0) {
     // for the second kernel, by the column of each token's first head
 #pragma unroll
     for (int t = 0; t < CT; ++t)
-      if (valid(t) && head(t) == 0)
+      if (valid(t) && head[t] == 0)
         part_rows(a)[sq.begin + index[t]] = {index[t], it.slot, it.chunks, it.blocks};
   }
 
@@ -399,14 +444,14 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   // where each column's keys begin, and (a tree) whether its window ends among the new tokens
   int from[CT];
   bool deep = false;
-  const u32* row[CT];
+  uint64_t bits[CT];                                  // a tree's row's first 64
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    row[t] = a.tree ? a.tree + (sq.begin + index[t]) * a.tree_row : nullptr;
+    bits[t] = a.tree ? (a.tree + (sq.begin + index[t]) * a.tree_row)[0] | (a.words > 1 ? (uint64_t)(a.tree + (sq.begin + index[t]) * a.tree_row)[1] << 32 : 0) : 0;
     from[t] = 0;
     if (a.window > 0) {
       int seen = index[t] + 1;
-      if (a.tree) seen = tree_count(a, row[t], sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
+      if (a.tree) seen = tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
       from[t] = sq.past + seen - a.window;
       deep |= a.tree && seen > a.window;
     }
@@ -415,7 +460,10 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   // Whether a column may not see a key before `next` from `base` on that is there: new ones, and
   // where windows begin (one for all waves: no column's begins behind this).
   const int from_most = a.window > 0 ? sq.past + sq.rows - a.window : 0;
-  const auto edge = [&](int base) { return base + KT > sq.past || base < from_most; };
+  const int past = sq.past;
+  const auto edge = [past, from_most](int base) EK_HERE {
+    return base + KT > past || base < from_most;
+  };
   if (!a.tree) {
     // a block of a chain: no key behind its last token, none before the window of its first
     const int last = block0 + COLS < all ? block0 + COLS : all;
@@ -434,47 +482,50 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const u32 lds = ek::lds_addr(s_stage);
   const int row_bytes = a.dim * CS;
 
-  // The page of key base + lane of a stage, read one stage before its keys; -1: none.
-  const auto page_id = [&](int base) -> int {
-    const int key = base + (lane & (KT - 1));
-    return key < hi ? table[page_of(a, key)] : -1;
+  // The page of key base + lane of a stage (`ids` of two stages in turn): copied into the LDS a stage
+  // before its keys are, by every wave for itself. There is one at every address read here.
+  const auto fetch_ids = [&](int ids, int base) EK_HERE {
+    const int key = base + (lane & (KT - 1)), last = hi - 1;
+    copy4(ek::lds_addr(s_ids[wave][ids]), table + page_of(a, key < last ? key : last));
   };
   // This lane's key's offset in the cache (-1 where there is none), and which keys there are.
-  const auto offset = [&](int base, int id, uint64_t& live) -> int64_t {
-    const int key = base + (lane & (KT - 1));
-    const bool ok = (u32)id < (u32)a.pages;
+  const auto offset = [&](int ids, int base, uint64_t& live) EK_HERE -> int64_t {
+    const int key = base + (lane & (KT - 1)), id = s_ids[wave][ids][lane];
+    const bool ok = key < hi && (u32)id < (u32)a.pages;
     live = __builtin_amdgcn_ballot_w64(ok);
     return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : -1;
   };
-  // A stage's keys and values on their way: zeros where there is no key, or no element of it.
-  const auto fetch = [&](int stage, int64_t off) {
+  // A stage's keys or values on their way: zeros where there is no key, or no element of it.
+  const auto fetch = [&](int to, const char* from, const auto& swap, int64_t off, bool full) EK_HERE {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int first = (k * W + wave) * 64, key = (first + lane) / CPR;
-      const int chunk = (first + lane) % CPR;
+      const int byte = (((first + lane) % CPR) ^ swap(key)) * 16;
       const int64_t o = ek::shfl(off, key);
-      const int kc = (chunk ^ k_swap(key)) * 16, vc = (chunk ^ v_swap(key)) * 16;
-      const u32 to = lds + stage * STAGE + first * 16;
-      copy16(to, o >= 0 && kc < row_bytes ? kbase + o + kc : zeros);
-      copy16(to + PART, o >= 0 && vc < row_bytes ? vbase + o + vc : zeros);
+      if (!EK_PAD && full) copy16(lds + to + first * 16, from + o + byte);
+      else copy16(lds + to + first * 16, o >= 0 && byte < row_bytes ? from + o + byte : zeros);
     }
   };
+  const auto swap_k = [](int key) EK_HERE { return k_swap(key); };
+  const auto swap_v = [](int key) EK_HERE { return v_swap(key); };
 
   uint64_t live = 0;
-  int id = -1;
   if (lo < hi) {
-    const int64_t off = offset(lo, page_id(lo), live);
-    fetch(0, off);
-    id = page_id(lo + KT);
+    fetch_ids(0, lo);
+    fetch_ids(1, lo + KT);
+    wait_for<0>();
+    const int64_t off = offset(0, lo, live);
+    fetch(0, kbase, swap_k, off, live == ~0ull);
+    fetch(PART, vbase, swap_v, off, live == ~0ull);
   }
 
   Query q[CT];
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    const T* src = a.q + (sq.begin + index[t]) * a.q_row + (g * a.group + head(t)) * a.q_head;
+    const T* src = a.q + (sq.begin + index[t]) * a.q_row + head[t] * a.q_head;
     constexpr int QN = sizeof(q[0].w) / 16, QE = 16 / sizeof(T);
-    const auto place = [&](int i) {
-      return EK_Q == 0 ? (i * 4 + c) * 4 : (i / (KE / QE) * 4 + c) * KE + i % (KE / QE) * 8;
+    const auto place = [&](int i) EK_HERE {
+      return EK_Q == 0 ? (i * NC + c) * 4 : (i / (KE / QE) * NC + c) * KE + i % (KE / QE) * 8;
     };
     words<4> x[QN];
 #pragma unroll
@@ -493,56 +544,65 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const float to_cap = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
   const float scale = scale_of(a);
   float m[CT], l[CT];
-  ek::f32x4 o[CT][NP];
+  Acc o[CT][NP];
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
     m[t] = -__builtin_inff(), l[t] = 0.0f;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) o[t][p] = ek::f32x4{0, 0, 0, 0};
+    for (int p = 0; p < NP; ++p) o[t][p] = Acc{} * 0.0f;
   }
   // the element of the head that o[t][p][i] is
-  const auto element_of = [&](int p, int i) {
-    return p / VE * 16 * VE + (c * 4 + i) * VE + p % VE;
+  const auto element_of = [&](int p, int i) EK_HERE {
+    return p / VE * TILE * VE + (i / 4 * 8 + c * 4 + i % 4) * VE + p % VE;
   };
 
-  // (all waves: the loads of this stage have arrived, and are seen by the others)
-  const auto arrive = [&] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
-  arrive();
+  // A stage's copies are waited for where they are needed: its keys at the end of the stage before
+  // (its values, the last that were issued, may still be on their way), its values before their
+  // products. A barrier behind the wait: the other waves' copies too.
+  wait_for<0>();
+  __syncthreads();
   int stage = 0;
   bool some_odd = false;
   for (int base = lo; base < hi; base += KT, stage ^= 1) {
-    const int next = base + KT;
+    const int next = base + KT, to = (stage ^ 1) * STAGE;
     uint64_t live_next = 0;
-    if (next < hi) {
-      fetch(stage ^ 1, offset(next, id, live_next));
-      id = page_id(next + KT);
-    }
     const char* keys = s_stage + stage * STAGE;
     const char* values = keys + PART;
-    constexpr int K0 = 16;                            // keys of a tile
-    const int tile0 = wk * NK;                        // this wave's first
+    const int key0 = wk * NK * TILE;                  // this wave's first
+    // the first of the four keys of a lane's run s
+    const auto run_key = [&](int s) EK_HERE {
+      return key0 + s / RA * TILE + s % RA * 8 + c * 4;
+    };
 
-    // scores: acc[t][s][i] is key 16 (tile0 + s) + 4 c + i of tile t's column r
-    ek::f32x4 acc[CT][NK];
-    words<4> kf[2][KL];                               // a tile's chunks, read a tile ahead
-    const auto read_keys = [&](int s) {
+    // a tile's chunks, read AHEAD tiles before they are used
+    constexpr int AHEAD = NK > 2 ? 2 : 1;
+    words<4> kf[AHEAD + 1][KL];
+    const auto read_keys = [&](int s) EK_HERE {
 #pragma unroll
       for (int i = 0; i < KL; ++i)
-        kf[s & 1][i] = lds_words<4>(keys + ((tile0 + s) * K0 + r) * ROW +
-                                    ((i * 4 + c) ^ k_swap(r)) * 16);
+        kf[s % (AHEAD + 1)][i] = lds_words<4>(keys + (key0 + s * TILE + r) * ROW +
+                                              ((i * NC + c) ^ k_swap(r)) * 16);
     };
-    read_keys(0);
+#pragma unroll
+    for (int s = 0; s < AHEAD && s < NK; ++s) read_keys(s);
+    if (next < hi) {
+      const int64_t off = offset(stage ^ 1, next, live_next);
+      fetch(to, kbase, swap_k, off, live_next == ~0ull);
+      fetch_ids(stage, next + KT);
+      fetch(to + PART, vbase, swap_v, off, live_next == ~0ull);
+    }
+    // scores: run s's keys and tile t's column r are at score(t, s, 0) to (t, s, 3)
+    Acc acc[CT][NK];
+#define score(t, s, i) acc[t][(s) / RA][(s) % RA * 4 + (i)]
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-      if (s + 1 < NK) read_keys(s + 1);
+      if (s + AHEAD < NK) read_keys(s + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);              // the reads before what they hide behind
 #pragma unroll
-      for (int t = 0; t < CT; ++t) acc[t][s] = ek::f32x4{0, 0, 0, 0};
+      for (int t = 0; t < CT; ++t) acc[t][s] = Acc{} * 0.0f;
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
-        const words<4>& k = kf[s & 1][i];
+        const words<4>& k = kf[s % (AHEAD + 1)][i];
 #if EK_Q == 0
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -573,48 +633,61 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       if (a.cap > 0.0f) {
+        // most scores are small next to their cap: where all are, without the other form
+        float most = 0.0f;
 #pragma unroll
-        for (int s = 0; s < NK; ++s)
+        for (int s = 0; s < RUNS; ++s)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][s][i] = a.cap * tanh_f(acc[t][s][i] * to_cap);
-      }
-      if (!full || masks) {
-#pragma unroll
-        for (int s = 0; s < NK; ++s) {
-          const int at = (tile0 + s) * K0 + c * 4, key = base + at, j = key - sq.past;
-          u32 ok = (u32)(live >> at) & 15u;
-          if (masks) {
-            if (a.tree) {
-              if (next > sq.past) {
-                ok &= tree_bits(a, row[t], j);
-                if (deep) {
-#pragma unroll 1
-                  for (int i = 0; i < 4; ++i)
-                    if (j + i >= 0 &&
-                        tree_count(a, row[t], j + i, sq.end - sq.past) > a.window)
-                      ok &= ~(1u << i);
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (key + i < from[t] && key + i < sq.past) ok &= ~(1u << i);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (key + i < from[t] || j + i > index[t]) ok &= ~(1u << i);
-            }
+          for (int i = 0; i < 4; ++i) {
+            score(t, s, i) *= to_cap;
+            most = __builtin_fmaxf(most, __builtin_fabsf(score(t, s, i)));
           }
+        const bool small = __builtin_amdgcn_ballot_w64(most >= SMALL) == 0;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            acc[t][s][i] = ok >> i & 1 ? acc[t][s][i] : -__builtin_inff();
+            score(t, s, i) = a.cap * (small ? tanh_small(score(t, s, i)) : tanh_f(score(t, s, i)));
+      }
+      if (!full || masks) {
+        // four bits for each run
+        u32 ok = 0;
+#pragma unroll 1
+        for (int s = 0; s < RUNS; ++s) {
+          const int at = run_key(s), key = base + at, j = key - sq.past;
+          u32 run = (u32)(live >> at) & 15u;
+          if (masks) {
+            if (a.tree) {
+              run &= tree_bits(a, (a.tree + (sq.begin + index[t]) * a.tree_row), bits[t], j);
+              if (deep) {
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i)
+                  if (j + i >= 0 && tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), j + i, sq.end - sq.past) > a.window)
+                    run &= ~(1u << i);
+              }
+            } else {
+              const int n = index[t] - j + 1;            // of the run that the token sees
+              run &= n <= 0 ? 0u : n < 4 ? (1u << n) - 1 : 15u;
+            }
+            // before the window: all keys of a chain, those before the new ones of a tree
+            const int stop = a.tree && from[t] > sq.past ? sq.past : from[t];
+            const int n = stop - key;
+            run &= n <= 0 ? 15u : n < 4 ? 15u << n : 0u;
+          }
+          ok |= run << s * 4;
         }
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            score(t, s, i) = ok >> (s * 4 + i) & 1 ? score(t, s, i) : -__builtin_inff();
       }
       float mt = -__builtin_inff();
 #pragma unroll
-      for (int s = 0; s < NK; ++s)
+      for (int s = 0; s < RUNS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mt = __builtin_fmaxf(mt, acc[t][s][i]);
-      mt = ek::reduce_xor<ek::Max, 16>(mt);
+        for (int i = 0; i < 4; ++i) mt = __builtin_fmaxf(mt, score(t, s, i));
+      if constexpr (TILE == 16) mt = ek::reduce_xor<ek::Max, 16>(mt);
       mt = ek::reduce_xor<ek::Max, 32>(mt);
       const float m_new = __builtin_fmaxf(m[t], mt);
       const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
@@ -627,14 +700,17 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
         for (int p = 0; p < NP; ++p) o[t][p] *= alpha;
       }
 #pragma unroll
-      for (int s = 0; s < NK; ++s)
+      for (int s = 0; s < RUNS; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          acc[t][s][i] = ek::exp2_fast((acc[t][s][i] - m_use) * scale);
-          l[t] += acc[t][s][i];
+          score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i) - m_use, scale, LIFT));
+          l[t] += score(t, s, i);
         }
     }
 
+    if (next < hi) wait_for<2 * LOADS + 1>();
+    else wait_for<0>();
+    __syncthreads();
     // A value that is not finite must not reach the columns that don't see its key, whose weight
     // is 0: it becomes 0, and what sees it NaN behind the loop.
     if (masks) {
@@ -659,112 +735,139 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       }
     }
 
+    // O^T += V^T P^T in steps of some reads of values, each step's made a step ahead
 #if EK_Q == 0
+    constexpr int STEPS = RUNS * 4;                   // a key of each lane
+    words<VW> vf[2][NP / VE];
+    const auto read_values = [&](int k) EK_HERE {
+      const char* at = values + (run_key(k / 4) + k % 4) * ROW + r * VE * CS;
 #pragma unroll
-    for (int s = 0; s < NK; ++s)
+      for (int p = 0; p < NP; p += VE) vf[k & 1][p / VE] = lds_words<VW>(at + p * TILE * CS);
+    };
+    read_values(0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = (tile0 + s) * K0 + c * 4 + j;
+    for (int k = 0; k < STEPS; ++k) {
+      if (k + 1 < STEPS) read_values(k + 1);
+      __builtin_amdgcn_sched_barrier(0);              // the reads before what they hide behind
 #pragma unroll
-        for (int p = 0; p < NP; p += VE) {
-          const words<VW> v = lds_words<VW>(values + key * ROW + (p * 16 + r * VE) * CS);
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-          for (int e = 0; e < VE; ++e)
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-              o[t][p + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  ek::bits_f32(v.w[e]), acc[t][s][j], o[t][p + e], 0, 0, 0);
-        }
-      }
+        for (int t = 0; t < CT; ++t)
+          o[t][p] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              ek::bits_f32(vf[k & 1][p / VE].w[p % VE]), score(t, k / 4, k % 4), o[t][p], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #else
-    constexpr int SS = NK == 1 ? 1 : 2;               // score tiles of a product
+    constexpr int SS = RUNS == 1 ? 1 : 2;             // runs of a product
+    constexpr int GROUP = !TR ? VE : NP < 4 ? NP : 4; // output tiles of a step
+    constexpr int PER = NP / GROUP, STEPS = RUNS / SS * PER;
+    u32 w_p[CT][TERMS][2 * SS];
+    const auto products = [&](int p, const auto* w) EK_HERE {
 #pragma unroll
-    for (int s = 0; s < NK; s += SS) {
-      u32 w_p[CT][TERMS][2 * SS];
+      for (int k = 0; k < TERMS; ++k)
 #pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2 * SS; ++i) {
-          const ek::f32x4& x = acc[t][s + i / 2];
-          split(x[i % 2 * 2] * LIFT, x[i % 2 * 2 + 1] * LIFT, w_p[t][0][i], w_p[t][1][i]);
+        for (int t = 0; t < CT; ++t) {
+          if constexpr (SS * sizeof(*w) == 4) mma_short<HALF>(o[t][p], w, w_p[t][k]);
+          else mma<HALF>(o[t][p], w, w_p[t][k]);
         }
-      const auto take = [&](int p, const u32* w) {
+    };
+#if EK_FP8
+    words<VW> vf[2][4 * SS];
+    const auto read_values = [&](int k) EK_HERE {
+#pragma unroll
+      for (int j = 0; j < 4 * SS; ++j) {
+        const char* at = values + (run_key(k / PER * SS + j / 4) + (j & 3)) * ROW;
+        vf[k & 1][j] = lds_words<VW>(at + k % PER * GROUP * TILE + r * VE);
+      }
+    };
+#else
+    // four lanes of 16 read a key each (its 4 elements from 4 * lane on): tr_read4
+    u32 vf[2][GROUP][2 * SS];
+    const int quad = lane >> 2 & 3, swap = v_swap(c * 4 + quad);
+    const int half = (TILE == 32 ? lane >> 4 & 1 : 0) * 2 + (lane >> 1 & 1);     // chunk
+    const char* at = values + quad * ROW + (lane & 1) * 8;
+    const auto read_values = [&](int k) EK_HERE {
+#pragma unroll
+      for (int x = 0; x < GROUP; ++x)
+#pragma unroll
+        for (int i = 0; i < SS; ++i) {                 // v_swap goes by the key within 8
+          const int p = k % PER * GROUP + x;
+          uint16_t y[4];
+          ek::tr_read4(y, (const uint16_t*)(at + run_key(k / PER * SS + i) * ROW +
+                                            ((p * TILE / 8 + half) ^ swap) * 16));
+          __builtin_memcpy(&vf[k & 1][x][2 * i], y, 8);
+        }
+    };
+#endif
+    read_values(0);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      if (k + 1 < STEPS) read_values(k + 1);
+      __builtin_amdgcn_sched_barrier(0);              // the reads before what they hide behind
+      if (k % PER == 0) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k) {
-            if constexpr (SS == 1) mma16<HALF>(o[t][p], w, w_p[t][k]);
-            else mma<HALF>(o[t][p], w, w_p[t][k]);
+          for (int i = 0; i < 2 * SS; ++i) {
+            const int s = k / PER * SS + i / 2, x = i % 2 * 2;
+            split(score(t, s, x), score(t, s, x + 1), w_p[t][0][i], w_p[t][1][i]);
           }
-      };
-#if EK_FP8
-#pragma unroll
-      for (int p = 0; p < NP; p += VE) {
-        // 4 SS keys' VE elements, 16 bits each
-        u32 x[4 * SS][VE / 2];
-#pragma unroll
-        for (int j = 0; j < 4 * SS; ++j) {
-          const int key = (tile0 + s + j / 4) * K0 + c * 4 + (j & 3);
-          const words<VW> v = lds_words<VW>(values + key * ROW + p * 16 + r * VE);
-#pragma unroll
-          for (int w = 0; w < VW; ++w) widen4<HALF>(v.w[w], &x[j][2 * w], &x[j][2 * w + 1]);
-        }
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          u32 w[2 * SS];
-#pragma unroll
-          for (int i = 0; i < 2 * SS; ++i)
-            w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
-                                         e & 1 ? 0x07060302u : 0x05040100u);
-          take(p + e, w);
-        }
       }
-#else
-      const int key = (tile0 + s) * K0 + c * 4 + (lane >> 2 & 3);
-      const char* at = values + key * ROW + (lane & 1) * 8;
-      const int chunk = lane >> 1 & 1, swap = v_swap(key);
+      const int p0 = k % PER * GROUP;
+#if EK_FP8
+      // 4 SS keys' VE elements, 16 bits each
+      u32 x[4 * SS][VE / 2];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
+      for (int j = 0; j < 4 * SS; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+          widen4<HALF>(vf[k & 1][j].w[w], &x[j][2 * w], &x[j][2 * w + 1]);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
         u32 w[2 * SS];
 #pragma unroll
-        for (int i = 0; i < SS; ++i) {               // v_swap goes by the key within 8
-          uint16_t x[4];
-          ek::tr_read4(x, (const uint16_t*)(at + i * K0 * ROW + ((2 * p + chunk) ^ swap) * 16));
-          __builtin_memcpy(&w[2 * i], x, 8);
-        }
-        take(p, w);
+        for (int i = 0; i < 2 * SS; ++i)
+          w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
+                                       e & 1 ? 0x07060302u : 0x05040100u);
+        products(p0 + e, w);
       }
+#else
+#pragma unroll
+      for (int x = 0; x < GROUP; ++x) products(p0 + x, vf[k & 1][x]);
 #endif
+      __builtin_amdgcn_sched_barrier(0);
     }
 #endif
+#undef score
     live = live_next;
-    arrive();
+    wait_for<LOADS>();
+    __syncthreads();
   }
 
   // The same stages' keys once more, one at a time: the elements of their values that are not finite.
   if (some_odd) {
 #pragma unroll 1
     for (int key = lo; key < hi; ++key) {
-      const int base = lo + (key - lo) / KT * KT, tile = (key - base) / 16;
-      if (!edge(base) || tile / NK != wk) continue;
+      const int base = lo + (key - lo) / KT * KT, tile = (key - base) / TILE;
       const int page = table[page_of(a, key)], j = key - sq.past;
-      if ((u32)page >= (u32)a.pages) continue;
+      if (!edge(base) || tile / NK != wk || (u32)page >= (u32)a.pages) continue;
       const char* v = vbase + page * a.c_page + (key - page_of(a, key) * a.page) * a.c_token;
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
         bool sees = key >= from[t] && j <= index[t];
-        if (a.tree)
-          sees = j < 0 ? key >= from[t]
-                       : (tree_bits(a, row[t], j) & 1) &&
-                             (!deep || tree_count(a, row[t], j, sq.end - sq.past) <= a.window);
-        if (!sees) continue;
+        if (a.tree) {
+          sees = j < 0 ? key >= from[t] : tree_bits(a, (a.tree + (sq.begin + index[t]) * a.tree_row), bits[t], j) & 1;
+          if (deep && j >= 0)
+            sees = sees && tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), j, sq.end - sq.past) <= a.window;
+        }
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < RA * 4; ++i) {
             const int d = element_of(p, i);
-            if (d < a.dim && !(__builtin_fabsf(element(v + d * CS)) < __builtin_inff()))
-              o[t][p][i] = __builtin_nanf("");
+            const float x = element(v + (d < a.dim ? d : 0) * CS);
+            // 0x207: a NaN or an infinity
+            o[t][p][i] = sees && __builtin_amdgcn_classf(x, 0x207) ? __builtin_nanf("") : o[t][p][i];
           }
       }
     }
@@ -772,64 +875,73 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    l[t] = ek::reduce_xor<ek::Sum, 16>(l[t]);
+    if constexpr (TILE == 16) l[t] = ek::reduce_xor<ek::Sum, 16>(l[t]);
     l[t] = ek::reduce_xor<ek::Sum, 32>(l[t]);
   }
   if constexpr (WK > 1) {
     // the waves of the same columns: to the first of them, in the order in which it holds its own
     float* part = (float*)s_stage;
-    constexpr int SIZE = CT * (NP * 256 + 128);
-    float* mine = part + ((wk - 1) * WC + wc) * SIZE;
+    constexpr int SIZE = CT * (NP * RA * 256 + 128), ML = CT * NP * RA * 256;
+    float* mine = part + ((wk - 1) * WC + wc) * SIZE + lane * 4;
     if (wk > 0) {
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
 #pragma unroll
         for (int p = 0; p < NP; ++p)
-          *(ek::f32x4*)(mine + (t * NP + p) * 256 + lane * 4) = o[t][p];
-        mine[CT * NP * 256 + t * 128 + lane] = m[t];
-        mine[CT * NP * 256 + t * 128 + 64 + lane] = l[t];
+#pragma unroll
+          for (int k = 0; k < RA; ++k)
+            *(ek::f32x4*)(mine + ((t * NP + p) * RA + k) * 256) =
+                ek::f32x4{o[t][p][k * 4], o[t][p][k * 4 + 1], o[t][p][k * 4 + 2], o[t][p][k * 4 + 3]};
+        mine[ML + t * 128 - lane * 3] = m[t];
+        mine[ML + t * 128 + 64 - lane * 3] = l[t];
       }
     }
     __syncthreads();
     if (wk > 0) return;
 #pragma unroll
-    for (int k = 0; k < WK - 1; ++k) {
-      const float* other = part + (k * WC + wc) * SIZE;
+    for (int x = 0; x < WK - 1; ++x) {
+      const float* other = part + (x * WC + wc) * SIZE;
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        const float mo = other[CT * NP * 256 + t * 128 + lane];
-        const float lo = other[CT * NP * 256 + t * 128 + 64 + lane];
+        const float mo = other[ML + t * 128 + lane], lo = other[ML + t * 128 + 64 + lane];
         const float top = __builtin_fmaxf(m[t], mo), use = top == -__builtin_inff() ? 0.0f : top;
         const float f = ek::exp2_fast((m[t] - use) * scale), fo = ek::exp2_fast((mo - use) * scale);
         m[t] = top;
         l[t] = l[t] * f + lo * fo;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          const ek::f32x4 y = *(const ek::f32x4*)(other + (t * NP + p) * 256 + lane * 4);
-          o[t][p] = o[t][p] * f + y * fo;
-        }
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int k = 0; k < RA; ++k) {
+            const ek::f32x4 y = *(const ek::f32x4*)(other + ((t * NP + p) * RA + k) * 256 +
+                                                    lane * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][p][k * 4 + i] = o[t][p][k * 4 + i] * f + y[i] * fo;
+          }
       }
     }
   }
 
-  // rows of VE or (transposed) 4 adjacent elements
+  // runs of VE or (transposed) 4 adjacent elements
   constexpr int OUT = TR ? 4 : VE;
-  const auto each_run = [&](int t, const auto& put) {
+  const auto each_run = [&](int t, const auto& put) EK_HERE {
     if constexpr (TR) {
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const float y[4] = {o[t][p][0], o[t][p][1], o[t][p][2], o[t][p][3]};
-        put(p * 16 + c * 4, y);
-      }
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int k = 0; k < RA; ++k) {
+          const float y[4] = {o[t][p][k * 4], o[t][p][k * 4 + 1], o[t][p][k * 4 + 2],
+                              o[t][p][k * 4 + 3]};
+          put(element_of(p, k * 4), y);
+        }
     } else {
 #pragma unroll
       for (int p = 0; p < NP; p += VE)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RA * 4; ++i) {
           float y[VE];
 #pragma unroll
           for (int e = 0; e < VE; ++e) y[e] = o[t][p + e][i];
-          put(p * 16 + (c * 4 + i) * VE, y);
+          put(element_of(p, i), y);
         }
     }
   };
@@ -837,12 +949,12 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   for (int t = 0; t < CT; ++t) {
     if (!valid(t)) continue;
     const int64_t token = sq.begin + index[t];
-    const int h = g * a.group + head(t);
+    const int h = head[t];
     if (it.chunks == 1) {
       const bool any = l[t] > 0.0f || l[t] != l[t];
-      const float f = any ? a.v_scale / LIFT / l[t] : 0.0f;
+      const float f = any ? a.v_scale / l[t] : 0.0f;
       T* dst = a.out + token * a.out_row + h * a.out_head;
-      each_run(t, [&](int d, const float* x) {
+      each_run(t, [&](int d, const float* x) EK_HERE {
         T y[OUT];
 #pragma unroll
         for (int e = 0; e < OUT; ++e) y[e] = result(x[e], f, any);
@@ -850,13 +962,13 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       });
       if (a.lse && c == 0)
         a.lse[token * a.heads + h] =
-            any ? (m[t] * scale + __builtin_log2f(l[t])) * LN2 : -__builtin_inff();
+            any ? (m[t] * scale + (__builtin_log2f(l[t]) - LIFT)) * LN2 : -__builtin_inff();
     } else {
       const int slot = it.slot + it.chunk * it.blocks + it.block;
       if (!a.part || slot < 0 || slot >= a.slots) continue;
-      const int64_t at = ((int64_t)slot * a.kv_heads + g) * COLS + wc * CT * 16 + t * 16 + r;
+      const int64_t at = ((int64_t)slot * a.kv_heads + g) * COLS + (wc * CT + t) * TILE + r;
       float* dst = a.part + at * a.dim;
-      each_run(t, [&](int d, const float* y) {
+      each_run(t, [&](int d, const float* y) EK_HERE {
         if (d < a.dim) {
 #pragma unroll
           for (int e = 0; e < OUT; e += 4) ek::vstore_u<float, 4>(dst + d + e, y + e);
@@ -870,12 +982,16 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     }
   }
 }
+#undef valid
 
-// Joins the chunks of a token's head, a wave each.
+// Joins the chunks of a token's head: `join` waves (1 or 4) take 16 of them in turn, all of their
+// loads on their way at once, and meet in the LDS.
 extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params a) {
-  constexpr int DW = (DP + 127) / 128;
-  const int lane = ek::lane_id(), token = blockIdx.x;
-  const int head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int DW = (DP + 127) / 128, BATCH = 16;
+  __shared__ float s_o[4][DP], s_m[4], s_l[4];
+  const int lane = ek::lane_id(), token = blockIdx.x, waves = a.join;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = waves == 1 ? blockIdx.y * 4 + wave : blockIdx.y, first = waves == 1 ? 0 : wave;
   if (head >= a.heads || token < a.cu[0] || token >= a.cu[a.batch * a.cu_step]) return;
   const Row row = part_rows(a)[token];
   if (row.chunks <= 1 || row.slot < 0 || row.blocks <= 0 || row.index < 0 ||
@@ -885,41 +1001,87 @@ extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params 
   const int block = col / COLS;
   if (block >= row.blocks) return;
   const float scale = scale_of(a);
-  const int64_t first = ((int64_t)(row.slot + block) * a.kv_heads + g) * COLS + col - block * COLS;
+  const int64_t at = ((int64_t)(row.slot + block) * a.kv_heads + g) * COLS + col - block * COLS;
   const int64_t step = (int64_t)row.blocks * a.kv_heads * COLS;    // from chunk to chunk
   float m = -__builtin_inff(), l = 0.0f, x[DW][2];
 #pragma unroll
   for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
 #pragma unroll 1
-  for (int i0 = 0; i0 < row.chunks; i0 += 64) {
-    // a lane each: the weights of 64 chunks
-    const int i = i0 + lane;
-    const float* ml = part_ml(a) + (first + (i < row.chunks ? i : i0) * step) * 2;
-    const float mi = i < row.chunks ? ml[0] : -__builtin_inff();
-    const float li = i < row.chunks ? ml[1] : 0.0f;
-    const float m_new = __builtin_fmaxf(m, wave_all<ek::Max>(mi));
-    const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-    const float f = ek::exp2_fast((m - mu) * scale), w = ek::exp2_fast((mi - mu) * scale);
-    l = l * f + wave_all<ek::Sum>(li * w);
-    m = m_new;
+  for (int i0 = first * BATCH; i0 < row.chunks; i0 += waves * BATCH) {
+    const int count = row.chunks - i0 < BATCH ? row.chunks - i0 : BATCH, i = lane & (BATCH - 1);
+    const float* ml = part_ml(a) + (at + (i0 + (i < count ? i : 0)) * step) * 2;
+    float mi = ml[0], li = ml[1], v[BATCH][DW][2];
+#pragma unroll
+    for (int j0 = 0; j0 < BATCH; j0 += 4)
+      if (j0 < count) {
+#pragma unroll
+        for (int j = j0; j < j0 + 4; ++j) {
+          const float* src = a.part + (at + (i0 + (j < count ? j : 0)) * step) * a.dim;
+#pragma unroll
+          for (int k = 0; k < DW; ++k) {
+            const int d = k * 128 + lane * 2;
+            ek::vload_u<float, 2>(v[j][k], src + (d < a.dim ? d : 0));
+          }
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);               // all of them before the first wait
+    mi = i < count ? mi : -__builtin_inff();
+    li = i < count ? li : 0.0f;
+    // lanes that differ in their upper bits have the same chunks
+    float top = ek::reduce_xor<ek::Max, 1>(mi);
+    top = ek::reduce_xor<ek::Max, 2>(top);
+    top = ek::reduce_xor<ek::Max, 4>(top);
+    top = __builtin_fmaxf(m, ek::reduce_xor<ek::Max, 8>(top));
+    const float use = top == -__builtin_inff() ? 0.0f : top;
+    const float f = ek::exp2_fast((m - use) * scale), w = ek::exp2_fast((mi - use) * scale);
+    float sum = ek::reduce_xor<ek::Sum, 1>(li * w);
+    sum = ek::reduce_xor<ek::Sum, 2>(sum);
+    sum = ek::reduce_xor<ek::Sum, 4>(sum);
+    sum = ek::reduce_xor<ek::Sum, 8>(sum);
+    l = __builtin_fmaf(l, f, sum);
+    m = top;
 #pragma unroll
     for (int k = 0; k < DW; ++k) x[k][0] *= f, x[k][1] *= f;
-    const int count = row.chunks - i0 < 64 ? row.chunks - i0 : 64;
-    for (int j = 0; j < count; ++j) {
-      const float y = ek::bits_f32((u32)__builtin_amdgcn_readlane((int)ek::f32_bits(w), j));
-      const float* src = a.part + (first + (i0 + j) * step) * a.dim;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j)
+      if (j < count) {
+        const float y = ek::bits_f32((u32)__builtin_amdgcn_readlane((int)ek::f32_bits(w), j));
+#pragma unroll
+        for (int k = 0; k < DW; ++k) {
+          x[k][0] = __builtin_fmaf(v[j][k][0], y, x[k][0]);
+          x[k][1] = __builtin_fmaf(v[j][k][1], y, x[k][1]);
+        }
+      }
+  }
+  if (waves > 1) {
+    // a part whose m is -inf has no weight, whatever wave it is
+#pragma unroll
+    for (int k = 0; k < DW; ++k) {
+      const int d = k * 128 + lane * 2;
+      if (d < DP) s_o[wave][d] = x[k][0], s_o[wave][d + 1] = x[k][1];
+    }
+    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float mo = s_m[w], top = __builtin_fmaxf(m, mo);
+      const float use = top == -__builtin_inff() ? 0.0f : top;
+      const float f = ek::exp2_fast((m - use) * scale), fo = ek::exp2_fast((mo - use) * scale);
+      l = l * f + s_l[w] * fo;
+      m = top;
 #pragma unroll
       for (int k = 0; k < DW; ++k) {
         const int d = k * 128 + lane * 2;
-        float v[2];
-        ek::vload_u<float, 2>(v, src + (d < a.dim ? d : 0));
-        x[k][0] = __builtin_fmaf(v[0], y, x[k][0]);
-        x[k][1] = __builtin_fmaf(v[1], y, x[k][1]);
+        if (d < DP) {
+          x[k][0] = x[k][0] * f + s_o[w][d] * fo;
+          x[k][1] = x[k][1] * f + s_o[w][d + 1] * fo;
+        }
       }
     }
   }
   const bool any = l > 0.0f || l != l;
-  const float f = any ? a.v_scale / LIFT / l : 0.0f;
+  const float f = any ? a.v_scale / l : 0.0f;
   T* dst = a.out + token * a.out_row + head * a.out_head;
 #pragma unroll
   for (int k = 0; k < DW; ++k) {
@@ -931,5 +1093,5 @@ extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params 
   }
   if (a.lse && lane == 0)
     a.lse[(int64_t)token * a.heads + head] =
-        any ? (m * scale + __builtin_log2f(l)) * LN2 : -__builtin_inff();
+        any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
 }

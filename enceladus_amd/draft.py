@@ -50,7 +50,7 @@ def _tree(tree, tokens: int):
 
 # -- attention -------------------------------------------------------------------------------
 
-_ATTEND = struct.Struct("<11q11iI4iI3f")
+_ATTEND = struct.Struct("<11q11iI5iI3f4x")
 _UNIT = 64                          # tokens: what a sequence is split in multiples of
 _MIN_UNITS = 1                      # of a chunk
 _GROUPS = 2                         # workgroups per CU
@@ -123,15 +123,20 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
     return (out, lse) if return_lse else out
 
 
-def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int]:
-    """(keys of a stage, column tiles of a wave, waves over columns, waves over keys) for sequences
-    of so many columns of a key head, in heads of `width` cached elements of `size` bytes."""
+def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, int]:
+    """(keys of a stage, columns of a tile, tiles of a wave, waves over columns, waves over keys) for
+    sequences of so many columns of a key head, in heads of `width` cached elements of `size`
+    bytes."""
     keys = max(16, min(64, 16384 // (width * size)))
-    tiles = 2 if width <= 128 and size <= 2 and columns > 16 else 1
-    over = 1
-    while over < 4 and (columns > 16 * tiles * over or keys < 64 // over):
-        over *= 2
-    return keys, tiles, over, 4 // over
+    if size == 4 or width == 256:
+        over = 1
+        while over < 4 and (columns > 16 * over or keys < 64 // over):
+            over *= 2
+        return keys, 16, 1, over, 4 // over
+    if columns <= 32:
+        return (keys, 16, 1, 1, 4) if columns <= 16 else (keys, 16, 1, 2, 2)
+    over = 2 if columns <= 64 else 4
+    return (keys, 16, 2, over, 4 // over) if width * size == 64 else (keys, 32, 1, over, 4 // over)
 
 
 def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree, scale, window,
@@ -177,8 +182,8 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
         capacity = 0
     window = min(window, _d.MAX_TOKENS)
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
-    keys, tiles, over, split = _shape(tokens / batch * group, width, kc.size)
-    cols = 16 * tiles * over
+    keys, tile, tiles, over, split = _shape(tokens / batch * group, width, kc.size)
+    cols = tile * tiles * over
     waves = over * split
     # blocks of columns: each sequence may have one that is not whole
     blocks = -(-tokens * group // cols) if batch == 1 else tokens * group // cols + \
@@ -191,22 +196,27 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
     need(x * 64 * waves < 1 << 32 and kv_heads <= 65535, f"{tokens} tokens are too many for one "
                                                          "call")
     macros = (("EK_Q", _d._Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
-              ("EK_KT", keys), ("EK_CT", tiles), ("EK_WC", over), ("EK_WK", split),
+              ("EK_PAD", int(dim != width)), ("EK_KT", keys), ("EK_TILE", tile),
+              ("EK_CT", tiles), ("EK_WC", over), ("EK_WK", split),
               ("EK_OCC", 1 if width * kc.size == 1024 else 2))
     launches = [("ek_tree_attention", (x, kv_heads), 64 * waves)]
     slots = workspace = 0
+    join = 1
     # one sequence of as many blocks as there are items has one chunk
     if most > _MIN_UNITS and not (batch == 1 and blocks >= items):
         slots = 2 * items
         workspace = slots * kv_heads * cols * (dim + 2) * 4 + 16 * tokens
-        launches.append(("ek_tree_attention_join", (tokens, -(-heads // 4)), 256))
+        # several waves where a token's head may have many chunks
+        join = 4 if min(items // blocks, most) > 16 else 1
+        launches.append(("ek_tree_attention_join", (tokens, heads if join > 1 else -(-heads // 4)),
+                         256))
     log2e = 1.4426950408889634
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], cu.strides[0],
         ta.strides[0] if ta else 0, tokens, batch, heads, kv_heads, group, dim, kc.shape[1],
         kc.shape[0], capacity, window, ta.shape[1] if ta else 0, *_d._page_division(kc.shape[1]),
-        items, slots, _MIN_UNITS,
+        items, slots, _MIN_UNITS, join,
         0 if scale >= 0 else 0x80000000 if qa.kind == "fp32" else 0x80008000,
         # so small a scale is as good as none, and keeps -inf (no key there) what it is
         max(abs(scale) * k_scale * log2e, 2.0 ** -126), softcap * log2e, v_scale)
