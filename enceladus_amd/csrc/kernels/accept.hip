@@ -18,7 +18,7 @@ typedef ek::bf16 T;
 #endif
 typedef uint32_t u32;
 constexpr int E = 16 / sizeof(T);                   // logits of a vector
-constexpr int THREADS = 256, UNROLL = 4;
+constexpr int THREADS = 256, UNROLL = 8;
 constexpr int MOST = 1024;                          // nodes of a tree
 
 struct Params {
@@ -56,43 +56,54 @@ EK_INLINE uint64_t largest(uint64_t x) {
   return larger_of<32>(x);
 }
 
+// A lane's largest so far, the vector that it is in, and the first vector with a NaN.
+struct Top { float value; int at, nan_at; };
+
+EK_INLINE void look_at(Top& top, const T* w, int at) {
+  float m = ek::f32(w[0]);
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const float x = ek::f32(w[e]), y = ek::f32(w[e + 1]);
+    m = __builtin_fmaxf(m, __builtin_fmaxf(x, y));
+    nan |= __builtin_isunordered(x, y);
+  }
+  top.at = m > top.value ? at : top.at;
+  top.value = m > top.value ? m : top.value;
+  top.nan_at = nan && at < top.nan_at ? at : top.nan_at;
+}
+
 extern "C" __global__ __launch_bounds__(THREADS) void ek_row_best(Params a) {
   __shared__ uint64_t s_best[THREADS / 64];
   const int row = blockIdx.x / (u32)a.pieces, piece = blockIdx.x - row * a.pieces;
   const T* x = a.logits + row * a.logits_row;
   const int begin = piece * a.span;
   const int end = a.vocab - begin < a.span ? a.vocab : begin + a.span;
-  float top = -__builtin_inff();
-  int at = begin + threadIdx.x * E, nan_at = 0x7FFFFFFF;       // the vectors' first logits
-  for (int base = begin + threadIdx.x * E; base < end; base += THREADS * E * UNROLL) {
+  const int first = begin + threadIdx.x * E;
+  constexpr int STEP = THREADS * E;
+  Top top = {-__builtin_inff(), first, 0x7FFFFFFF};
+  int base = begin;
+  // whole rounds without a branch, so that all of their loads are on their way at once
+  for (; base + STEP * UNROLL <= end; base += STEP * UNROLL) {
     T w[UNROLL][E];
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-      const int i = base + k * THREADS * E;
-      if (i + E <= end) ek::vload_u<T, E>(w[k], x + i);
-      else
+    for (int k = 0; k < UNROLL; ++k)
+      ek::vload_nt_u<T, E>(w[k], x + base + threadIdx.x * E + k * STEP);
 #pragma unroll
-        for (int e = 0; e < E; ++e) w[k][e] = i + e < end ? x[i + e] : ek::cvt<T>(-__builtin_inff());
-    }
+    for (int k = 0; k < UNROLL; ++k) look_at(top, w[k], base + threadIdx.x * E + k * STEP);
+  }
+  for (; base < end; base += STEP) {
+    const int at = base + threadIdx.x * E;
+    T w[E];
+    if (at + E <= end) ek::vload_nt_u<T, E>(w, x + at);
+    else
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-      const int i = base + k * THREADS * E;
-      float m = ek::f32(w[k][0]);
-      bool nan = m != m;
-#pragma unroll
-      for (int e = 1; e < E; ++e) {
-        const float y = ek::f32(w[k][e]);
-        m = __builtin_fmaxf(m, y);
-        nan |= y != y;
-      }
-      at = m > top ? i : at;
-      top = m > top ? m : top;
-      nan_at = nan && i < nan_at ? i : nan_at;
-    }
+      for (int e = 0; e < E; ++e) w[e] = at + e < end ? x[at + e] : ek::cvt<T>(-__builtin_inff());
+    if (at < end) look_at(top, w, at);
   }
   // the largest of the lane's vector, by its place
   uint64_t mine = 0;
-  const int look = nan_at != 0x7FFFFFFF ? nan_at : at;
+  const int look = top.nan_at != 0x7FFFFFFF ? top.nan_at : top.at;
   if (look < end) {
 #pragma unroll
     for (int e = 0; e < E; ++e)

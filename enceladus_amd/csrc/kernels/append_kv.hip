@@ -111,6 +111,16 @@ template <bool NT = false, typename S> EK_INLINE void load(float* x, const S* p)
 
 __device__ const float s_zeros[8] = {};              // what is no cos or sin
 
+#if EK_AXES
+// The row of cos and sin by which pair j turns, of those on the four axes.
+EK_INLINE int turn_at(const Params& a, int j, int on0, int on1, int on2, int on3) {
+  const uint64_t w = j < 64 ? j < 32 ? a.pair_axes[0] : a.pair_axes[1]
+                            : j < 96 ? a.pair_axes[2] : a.pair_axes[3];
+  const int x = (int)(w >> 2 * (j & 31)) & 3;
+  return x < 2 ? x < 1 ? on0 : on1 : x < 3 ? on2 : on3;
+}
+#endif
+
 extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
   const int lane = ek::lane_id();
   const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -151,21 +161,15 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
   const int pos = (len > 0 ? len : 0) - back;      // a negative length is none: no wrapping round
 #if EK_AXES
   if (pos < 0 || pos >= a.capacity) return;
-  // its places in cos and sin: all four on their way at once, those of no axis the first's
-  int turn_of[4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-    turn_of[x] = a.turns[(x < a.axes ? x : 0) * a.turn_axis + t * a.turn_step];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-    if ((uint32_t)turn_of[x] >= (uint32_t)a.positions) return;
-  // of pair j
-  const auto turn_at = [&](int j) {
-    const uint64_t w = j < 64 ? j < 32 ? a.pair_axes[0] : a.pair_axes[1]
-                              : j < 96 ? a.pair_axes[2] : a.pair_axes[3];
-    const int x = (int)(w >> 2 * (j & 31)) & 3;
-    return x < 2 ? x < 1 ? turn_of[0] : turn_of[1] : x < 3 ? turn_of[2] : turn_of[3];
-  };
+  // its rows of cos and sin, on their way at once: an axis that is not there is the first
+  const int32_t* turns = a.turns + t * a.turn_step;
+  const int on0 = turns[0], on1 = turns[a.axes > 1 ? a.turn_axis : 0];
+  const int on2 = turns[a.axes > 2 ? 2 * a.turn_axis : 0];
+  const int on3 = turns[a.axes > 3 ? 3 * a.turn_axis : 0];
+  const uint32_t most = a.positions;
+  if ((uint32_t)on0 >= most || (uint32_t)on1 >= most || (uint32_t)on2 >= most ||
+      (uint32_t)on3 >= most)
+    return;
 #else
   if (pos < 0 || pos >= a.capacity || (a.rotary && pos >= a.positions)) return;
 #endif
@@ -190,13 +194,13 @@ extern "C" __global__ __launch_bounds__(256) void ek_append_kv(Params a) {
 #if EK_AXES == 2
 #pragma unroll
     for (int i = 0; i < (EK_PAIRS ? V / 2 : V); ++i) {
-      const int at = turn_at(turn ? j0 + i : 0);
+      const int at = turn_at(a, turn ? j0 + i : 0, on0, on1, on2, on3);
       cs[i] = turn ? a.cos[at * a.cos_row + j0 + i] : 0.0f;
       sn[i] = turn ? a.sin[at * a.sin_row + j0 + i] : 0.0f;
     }
 #else
 #if EK_AXES
-    const int at = turn_at(turn ? j0 : 0);
+    const int at = turn_at(a, turn ? j0 : 0, on0, on1, on2, on3);
 #else
     const int at = pos;
 #endif

@@ -699,13 +699,27 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #pragma unroll
         for (int p = 0; p < NP; ++p) o[t][p] *= alpha;
       }
+      // exp2(scale (s - m)): in one step where scale m has digits to spare next to 2^-17, which a
+      // weight's terms leave out, else the difference first
+      const float top = m_use * scale;
+      if (__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(top) < 256.0f)) == 0) {
+        const float less = LIFT - top;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i), scale, less));
+      } else {
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i) - m_use, scale, LIFT));
+      }
 #pragma unroll
       for (int s = 0; s < RUNS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i) - m_use, scale, LIFT));
-          l[t] += score(t, s, i);
-        }
+        for (int i = 0; i < 4; ++i) l[t] += score(t, s, i);
     }
 
     if (next < hi) wait_for<2 * LOADS + 1>();

@@ -272,7 +272,7 @@ def accept(logits, tokens, cu_tokens, *, tree=None, most: int | None = None):
     return tuple(new)
 
 
-_BEST_THREADS, _BEST_UNROLL = 256, 4     # of a workgroup of accept.hip
+_BEST_THREADS, _BEST_UNROLL = 256, 8     # of a workgroup of accept.hip
 
 
 def _accept_plan(logits, tokens, cu_tokens, tree, most):
@@ -300,8 +300,6 @@ def _accept_plan(logits, tokens, cu_tokens, tree, most):
     span = vector * _BEST_UNROLL
     while span > vector and rows * -(-vocab // span) < 2 * C.coarsen_cap():
         span //= 2
-    while span < 8 * vector and rows * -(-vocab // span) > 32 * C.coarsen_cap():
-        span *= 2
     pieces = -(-vocab // span)
     need(rows * pieces < 1 << 24, f"logits of shape {la.shape} are too large for one call")
     launches = [("ek_accept", (batch, 1), _BEST_THREADS)] if batch else []
