@@ -3,8 +3,10 @@
 //
 // The first kernel reads the logits once, which is the time of a large call (the HBM rate); a small
 // one is two launches. A lane keeps the largest of each vector that it reads and which vector that
-// was, a bit more than two instructions per logit, and only the largest of a stretch is looked up
-// in its vector. Whole numbers alone leave it: the order of a row's stretches does not matter.
+// was, two instructions per logit; only the row's best vector is looked into, by the second kernel
+// (every lane's own, in the first, read them twice as far as memory goes: 1381 rows of 128000 bf16,
+// 354 MB, 151 us a call instead of 62). Whole numbers alone leave it: the order of a row's stretches
+// does not matter.
 //
 // Macros: EK_Q (logits: 0 fp32, 1 fp16, 2 bf16).
 #include "enceladus_cdna4.h"
@@ -29,7 +31,7 @@ struct Params {
   int32_t* path;                     // [batch, most]
   int32_t* count;
   int32_t* chosen;
-  uint64_t* best;                    // [rows, pieces]: value and place of a stretch's largest
+  uint64_t* best;                    // [rows, pieces]: a stretch's largest value, and its vector
   int64_t logits_row, tokens_step, cu_step, tree_row;
   int32_t rows, vocab, batch, words, most, pieces, span;
 };
@@ -101,14 +103,9 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_row_best(Params a) {
       for (int e = 0; e < E; ++e) w[e] = at + e < end ? x[at + e] : ek::cvt<T>(-__builtin_inff());
     if (at < end) look_at(top, w, at);
   }
-  // the largest of the lane's vector, by its place
-  uint64_t mine = 0;
-  const int look = top.nan_at != 0x7FFFFFFF ? top.nan_at : top.at;
-  if (look < end) {
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (look + e < end) mine = larger(mine, rank(ek::f32(x[look + e]), look + e));
-  }
+  uint64_t mine = rank(top.value, top.at);
+  if (top.nan_at != 0x7FFFFFFF) mine = rank(__builtin_nanf(""), top.nan_at);
+  if (first >= end) mine = 0;
   mine = largest(mine);
   if (ek::lane_id() == 0) s_best[threadIdx.x >> 6] = mine;
   __syncthreads();
@@ -119,11 +116,21 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_row_best(Params a) {
   }
 }
 
+// The place of a row's largest logit: the best of its stretches, then the first of its vector.
 EK_INLINE int best_of(const Params& a, int row) {
   uint64_t r = 0;
 #pragma unroll 4
   for (int p = 0; p < a.pieces; ++p) r = larger(r, a.best[(int64_t)row * a.pieces + p]);
-  return place(r);
+  const int at = place(r);
+  const T* x = a.logits + row * a.logits_row + at;
+  float w[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) w[e] = ek::f32(x[at + e < a.vocab ? e : 0]);
+  int found = 0;
+#pragma unroll
+  for (int e = E - 1; e >= 0; --e)
+    if (at + e < a.vocab && rank(w[e], 0) >> 32 == r >> 32) found = e;
+  return at + found;
 }
 
 extern "C" __global__ __launch_bounds__(THREADS) void ek_accept(Params a) {
