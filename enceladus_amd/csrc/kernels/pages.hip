@@ -57,25 +57,30 @@ struct Walk {
   }
 };
 
-constexpr int THREADS = 256, UNROLL = 4;             // of a copy: 16 KB per workgroup
+constexpr int THREADS = 256;
+// Accesses of a thread: whole pages are copied best by small pieces (1258 MB: 197 us with 1, 228 with
+// 2, 238 with 4, 243 with 8), parts of them by few (192 forks of 7 tokens in 32 caches, 206 MB: 34 us
+// with 8, 39 with 4, 60 with 1).
+constexpr int COPY = 1, FORK = 8;
 
 // `tokens` tokens of page `from` into page `to`: piece `piece` of them, in one cache.
-EK_INLINE void copy_piece(const Params& a, char* cache, int from, int to, int tokens, int piece) {
+template <int N> EK_INLINE void copy_piece(const Params& a, char* cache, int from, int to,
+                                           int tokens, int piece) {
   const u32 all = (u32)tokens * (u32)a.heads * (u32)(a.row_bytes / V);
   const char* src = cache + from * a.c_page;
   char* dst = cache + to * a.c_page;
-  const u32 base = (u32)piece * (THREADS * UNROLL) + threadIdx.x;
+  const u32 base = (u32)piece * (THREADS * N) + threadIdx.x;
   const Walk place(a, tokens);
-  uint8_t w[UNROLL][V];
-  int64_t at[UNROLL];
+  uint8_t w[N][V];
+  int64_t at[N];
 #pragma unroll
-  for (int k = 0; k < UNROLL; ++k) {
+  for (int k = 0; k < N; ++k) {
     const u32 i = base + k * THREADS;
     at[k] = place(i < all ? i : 0);
     if (i < all) get(w[k], src + at[k]);
   }
 #pragma unroll
-  for (int k = 0; k < UNROLL; ++k)
+  for (int k = 0; k < N; ++k)
     if (base + k * THREADS < all) put(dst + at[k], w[k]);
 }
 
@@ -84,7 +89,7 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_copy_pages(Params a) {
   const int i = blockIdx.x / (u32)a.pieces, piece = blockIdx.x - i * a.pieces;
   const int from = a.first[i * a.first_step], to = a.second[i * a.second_step];
   if ((u32)from >= (u32)a.pages || (u32)to >= (u32)a.pages || from == to) return;
-  copy_piece(a, a.caches[blockIdx.y], from, to, a.page, piece);
+  copy_piece<COPY>(a, a.caches[blockIdx.y], from, to, a.page, piece);
 }
 
 // Token first[b] + second[b][i] becomes token first[b] + i of sequence b, for i < counts[b], in
@@ -192,22 +197,37 @@ EK_INLINE int64_t scan_group(u32 x, int64_t* total, u32* s_wave) {
   return before + end - x;
 }
 
-// The lowest `want` free pages into `found`, in their order; how many there are.
-EK_INLINE int find_free(const Params& a, int want, int32_t* found, u32* s_wave) {
-  constexpr int EACH = 8;
+constexpr int EACH = 8;                            // counts of a thread and round
+struct Counts { int32_t r[EACH]; };
+
+// The counts of this thread's pages from p on (1 behind the last).
+EK_INLINE Counts counts_at(const Params& a, int p) {
+  Counts c;
+  if (p + EACH <= a.pages) {
+    ek::vload_u<int32_t, 4>(c.r, a.refs + p);
+    ek::vload_u<int32_t, 4>(c.r + 4, a.refs + p + 4);
+  } else {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) c.r[k] = p + k < a.pages ? a.refs[p + k] : 1;
+  }
+  return c;
+}
+
+// The lowest `want` free pages into `found`, in their order; how many there are. `c`: the counts of
+// the first round, read before they are needed.
+EK_INLINE int find_free(const Params& a, int want, int32_t* found, u32* s_wave, Counts c) {
   int have = 0;
   for (int base = 0; base < a.pages && have < want; base += WG * EACH) {
     const int p = base + threadIdx.x * EACH;
-    int r[EACH], count = 0;
+    if (base > 0) c = counts_at(a, p);
+    int count = 0;
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) r[k] = p + k < a.pages ? a.refs[p + k] : 1;
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) count += r[k] == 0;
+    for (int k = 0; k < EACH; ++k) count += c.r[k] == 0;
     int64_t total;
     int at = have + (int)scan_group(count, &total, s_wave);
 #pragma unroll
     for (int k = 0; k < EACH; ++k)
-      if (r[k] == 0) {
+      if (c.r[k] == 0) {
         if (at < want) found[at] = p + k;
         ++at;
       }
@@ -216,6 +236,9 @@ EK_INLINE int find_free(const Params& a, int want, int32_t* found, u32* s_wave) 
   __syncthreads();                                 // `found` is read by others next
   return have < want ? have : want;
 }
+
+// What threads exchange about up to SMALL rows is in the LDS, of more in memory.
+constexpr int SMALL = 4096;
 
 // Pages that row b still needs for first[b] tokens, or -1 where it can't have them.
 EK_INLINE int need_of(const Params& a, int b, int& have) {
@@ -228,11 +251,14 @@ EK_INLINE int need_of(const Params& a, int b, int& have) {
 
 // Sequence b grows to first[b] tokens: rows in their order take the lowest free pages. A row is
 // served if the pages that it and the rows before it need are there. `work`: the ends of the rows'
-// shares [rows], then the pages found [most].
+// shares [rows], then the pages found [most]. 256 rows, 65536 pages: a chain of loads and barriers,
+// 5.2 us.
 extern "C" __global__ __launch_bounds__(WG) void ek_take_pages(Params a) {
   __shared__ u32 s_wave[WG / 64];
-  int32_t* ends = a.work;
+  __shared__ int32_t s_ends[SMALL];
+  int32_t* ends = a.n <= SMALL ? s_ends : a.work;
   int32_t* found = a.work + a.n;
+  const Counts counts = counts_at(a, threadIdx.x * EACH);
   int64_t sum = 0;
   for (int b0 = 0; b0 < a.n; b0 += WG) {
     const int b = b0 + threadIdx.x;
@@ -246,7 +272,7 @@ extern "C" __global__ __launch_bounds__(WG) void ek_take_pages(Params a) {
   }
   const int want = sum > a.pages ? a.pages : (int)sum;
   __syncthreads();
-  const int got = find_free(a, want, found, s_wave);
+  const int got = find_free(a, want, found, s_wave, counts);
   // the pages to their rows: the first row whose share ends behind a page's rank
   for (int r = threadIdx.x; r < got; r += WG) {
     int lo = 0, hi = a.n - 1;
@@ -257,9 +283,9 @@ extern "C" __global__ __launch_bounds__(WG) void ek_take_pages(Params a) {
     }
     if (ends[lo] > got) continue;                  // not all of its pages are there
     int have;
-    const int need = need_of(a, lo, have);
-    a.table[lo * a.table_row + have + r - (ends[lo] - need)] = found[r];
-    a.refs[found[r]] = 1;
+    const int need = need_of(a, lo, have), page = found[r];
+    a.table[lo * a.table_row + have + r - (ends[lo] - need)] = page;
+    a.refs[page] = 1;
   }
   __syncthreads();                                 // lengths are still read above
   for (int b = threadIdx.x; b < a.n; b += WG) {
@@ -274,49 +300,55 @@ extern "C" __global__ __launch_bounds__(WG) void ek_take_pages(Params a) {
 
 // Which forks are served, and the fresh pages of those whose source ends inside a page. `work`:
 // [rows] the first fork to each row, [rows] whether the row is a source, [n] ends of the shares,
-// [n] a fork's fresh page (-1: none), [n] pages found.
-EK_INLINE int fork_need(const Params& a, int i, bool& ok) {
+// [n] a fork's fresh page (-1: none), [n] pages found. 192 forks in 256 rows: 5.2 us.
+struct Fork { bool ok; int need; };
+
+EK_INLINE Fork fork_of(const Params& a, int i, const int32_t* owner, const int32_t* source) {
   const int from = a.first[i * a.first_step], to = a.second[i * a.second_step];
-  ok = (u32)from < (u32)a.rows && (u32)to < (u32)a.rows;
-  if (!ok) return 0;
-  const int len = a.lens[from * a.lens_step];
-  ok = a.work[to] == i && a.work[a.rows + to] == 0 && a.lens[to * a.lens_step] <= 0 &&
-       pages_of(len < 0 ? 0 : len, a.page) <= a.width;
-  if (!ok || len <= 0 || len % a.page == 0) return 0;
-  return (u32)a.table[from * a.table_row + len / a.page] < (u32)a.pages;
+  if ((u32)from >= (u32)a.rows || (u32)to >= (u32)a.rows) return {false, 0};
+  const int len = a.lens[from * a.lens_step], held = a.lens[to * a.lens_step];
+  const auto mark = [](const int32_t* p) {         // past this CU's cache: others' atomics wrote it
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  const bool ok = mark(&owner[to]) == i && mark(&source[to]) == 0 && held <= 0 &&
+                  pages_of(len < 0 ? 0 : len, a.page) <= a.width;
+  if (!ok || len <= 0 || len % a.page == 0) return {ok, 0};
+  return {ok, (u32)a.table[from * a.table_row + len / a.page] < (u32)a.pages};
 }
 
 extern "C" __global__ __launch_bounds__(WG) void ek_fork_plan(Params a) {
   __shared__ u32 s_wave[WG / 64];
-  int32_t *owner = a.work, *source = owner + a.rows, *ends = source + a.rows, *fresh = ends + a.n;
+  __shared__ int32_t s_marks[2 * SMALL];
+  int32_t* owner = a.rows <= SMALL ? s_marks : a.work;
+  int32_t *source = owner + a.rows, *ends = a.work + 2 * a.rows, *fresh = ends + a.n;
   int32_t* found = fresh + a.n;
+  const Counts counts = counts_at(a, threadIdx.x * EACH);
   for (int r = threadIdx.x; r < a.rows; r += WG) owner[r] = 0x7FFFFFFF, source[r] = 0;
-  __threadfence();
   __syncthreads();
   for (int i = threadIdx.x; i < a.n; i += WG) {
     const int from = a.first[i * a.first_step], to = a.second[i * a.second_step];
     if ((u32)to < (u32)a.rows) atomicMin(&owner[to], i);
     if ((u32)from < (u32)a.rows) atomicOr(&source[from], 1);
   }
-  __threadfence();
   __syncthreads();
-  int sum = 0;
+  Fork mine = {false, 0};                          // this thread's first, and where its share ends
+  int mine_end = 0, sum = 0;
   for (int i0 = 0; i0 < a.n; i0 += WG) {
     const int i = i0 + threadIdx.x;
-    bool ok;
-    const int need = i < a.n ? fork_need(a, i, ok) : 0;
+    const Fork f = i < a.n ? fork_of(a, i, owner, source) : Fork{false, 0};
     int64_t total;
-    const int end = sum + (int)scan_group(need, &total, s_wave) + need;
-    if (i < a.n) ends[i] = end;
+    const int end = sum + (int)scan_group(f.need, &total, s_wave) + f.need;
+    if (i0 == 0) mine = f, mine_end = end;
+    else if (i < a.n) ends[i] = end;
     sum += (int)total;
   }
   __syncthreads();
-  const int got = find_free(a, sum, found, s_wave);
+  const int got = find_free(a, sum, found, s_wave, counts);
   for (int i = threadIdx.x; i < a.n; i += WG) {
-    bool ok;
-    const int need = fork_need(a, i, ok);
-    ok = ok && (need == 0 || ends[i] <= got);
-    const int page = ok && need ? found[ends[i] - 1] : -1;
+    const Fork f = i < WG ? mine : fork_of(a, i, owner, source);
+    const int end = i < WG ? mine_end : ends[i];
+    const bool ok = f.ok && (f.need == 0 || end <= got);
+    const int page = ok && f.need ? found[end - 1] : -1;
     fresh[i] = page;
     if (page >= 0) a.refs[page] = 1;
     a.served[i] = ok;
@@ -333,8 +365,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_fork_copy(Params a) {
   const int whole = len < 0 ? 0 : len / a.page;
   const int32_t* old = a.table + from * a.table_row;
   if ((int)blockIdx.y < a.caches_used) {
-    if (fresh >= 0) copy_piece(a, a.caches[blockIdx.y], old[whole], fresh, len - whole * a.page,
-                               piece);
+    if (fresh >= 0) copy_piece<FORK>(a, a.caches[blockIdx.y], old[whole], fresh,
+                                     len - whole * a.page, piece);
     return;
   }
   int32_t* row = a.table + to * a.table_row;

@@ -127,11 +127,14 @@ class _Plan:
         """Launches the kernels for `objs` (in the order of the plan's arrays)."""
         if not self.on_gpu:
             return self._run_general(objs)
+        self.run_at([0 if x is None else x.data_ptr() for x in objs])
+
+    def run_at(self, ptrs: list) -> None:
+        """The same for arrays on a GPU by their addresses (0 where there is none)."""
         device = self.device
         if _cuda.here() != device:
             with _torch().cuda.device(device):
-                return self.run(objs)
-        ptrs = [0 if x is None else x.data_ptr() for x in objs]
+                return self.run_at(ptrs)
         if self.workspace:
             keep = _cuda.empty(self.workspace, dtype=_cuda.uint8, device=self.where)
             ptrs.append(keep.data_ptr())

@@ -265,8 +265,11 @@ def accept(logits, tokens, cu_tokens, *, tree=None, most: int | None = None):
     if plan is None:
         plan = _accept_plan(logits, tokens, cu_tokens, tree, most)
         _d._keep(key, plan)
-    new = [T.new_empty(cu_tokens, shape, np.int32)
-           for shape in ((plan.batch, plan.most), (plan.batch,), (plan.batch,))]
+    shapes = (plan.batch, plan.most), (plan.batch,), (plan.batch,)
+    if plan.on_gpu:
+        new = [cu_tokens.new_empty(shape) for shape in shapes]
+    else:
+        new = [T.new_empty(cu_tokens, shape, np.int32) for shape in shapes]
     if plan.launches:
         plan.run([logits, tokens, cu_tokens, tree, *new])
     return tuple(new)

@@ -37,7 +37,7 @@ __all__ = ["copy", "compact", "fork", "take", "free"]
 
 _PARAMS = struct.Struct("<8q10i")
 _FILE = "pages.hip"
-_THREADS, _UNROLL = 256, 4          # of a workgroup that copies: pages.hip
+_THREADS, _COPY, _FORK = 256, 1, 8  # of a workgroup that copies, and its accesses: pages.hip
 MAX_CACHES = 256                    # of a call: their addresses are kernel arguments
 MAX_PAGES = (1 << 25) - 1           # sums over a wave's rows stay in 32 bits
 MAX_BLOCKS = (1 << 24) - 1          # of 256 threads: a grid holds fewer than 2^32 threads
@@ -58,9 +58,11 @@ def _listed(caches) -> list:
     raise TypeError(f"`caches` must be arrays, got {type(caches).__name__}")
 
 
-def _key(caches: list):
+def _key(caches):
     """What a plan depends on of the caches; raises where they are none or differ (the checks of
     a new plan say how)."""
+    if not isinstance(caches, (list, tuple)):
+        return _d._of(caches)
     c = caches[0]
     dtype, shape, strides, device = _d._of(c)
     for x in caches:
@@ -90,13 +92,17 @@ def _check_caches(caches: list) -> _d._Array:
     return first
 
 
-def _check_apart(plan, caches: list) -> None:
-    """Refuses caches that share elements. Whether two do goes by their distance alone."""
-    if len(caches) < 2:
+def _check_apart(plan, at: list) -> None:
+    """Refuses caches that share elements, from their addresses. Whether two do goes by their distance
+    alone, so what was found for one is kept."""
+    span, last = plan.span, None
+    at = sorted(at)
+    for i, p in enumerate(at):
+        if last is not None and p - last < span:
+            break
+        last = p
+    else:
         return
-    at = sorted(_d._Array("caches", x).address() for x in caches) if not plan.on_gpu else \
-        sorted([x.data_ptr() for x in caches])
-    span = plan.span
     for i, p in enumerate(at):
         for q in at[i + 1:]:
             if q - p >= span:
@@ -167,8 +173,11 @@ def _pages_plan(launches, caches, arrays, written, workspace, numbers, access=16
         tail = bytes(8) + tail
     plan = _d._Plan(_FILE, (("EK_CACHES", slots), ("EK_V", access), ("EK_STREAM", int(stream))),
                     launches, named, set(range(len(caches))) | {slots + i for i in written},
-                    workspace, tail, [(slots + i, slots + j, False) for i, j in apart])
-    plan.pad = [None] * (slots - len(caches))
+                    workspace, tail)
+    # (written, bytes, other, bytes, their names), by their places among `arrays`
+    plan.pairs = [(i, arrays[i][1].span(), j, arrays[j][1].span(), (arrays[i][0], arrays[j][0]))
+                  for i, j in apart if arrays[i][1] and arrays[j][1]]
+    plan.pad = [0] * (slots - len(caches))
     plan.gaps = {}
     if caches:
         plan.span, plan.steps, plan.element = \
@@ -176,12 +185,37 @@ def _pages_plan(launches, caches, arrays, written, workspace, numbers, access=16
     return plan
 
 
-def _run(plan, caches: list, arrays: list) -> None:
-    objs = caches + plan.pad + arrays
-    _check_apart(plan, caches)
-    if plan.apart:
-        plan.check_apart(objs)
-    plan.run(objs)
+def _run(plan, caches, arrays: list) -> None:
+    """Launches the plan, unless arrays that it writes overlap others."""
+    if not plan.on_gpu:
+        caches = _listed(caches)
+        at = [_d._Array("caches", x).address() for x in caches]
+        rest = [0 if x is None else _d._Array("", x).address() for x in arrays]
+    else:
+        rest = [0 if x is None else x.data_ptr() for x in arrays]
+        if isinstance(caches, (list, tuple)):
+            at = [x.data_ptr() for x in caches]
+        elif len(caches.shape) == 4:
+            at = [caches.data_ptr()]
+        else:
+            first, step = caches.data_ptr(), caches.stride(0) * plan.element
+            at = [first + i * step for i in range(caches.shape[0])]
+    if len(at) > 1:
+        _check_apart(plan, at)
+    for i, n, j, m, names in plan.pairs:
+        if rest[i] < rest[j] + m and rest[j] < rest[i] + n:
+            _d._apart(names[0], _d._Array(names[0], arrays[i]), names[1],
+                      _d._Array(names[1], arrays[j]), False)
+    if plan.on_gpu:
+        plan.run_at(at + plan.pad + rest)
+    else:
+        plan.run(caches + [None] * len(plan.pad) + arrays)
+
+
+def _served(plan, like):
+    """A new int32 array of the shape of `like`, which is one."""
+    return like.new_empty(like.shape) if plan is not None and plan.on_gpu else \
+        T.new_empty(like, tuple(like.shape), np.int32)
 
 
 def _step(a) -> int:
@@ -200,7 +234,6 @@ def copy(caches, source, target) -> None:
         caches: the caches, written in place.
         source, target: int32 `[pairs]`.
     """
-    caches = _listed(caches)
     try:
         key = (3, *_key(caches), _d._of(source), _d._of(target))
         plan = _d._plans.get(key)
@@ -215,6 +248,7 @@ def copy(caches, source, target) -> None:
 
 
 def _copy_plan(caches, source, target):
+    caches = _listed(caches)
     c = _check_caches(caches)
     sa = _d._array("source", source, ("i32",), 1, dense=False)
     ta = _d._array("target", target, ("i32",), 1, sa.shape, dense=False)
@@ -226,7 +260,7 @@ def _copy_plan(caches, source, target):
     if n == 0 or heads * row == 0 or c.shape[0] == 0:
         return None
     v = _access(row)
-    pieces = -(-(c.shape[1] * heads * row // v) // (_THREADS * _UNROLL))
+    pieces = -(-(c.shape[1] * heads * row // v) // (_THREADS * _COPY))
     _d._need(n * pieces <= MAX_BLOCKS, f"{n} pages of {c.shape[1] * heads * row} bytes are too "
                                        "many for one call")
     moved = 2 * n * len(caches) * c.shape[1] * heads * row
@@ -258,7 +292,6 @@ def compact(caches, block_table, starts, keep, counts, *, seq_lens=None) -> None
         seq_lens: int32 `[rows]`, which becomes `starts[b] + counts[b]`; without it nothing is
             written but the caches.
     """
-    caches = _listed(caches)
     try:
         key = (4, *_key(caches), _d._of(block_table), _d._of(starts), _d._of(keep),
                _d._of(counts), None if seq_lens is None else _d._of(seq_lens))
@@ -274,6 +307,7 @@ def compact(caches, block_table, starts, keep, counts, *, seq_lens=None) -> None
 
 
 def _compact_plan(caches, block_table, starts, keep, counts, seq_lens):
+    caches = _listed(caches)
     c = _check_caches(caches)
     bt, sl = _table(block_table, seq_lens, c.shape[1], written=False)
     rows = bt.shape[0]
@@ -319,7 +353,6 @@ def fork(caches, refs, block_table, seq_lens, source, target):
     Returns:
         int32 `[forks]`: 1 where a fork was served, else 0.
     """
-    caches = _listed(caches)
     try:
         key = (5, *_key(caches), _d._of(refs), _d._of(block_table), _d._of(seq_lens),
                _d._of(source), _d._of(target))
@@ -330,13 +363,14 @@ def fork(caches, refs, block_table, seq_lens, source, target):
         plan = _fork_plan(caches, refs, block_table, seq_lens, source, target)
         if plan is not None:
             _d._keep(key, plan)
-    served = T.new_empty(source, tuple(source.shape), np.int32)
+    served = _served(plan, source)
     if plan is not None:
         _run(plan, caches, [refs, block_table, seq_lens, source, target, None, served])
     return served
 
 
 def _fork_plan(caches, refs, block_table, seq_lens, source, target):
+    caches = _listed(caches)
     c = _check_caches(caches)
     ra = _refs(refs, c.shape[0])
     bt, sl = _table(block_table, seq_lens, c.shape[1])
@@ -350,7 +384,7 @@ def _fork_plan(caches, refs, block_table, seq_lens, source, target):
         return None
     heads, row, *strides = _row_form(c)
     v = _access(row) if row else 1
-    pieces = max(1, -(-(c.shape[1] * heads * row // v) // (_THREADS * _UNROLL)))
+    pieces = max(1, -(-(c.shape[1] * heads * row // v) // (_THREADS * _FORK)))
     _d._need(n * pieces <= MAX_BLOCKS, f"{n} forks of pages of {c.shape[1] * heads * row} bytes "
                                        "are too many for one call")
     _d._need(rows <= 1 << 22, f"at most {1 << 22} rows are supported, got {rows}")
@@ -395,7 +429,7 @@ def take(refs, block_table, seq_lens, new_lens, *, page_size: int):
         plan = _rows_plan(refs, block_table, seq_lens, new_lens, page_size, True)
         if plan is not None:
             _d._keep(key, plan)
-    served = T.new_empty(seq_lens, tuple(seq_lens.shape), np.int32)
+    served = _served(plan, seq_lens)
     if plan is not None:
         _run(plan, [], [refs, block_table, seq_lens, new_lens, None, None, served])
     return served

@@ -217,11 +217,11 @@ def test_caches_that_share_elements():
         plan = pages._pages_plan([], [decode._Array("c", x) for x in bad], [], set(), 0,
                                  (0,) * 18)
         with pytest.raises(ValueError, match="share elements"):
-            pages._check_apart(plan, bad)
+            pages._check_apart(plan, [x.data_ptr() for x in bad])
     for good in (apart, [a[:, 0, :, :, :32], a[:, 0, :, :, 32:]], [rows[:5], rows[5:10]]):
         plan = pages._pages_plan([], [decode._Array("c", x) for x in good], [], set(), 0,
                                  (0,) * 18)
-        pages._check_apart(plan, good)
+        pages._check_apart(plan, [x.data_ptr() for x in good])
     if not torch.cuda.is_available():
         with pytest.raises(ValueError, match="share elements"):
             pages.copy([a[:, 0], a[:, 0]], i32(1), i32(1))

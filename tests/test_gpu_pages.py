@@ -290,7 +290,7 @@ def test_fork_of_a_last_page_that_is_not_in_the_cache():
         assert r.tolist() == [2, 0, 0] and t[1].tolist() == [0, wild] and m.tolist() == [20, 20]
 
 
-@pytest.mark.parametrize("forks", [1, 1024, 1500])
+@pytest.mark.parametrize("forks", [1, 1024, 1500, 5000])
 def test_fork_of_many(forks):
     gen = torch.Generator().manual_seed(forks)
     lens = torch.randint(0, 60, (50,), generator=gen).tolist()
