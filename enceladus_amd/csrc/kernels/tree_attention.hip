@@ -10,16 +10,19 @@
 // The (token, query head) pairs of a key head are the columns of every product: rows * heads per
 // key head of them share each key and value. Few columns take the cache's bytes over the HBM rate;
 // many take the products and, as long, the VALU's softmax. So each key and value is read once for
-// all columns of a workgroup: its waves copy KT keys at a time into the LDS, straight from memory and
-// a stage ahead, and WC of them take CT tiles of 16 columns each. Where that leaves waves without
-// columns, WK waves share the columns and split a stage's keys; they join in the LDS at the end.
+// all columns of a workgroup: its waves copy KT keys at a time into the LDS, straight from memory
+// and a stage ahead, and WC of them take CT tiles of TILE columns each. Where that leaves waves
+// without columns, WK waves share the columns and split a stage's keys; they join in the LDS at the
+// end. Tiles are 32 columns wide where there are as many: an instruction holds up the VALU as long
+// as one of 16 does and multiplies twice as much.
 //
-// Layout (16x16 MFMA, lane l, r = l % 16, c = l / 16):
-// - S^T = K Q^T: lane l reads a chunk of key r; its accumulator holds keys 4 c + i of column r.
-// - O^T = V^T P^T: the product over 32 keys gives lane l's slot j the key 4 c + j (j < 4) of the
-//   first and of the second 16 keys, so that P is where S left it. 16-bit values come transposed
-//   out of the LDS (tr_read4: 4 keys of one element); of others lane l reads VE consecutive elements
-//   of those keys from element VE r on, and the m-th product takes element VE r + m of them.
+// Layout (lane l, r = l % TILE, c = l / TILE; runs of four keys, one for 16 columns, four for 32):
+// - S^T = K Q^T: lane l reads a chunk of key r; its accumulator holds the runs' keys 4 c + i (32
+//   columns: 8 s + 4 c + i) of column r.
+// - O^T = V^T P^T: the product over two runs gives lane l's slots the keys of its own first and its
+//   own second run, so that P is where S left it. 16-bit values come transposed out of the LDS
+//   (tr_read4: 4 keys of one element); of others lane l reads VE consecutive elements of those keys
+//   from element VE r on, and the m-th product takes element VE r + m of them.
 // - A weight is two terms of the values' 16-bit type, a product each: 2^-17 of it is left out in
 //   bf16 and 2^-22 in fp16 and e4m3 (whose values are exact in fp16). One term would be half a
 //   step of the output's own type off in every weight, as much again as its rounding.
@@ -27,10 +30,17 @@
 //   pass (256 bytes) meet in a bank: chunk x of key k is at x ^ k_swap(k) or x ^ v_swap(k). The
 //   copy does it for nothing: each lane picks the chunk that belongs at its place.
 //
-// Work: the (chunk, block of WC CT 16 columns) pairs of all sequences are items, a workgroup each, of
+// Work: the (chunk, block of COLS columns) pairs of all sequences are items, a workgroup each, of
 // one key head. The chunks' length comes from all sequences' lengths and rows, on the device.
 // Sequences of one chunk are finished here; the others leave (O, m, l) per chunk and column to the
 // second kernel.
+//
+// 128 columns over 131075 fp16 keys of 8 heads (537 MB, 103 GFLOP of products): 143 us and 11 to
+// join, 3.8 TB/s. The copies alone take 100 us, the rest without them 101 (softmax and products
+// in turn, each about half): one covers the other only in part. Some 25 columns of each of 24
+// sequences of up to 16384 8-bit keys (156 MB): 78 us. A tree of 16 tokens after 1983 (8.4 MB, one
+// stage for each workgroup): 14 us, of which 6 are the way to the first key (lengths, pages, keys:
+// three reads, each waiting for the one before).
 //
 // Macros: EK_Q (0 fp32, 1 fp16, 2 bf16), EK_FP8 (the cache is e4m3), EK_DP (64, 128 or 256: the
 // head dimension it is compiled for), EK_PAD (the head dimension is smaller), EK_KT (keys of a
@@ -78,7 +88,7 @@ constexpr bool HALF = EK_Q == 1 || EK_FP8;          // the weights' terms are fp
 constexpr int TERMS = 2;
 constexpr float LIFT = HALF ? 14.0f : 0.0f;        // log2, in the exponents: l is lifted too
 
-#define EK_HERE __attribute__((always_inline))      // of a lambda: what it captures stays in registers
+#define EK_HERE __attribute__((always_inline))      // of a lambda: its captures stay in registers
 
 typedef uint32_t u32;
 typedef float Acc __attribute__((ext_vector_type(RA * 4)));    // of a tile
@@ -111,7 +121,7 @@ struct Params {
   int64_t table_row, lens_step, cu_step, tree_row;      // elements
   int32_t tokens, batch, heads, kv_heads, group, dim, page, pages, capacity, window, words;
   uint32_t page_mul;
-  int32_t page_shift, items, slots, min_units, join;
+  int32_t page_shift, items, rounds, slots, join;
   uint32_t q_sign;                   // the sign bits of the queries' words, if scale is negative
   float scale, cap, v_scale;         // scale > 0, with log2(e); cap in the same unit, or 0
 };
@@ -176,9 +186,10 @@ struct Item {
 };
 
 // The items of all sequences in their order are 0, 1, ...: a chunk has as many units of UNIT keys
-// as give `items` of them in all, and at most one more for each block of columns. Slots are
-// counted over the sequences with several chunks alone, of which there are at most 2 `items`.
-// Every wave finds its own from lengths and rows, 64 sequences at a time, a lane each.
+// as give `items` of them in all, and at most one more for each block of columns; or some more, so
+// that there are at most `items`, or twice as many. Slots are counted over the sequences with
+// several chunks alone, of which there are at most 2 `items`. Every wave finds its
+// own from lengths and rows, 64 sequences at a time, a lane each.
 EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
   const int lane = ek::lane_id();
   const Seq s0 = seq_of(a, lane);
@@ -189,18 +200,30 @@ EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
   }
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
   int per = (int)((u32)(total + a.items - 1) / (u32)a.items);
-  per = per < a.min_units ? a.min_units : per;
-  // Each sequence may have a chunk more than its share for each of its blocks. If chunks of up to
-  // half as many units again fit all of them into `items`, that saves a last round of few waves.
+  per = per < 1 ? 1 : per;
+  // Each sequence may have a chunk more than its share for each of its blocks, and a few workgroups
+  // beyond `items` make a round of their own. So the chunks are made as long as it takes for all of
+  // them to fit into one round, or two where the grid has them, whichever ends first if a chunk
+  // costs 3 units besides its own (24 sequences of up to 16384 8-bit keys: 78 us, 82 in even
+  // shares; 64 of up to 8192: 194 us in even shares, 178 in two rounds). Chunks of less than 8
+  // units are not worth two rounds (55 sequences of at most 189 keys: 67 us without, 74 with).
   if (a.batch <= 64) {
-    int try_per = per;
+    int best = 1 << 30;
 #pragma unroll 1
-    for (int k = 0; k < 4; ++k) {
-      const int all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(
-          blocks_of(a, s0) * chunks_of(units_of(s0), try_per)));
-      if (all <= a.items) per = try_per;
-      if (all <= a.items || all > a.items + a.items / 2) break;
-      try_per += (try_per + 7) >> 3;
+    for (int rounds = 1; rounds <= a.rounds; ++rounds) {
+      const int room = rounds * a.items;
+      int try_per = (int)((u32)(total + room - 1) / (u32)room);
+      if (rounds > 1 && try_per < 8) break;
+      try_per = try_per < 1 ? 1 : try_per;
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k) {
+        const int all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(
+            blocks_of(a, s0) * chunks_of(units_of(s0), try_per)));
+        const int cost = rounds * (try_per + 3);
+        if (cost >= best) break;
+        if (all <= room) { best = cost, per = try_per; break; }
+        try_per += (try_per + 15) >> 4;
+      }
     }
   }
   // without room for parts each has one chunk, as when rows enough for all items are there
@@ -402,7 +425,8 @@ EK_INLINE int tree_count(const Params& a, const u32* row, int lo, int hi) {
 
 EK_INLINE T result(float o, float f, bool any) { return ek::cvt<T>(any ? o * f : 0.0f); }
 
-// What differences of the running maxima are multiplied by for exp2: capped scores are in log2 units.
+// What differences of the running maxima are multiplied by for exp2: capped scores are in log2
+// units.
 EK_INLINE float scale_of(const Params& a) { return a.cap > 0.0f ? 1.0f : a.scale; }
 
 extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(Params a) {
@@ -427,6 +451,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     head[t] = g * a.group + x - index[t] * a.group;
   }
 #define valid(t) (col0 + (t) * TILE + r < all)
+#define tree_of(t) (a.tree + (sq.begin + index[t]) * a.tree_row)
   if (a.part && it.chunk == 0 && g == 0 && wk == 0 && c == 0) {
     // for the second kernel, by the column of each token's first head
 #pragma unroll
@@ -447,11 +472,16 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   uint64_t bits[CT];                                  // a tree's row's first 64
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    bits[t] = a.tree ? (a.tree + (sq.begin + index[t]) * a.tree_row)[0] | (a.words > 1 ? (uint64_t)(a.tree + (sq.begin + index[t]) * a.tree_row)[1] << 32 : 0) : 0;
+    bits[t] = 0;
+    if (a.tree) {
+      bits[t] = tree_of(t)[0];
+      if (a.words > 1) bits[t] |= (uint64_t)tree_of(t)[1] << 32;
+    }
     from[t] = 0;
     if (a.window > 0) {
       int seen = index[t] + 1;
-      if (a.tree) seen = tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
+      if (a.tree)
+        seen = tree_count(a, tree_of(t), sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
       from[t] = sq.past + seen - a.window;
       deep |= a.tree && seen > a.window;
     }
@@ -482,8 +512,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   const u32 lds = ek::lds_addr(s_stage);
   const int row_bytes = a.dim * CS;
 
-  // The page of key base + lane of a stage (`ids` of two stages in turn): copied into the LDS a stage
-  // before its keys are, by every wave for itself. There is one at every address read here.
+  // The page of key base + lane of a stage (`ids` of two stages in turn): copied into the LDS a
+  // stage before its keys are, by every wave for itself. There is one at every address read here.
   const auto fetch_ids = [&](int ids, int base) EK_HERE {
     const int key = base + (lane & (KT - 1)), last = hi - 1;
     copy4(ek::lds_addr(s_ids[wave][ids]), table + page_of(a, key < last ? key : last));
@@ -496,7 +526,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     return ok ? id * a.c_page + (key - page_of(a, key) * a.page) * a.c_token : -1;
   };
   // A stage's keys or values on their way: zeros where there is no key, or no element of it.
-  const auto fetch = [&](int to, const char* from, const auto& swap, int64_t off, bool full) EK_HERE {
+  const auto fetch = [&](int to, const char* from, const auto& swap, int64_t off,
+                         bool full) EK_HERE {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int first = (k * W + wave) * 64, key = (first + lane) / CPR;
@@ -658,11 +689,12 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
           u32 run = (u32)(live >> at) & 15u;
           if (masks) {
             if (a.tree) {
-              run &= tree_bits(a, (a.tree + (sq.begin + index[t]) * a.tree_row), bits[t], j);
+              run &= tree_bits(a, tree_of(t), bits[t], j);
               if (deep) {
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i)
-                  if (j + i >= 0 && tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), j + i, sq.end - sq.past) > a.window)
+                  if (j + i >= 0 &&
+                      tree_count(a, tree_of(t), j + i, sq.end - sq.past) > a.window)
                     run &= ~(1u << i);
               }
             } else {
@@ -858,7 +890,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     __syncthreads();
   }
 
-  // The same stages' keys once more, one at a time: the elements of their values that are not finite.
+  // The same stages' keys once more, one at a time: the elements of their values that are not
+  // finite.
   if (some_odd) {
 #pragma unroll 1
     for (int key = lo; key < hi; ++key) {
@@ -870,9 +903,9 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
       for (int t = 0; t < CT; ++t) {
         bool sees = key >= from[t] && j <= index[t];
         if (a.tree) {
-          sees = j < 0 ? key >= from[t] : tree_bits(a, (a.tree + (sq.begin + index[t]) * a.tree_row), bits[t], j) & 1;
+          sees = j < 0 ? key >= from[t] : tree_bits(a, tree_of(t), bits[t], j) & 1;
           if (deep && j >= 0)
-            sees = sees && tree_count(a, (a.tree + (sq.begin + index[t]) * a.tree_row), j, sq.end - sq.past) <= a.window;
+            sees = sees && tree_count(a, tree_of(t), j, sq.end - sq.past) <= a.window;
         }
 #pragma unroll
         for (int p = 0; p < NP; ++p)
@@ -881,7 +914,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
             const int d = element_of(p, i);
             const float x = element(v + (d < a.dim ? d : 0) * CS);
             // 0x207: a NaN or an infinity
-            o[t][p][i] = sees && __builtin_amdgcn_classf(x, 0x207) ? __builtin_nanf("") : o[t][p][i];
+            if (sees && __builtin_amdgcn_classf(x, 0x207)) o[t][p][i] = __builtin_nanf("");
           }
       }
     }
@@ -904,8 +937,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
         for (int p = 0; p < NP; ++p)
 #pragma unroll
           for (int k = 0; k < RA; ++k)
-            *(ek::f32x4*)(mine + ((t * NP + p) * RA + k) * 256) =
-                ek::f32x4{o[t][p][k * 4], o[t][p][k * 4 + 1], o[t][p][k * 4 + 2], o[t][p][k * 4 + 3]};
+            *(ek::f32x4*)(mine + ((t * NP + p) * RA + k) * 256) = ek::f32x4{
+                o[t][p][k * 4], o[t][p][k * 4 + 1], o[t][p][k * 4 + 2], o[t][p][k * 4 + 3]};
         mine[ML + t * 128 - lane * 3] = m[t];
         mine[ML + t * 128 + 64 - lane * 3] = l[t];
       }
@@ -997,6 +1030,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
   }
 }
 #undef valid
+#undef tree_of
 
 // Joins the chunks of a token's head: `join` waves (1 or 4) take 16 of them in turn, all of their
 // loads on their way at once, and meet in the LDS.
@@ -1008,10 +1042,12 @@ extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params 
   const int head = waves == 1 ? blockIdx.y * 4 + wave : blockIdx.y, first = waves == 1 ? 0 : wave;
   if (head >= a.heads || token < a.cu[0] || token >= a.cu[a.batch * a.cu_step]) return;
   const Row row = part_rows(a)[token];
+  // rows that descend may have left this unwritten
   if (row.chunks <= 1 || row.slot < 0 || row.blocks <= 0 || row.index < 0 ||
       row.slot + (int64_t)row.chunks * row.blocks > a.slots)
     return;
-  const int g = head / a.group, col = row.index * a.group + head - g * a.group;
+  const int g = head / a.group;
+  const u32 col = (u32)row.index * a.group + (head - g * a.group);
   const int block = col / COLS;
   if (block >= row.blocks) return;
   const float scale = scale_of(a);

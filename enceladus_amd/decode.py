@@ -994,6 +994,10 @@ def specializations():
             for stream in (0, 1):
                 yield "append_kv.hip", (("EK_Q", q), ("EK_FP8", fp8), ("EK_V", 8 if q else 4),
                                         ("EK_PAIRS", pairs), ("EK_STREAM", stream))
+                for axes in (1, 2):
+                    yield "append_kv.hip", (("EK_Q", q), ("EK_FP8", fp8),
+                                            ("EK_V", 8 if q else 4), ("EK_PAIRS", pairs),
+                                            ("EK_STREAM", stream), ("EK_AXES", axes))
     for q in (0, 1, 2):
         for n, stream in ((4096, 0), (8192, 0), (8192, 1)):
             yield "adjust_logits.hip", (("EK_Q", q), ("EK_N", n), ("EK_STREAM", stream))

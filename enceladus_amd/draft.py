@@ -52,8 +52,6 @@ def _tree(tree, tokens: int):
 
 _ATTEND = struct.Struct("<11q11iI5iI3f4x")
 _UNIT = 64                          # tokens: what a sequence is split in multiples of
-_MIN_UNITS = 1                      # of a chunk
-_GROUPS = 2                         # workgroups per CU
 
 
 def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tree=None,
@@ -123,20 +121,31 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
     return (out, lse) if return_lse else out
 
 
-def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, int]:
-    """(keys of a stage, columns of a tile, tiles of a wave, waves over columns, waves over keys) for
-    sequences of so many columns of a key head, in heads of `width` cached elements of `size`
-    bytes."""
+def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, int, int]:
+    """(keys of a stage, columns of a tile, tiles of a wave, waves over columns, waves over keys,
+    workgroups of a CU) for sequences of so many columns of a key head, in heads of `width` cached
+    elements of `size` bytes."""
     keys = max(16, min(64, 16384 // (width * size)))
     if size == 4 or width == 256:
         over = 1
         while over < 4 and (columns > 16 * over or keys < 64 // over):
             over *= 2
-        return keys, 16, 1, over, 4 // over
+        return keys, 16, 1, over, 4 // over, 1 if width * size == 1024 else 2
     if columns <= 32:
-        return (keys, 16, 1, 1, 4) if columns <= 16 else (keys, 16, 1, 2, 2)
+        # 94 to 113 registers at 64 elements; 129 to 152 at 128, of which only the 8-bit ones' stages
+        # leave the LDS to a third workgroup
+        at_once = 4 if width == 64 else 3 if size == 1 else 2
+        return (keys, 16, 1, 1, 4, at_once) if columns <= 16 else (keys, 16, 1, 2, 2, at_once)
     over = 2 if columns <= 64 else 4
-    return (keys, 16, 2, over, 4 // over) if width * size == 64 else (keys, 32, 1, over, 4 // over)
+    at_once = 3 if width == 64 and (size == 2 or over == 2) else 2
+    return (keys, 16, 2, over, 4 // over, at_once) if width * size == 64 else \
+        (keys, 32, 1, over, 4 // over, at_once)
+
+
+def _macros(q: int, fp8: bool, width: int, pad: bool, shape) -> tuple:
+    names = ("EK_Q", "EK_FP8", "EK_DP", "EK_PAD", "EK_KT", "EK_TILE", "EK_CT", "EK_WC", "EK_WK",
+             "EK_OCC")
+    return tuple(zip(names, (q, int(fp8), width, int(pad), *shape)))
 
 
 def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree, scale, window,
@@ -182,28 +191,32 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
         capacity = 0
     window = min(window, _d.MAX_TOKENS)
     width = 64 if dim <= 64 else 128 if dim <= 128 else 256
-    keys, tile, tiles, over, split = _shape(tokens / batch * group, width, kc.size)
+    shape = _shape(tokens / batch * group, width, kc.size)
+    _, tile, tiles, over, split, at_once = shape
     cols = tile * tiles * over
     waves = over * split
     # blocks of columns: each sequence may have one that is not whole
     blocks = -(-tokens * group // cols) if batch == 1 else tokens * group // cols + \
         min(batch, tokens)
     most = -(-capacity // _UNIT)
+    if window:
+        most = min(most, -(-(window + tokens) // _UNIT))
     need(blocks * max(most, 1) < 1 << 31, f"{tokens} tokens over tables of {capacity} tokens are "
                                           "too many for one call")
-    items = max(1, _GROUPS * C.coarsen_cap() // kv_heads)
-    x = items + blocks
+    items = max(1, at_once * C.coarsen_cap() // kv_heads)
+    # A chunk for every block besides their even shares, and no more than there are units. Room for
+    # two rounds of them is there if the blocks are as many as fit at once (workgroups that find
+    # nothing to do cost 1 us and more: there are none for its sake).
+    x = min(items + blocks, blocks * max(most, 1))
+    rounds = 2 if x >= 2 * items else 1
     need(x * 64 * waves < 1 << 32 and kv_heads <= 65535, f"{tokens} tokens are too many for one "
                                                          "call")
-    macros = (("EK_Q", _d._Q[qa.kind]), ("EK_FP8", int(kc.kind == "fp8")), ("EK_DP", width),
-              ("EK_PAD", int(dim != width)), ("EK_KT", keys), ("EK_TILE", tile),
-              ("EK_CT", tiles), ("EK_WC", over), ("EK_WK", split),
-              ("EK_OCC", 1 if width * kc.size == 1024 else 2))
+    macros = _macros(_d._Q[qa.kind], kc.kind == "fp8", width, dim != width, shape)
     launches = [("ek_tree_attention", (x, kv_heads), 64 * waves)]
     slots = workspace = 0
     join = 1
     # one sequence of as many blocks as there are items has one chunk
-    if most > _MIN_UNITS and not (batch == 1 and blocks >= items):
+    if most > 1 and not (batch == 1 and blocks >= items):
         slots = 2 * items
         workspace = slots * kv_heads * cols * (dim + 2) * 4 + 16 * tokens
         # several waves where a token's head may have many chunks
@@ -216,7 +229,7 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
         *(s * kc.size for s in kc.strides[:3]), bt.strides[0], sl.strides[0], cu.strides[0],
         ta.strides[0] if ta else 0, tokens, batch, heads, kv_heads, group, dim, kc.shape[1],
         kc.shape[0], capacity, window, ta.shape[1] if ta else 0, *_d._page_division(kc.shape[1]),
-        items, slots, _MIN_UNITS, join,
+        items, rounds, slots, join,
         0 if scale >= 0 else 0x80000000 if qa.kind == "fp32" else 0x80008000,
         # so small a scale is as good as none, and keeps -inf (no key there) what it is
         max(abs(scale) * k_scale * log2e, 2.0 ** -126), softcap * log2e, v_scale)
@@ -318,5 +331,11 @@ def _accept_plan(logits, tokens, cu_tokens, tree, most):
 
 def specializations():
     """(source, macros) of the kernels that are worth compiling ahead."""
+    for q, fp8 in ((2, False), (1, False), (0, False), (2, True), (1, True)):
+        size = 1 if fp8 else 2 if q else 4
+        for width in (64, 128, 256):
+            for shape in sorted({_shape(columns, width, size) for columns in (16, 32, 64, 128)}):
+                for pad in (False, True) if size == 2 else (False,):
+                    yield "tree_attention.hip", _macros(q, fp8, width, pad, shape)
     for q in (0, 1, 2):
         yield "accept.hip", (("EK_Q", q),)
