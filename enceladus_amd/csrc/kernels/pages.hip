@@ -124,7 +124,8 @@ extern "C" __global__ __launch_bounds__(64) void ek_compact(Params a) {
       const int k = keep[i0 + lane];
       const int64_t old = (int64_t)start + k, now = (int64_t)start + i0 + lane;
       if (k > i0 + lane && old < capacity) {
-        const int po = (int)(old / a.page), pn = (int)(now / a.page);
+        // now < old: both fit 32 bits, like the capacity
+        const int po = (int)((u32)old / (u32)a.page), pn = (int)((u32)now / (u32)a.page);
         const int ido = row[po], idn = row[pn];
         if ((u32)ido < (u32)a.pages && (u32)idn < (u32)a.pages) {
           from = ido * a.c_page + (old - (int64_t)po * a.page) * a.c_token;
