@@ -137,6 +137,15 @@ EK_INLINE Row* part_rows(const Params& a) {
   return (Row*)(part_ml(a) + (int64_t)a.slots * a.kv_heads * COLS * 2);
 }
 
+EK_INLINE float lane_value(float x, int lane) {
+  return ek::bits_f32((u32)__builtin_amdgcn_readlane((int)ek::f32_bits(x), lane));
+}
+EK_INLINE int64_t lane_value(int64_t x, int lane) {
+  const u32 lo = (u32)__builtin_amdgcn_readlane((int)(u32)(uint64_t)x, lane);
+  return (int64_t)((uint64_t)(u32)__builtin_amdgcn_readlane((int)((uint64_t)x >> 32), lane) << 32 |
+                   lo);
+}
+
 EK_INLINE int page_of(const Params& a, int key) {
   return a.page == 1 ? key : (int)(__umulhi((u32)key, a.page_mul) >> a.page_shift);
 }
@@ -661,6 +670,7 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     // softmax: scores and m stay as the product gave them (or capped, in log2 units) until exp2
     const bool full = live == ~0ull;
     const bool masks = edge(base);
+    float less[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       if (a.cap > 0.0f) {
@@ -731,28 +741,27 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #pragma unroll
         for (int p = 0; p < NP; ++p) o[t][p] *= alpha;
       }
-      // exp2(scale (s - m)): in one step where scale m has digits to spare next to 2^-17, which a
-      // weight's terms leave out, else the difference first
+      // The weights are exp2(scale (s - m)): in one step where scale m has digits to spare next to
+      // 2^-17, which a weight's terms leave out, else the difference first.
       const float top = m_use * scale;
-      if (__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(top) < 256.0f)) == 0) {
-        const float less = LIFT - top;
+      less[t] = LIFT - top;
+      if (__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(top) < 256.0f)) != 0) {
+        less[t] = LIFT;
 #pragma unroll
         for (int s = 0; s < RUNS; ++s)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i), scale, less));
-      } else {
-#pragma unroll
-        for (int s = 0; s < RUNS; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i) - m_use, scale, LIFT));
+          for (int i = 0; i < 4; ++i) score(t, s, i) -= m_use;
       }
-#pragma unroll
-      for (int s = 0; s < RUNS; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[t] += score(t, s, i);
     }
+    const auto weigh = [&](int s) EK_HERE {
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          score(t, s, i) = ek::exp2_fast(__builtin_fmaf(score(t, s, i), scale, less[t]));
+          l[t] += score(t, s, i);
+        }
+    };
 
     if (next < hi) wait_for<2 * LOADS + 1>();
     else wait_for<0>();
@@ -792,6 +801,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     };
     read_values(0);
 #pragma unroll
+    for (int s = 0; s < RUNS; ++s) weigh(s);
+#pragma unroll
     for (int k = 0; k < STEPS; ++k) {
       if (k + 1 < STEPS) read_values(k + 1);
       __builtin_amdgcn_sched_barrier(0);              // the reads before what they hide behind
@@ -807,14 +818,28 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     constexpr int SS = RUNS == 1 ? 1 : 2;             // runs of a product
     constexpr int GROUP = !TR ? VE : NP < 4 ? NP : 4; // output tiles of a step
     constexpr int PER = NP / GROUP, STEPS = RUNS / SS * PER;
-    u32 w_p[CT][TERMS][2 * SS];
-    const auto products = [&](int p, const auto* w) EK_HERE {
+    // The weights of a step's runs are made between the products of the step before: the VALU has
+    // work while an instruction multiplies.
+    u32 w_p[2][CT][TERMS][2 * SS];
+    const auto weights = [&](int k) EK_HERE {
 #pragma unroll
-      for (int k = 0; k < TERMS; ++k)
+      for (int s = 0; s < SS; ++s) weigh(k * SS + s);
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2 * SS; ++i) {
+          const int s = k * SS + i / 2, x = i % 2 * 2;
+          split(score(t, s, x), score(t, s, x + 1), w_p[k & 1][t][0][i], w_p[k & 1][t][1][i]);
+        }
+    };
+    const auto products = [&](int k, int p, const auto* w) EK_HERE {
+#pragma unroll
+      for (int x = 0; x < TERMS; ++x)
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-          if constexpr (SS * sizeof(*w) == 4) mma_short<HALF>(o[t][p], w, w_p[t][k]);
-          else mma<HALF>(o[t][p], w, w_p[t][k]);
+          const auto* y = w_p[k / PER & 1][t][x];
+          if constexpr (SS * sizeof(*w) == 4) mma_short<HALF>(o[t][p], w, y);
+          else mma<HALF>(o[t][p], w, y);
         }
     };
 #if EK_FP8
@@ -846,19 +871,11 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     };
 #endif
     read_values(0);
+    weights(0);
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
       if (k + 1 < STEPS) read_values(k + 1);
       __builtin_amdgcn_sched_barrier(0);              // the reads before what they hide behind
-      if (k % PER == 0) {
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int i = 0; i < 2 * SS; ++i) {
-            const int s = k / PER * SS + i / 2, x = i % 2 * 2;
-            split(score(t, s, x), score(t, s, x + 1), w_p[t][0][i], w_p[t][1][i]);
-          }
-      }
       const int p0 = k % PER * GROUP;
 #if EK_FP8
       // 4 SS keys' VE elements, 16 bits each
@@ -875,12 +892,21 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
         for (int i = 0; i < 2 * SS; ++i)
           w[i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2],
                                        e & 1 ? 0x07060302u : 0x05040100u);
-        products(p0 + e, w);
+        products(k, p0 + e, w);
       }
 #else
 #pragma unroll
-      for (int x = 0; x < GROUP; ++x) products(p0 + x, vf[k & 1][x]);
+      for (int x = 0; x < GROUP; ++x) products(k, p0 + x, vf[k & 1][x]);
 #endif
+      if ((k + 1) % PER == 0 && k + 1 < STEPS) {
+        weights((k + 1) / PER);
+        // of the step's products and what makes the next weights, in turn
+#pragma unroll
+        for (int x = 0; x < GROUP * TERMS * CT; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x402, (6), 0);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
 #endif
@@ -1032,116 +1058,150 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #undef valid
 #undef tree_of
 
-// Joins the chunks of a token's head: `join` waves (1 or 4) take 16 of them in turn, all of their
-// loads on their way at once, and meet in the LDS.
-extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params a) {
-  constexpr int DW = (DP + 127) / 128, BATCH = 16;
-  __shared__ float s_o[4][DP], s_m[4], s_l[4];
-  const int lane = ek::lane_id(), token = blockIdx.x, waves = a.join;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = waves == 1 ? blockIdx.y * 4 + wave : blockIdx.y, first = waves == 1 ? 0 : wave;
-  if (head >= a.heads || token < a.cu[0] || token >= a.cu[a.batch * a.cu_step]) return;
+// Joins the chunks of H heads of a token in a wave, CHUNKS of each at once: lanes H' CHUNKS + i have
+// head H' and chunk i, and all of their loads are on their way together. With `join` 1 or 4, H is
+// as much: 4 where chunks are few, since a wave takes as long for one head as for four (64
+// sequences of 27 tokens and less, 32 heads, 2 or 3 chunks: 20 us with 1, 12 with 4). Where
+// chunks are many (`join` 0), a workgroup's four waves take one head's in turn and meet in the LDS.
+template <int H> EK_INLINE void join_heads(const Params& a, int token, int head0, int first,
+                                           int waves) {
+  constexpr int DW = (DP + 127) / 128, CHUNKS = 16 / H;
+  __shared__ float s_o[4][H == 1 ? DP : 1], s_m[4], s_l[4];
+  const int lane = ek::lane_id(), i = lane % CHUNKS, mine = head0 + lane / CHUNKS % H;
+  if (head0 >= a.heads || token < a.cu[0] || token >= a.cu[a.batch * a.cu_step]) return;
   const Row row = part_rows(a)[token];
   // rows that descend may have left this unwritten
   if (row.chunks <= 1 || row.slot < 0 || row.blocks <= 0 || row.index < 0 ||
       row.slot + (int64_t)row.chunks * row.blocks > a.slots)
     return;
-  const int g = head / a.group;
+  const int head = mine < a.heads ? mine : a.heads - 1, g = head / a.group;
   const u32 col = (u32)row.index * a.group + (head - g * a.group);
   const int block = col / COLS;
-  if (block >= row.blocks) return;
+  if (__builtin_amdgcn_ballot_w64(block >= row.blocks) != 0) return;
   const float scale = scale_of(a);
   const int64_t at = ((int64_t)(row.slot + block) * a.kv_heads + g) * COLS + col - block * COLS;
   const int64_t step = (int64_t)row.blocks * a.kv_heads * COLS;    // from chunk to chunk
-  float m = -__builtin_inff(), l = 0.0f, x[DW][2];
+  float m = -__builtin_inff(), l = 0.0f, x[H][DW][2];
+  int64_t from[H];
 #pragma unroll
-  for (int k = 0; k < DW; ++k) x[k][0] = x[k][1] = 0.0f;
+  for (int h = 0; h < H; ++h) {
+    from[h] = lane_value(at, h * CHUNKS);
+#pragma unroll
+    for (int k = 0; k < DW; ++k) x[h][k][0] = x[h][k][1] = 0.0f;
+  }
 #pragma unroll 1
-  for (int i0 = first * BATCH; i0 < row.chunks; i0 += waves * BATCH) {
-    const int count = row.chunks - i0 < BATCH ? row.chunks - i0 : BATCH, i = lane & (BATCH - 1);
+  for (int i0 = first * CHUNKS; i0 < row.chunks; i0 += waves * CHUNKS) {
+    const int count = row.chunks - i0 < CHUNKS ? row.chunks - i0 : CHUNKS;
     const float* ml = part_ml(a) + (at + (i0 + (i < count ? i : 0)) * step) * 2;
-    float mi = ml[0], li = ml[1], v[BATCH][DW][2];
+    float mi = ml[0], li = ml[1], v[H][CHUNKS][DW][2];
 #pragma unroll
-    for (int j0 = 0; j0 < BATCH; j0 += 4)
+    for (int j0 = 0; j0 < CHUNKS; j0 += 4)
       if (j0 < count) {
 #pragma unroll
-        for (int j = j0; j < j0 + 4; ++j) {
-          const float* src = a.part + (at + (i0 + (j < count ? j : 0)) * step) * a.dim;
+        for (int j = j0; j < j0 + 4; ++j)
 #pragma unroll
-          for (int k = 0; k < DW; ++k) {
-            const int d = k * 128 + lane * 2;
-            ek::vload_u<float, 2>(v[j][k], src + (d < a.dim ? d : 0));
+          for (int h = 0; h < H; ++h) {
+            const float* src = a.part + (from[h] + (i0 + (j < count ? j : 0)) * step) * a.dim;
+#pragma unroll
+            for (int k = 0; k < DW; ++k) {
+              const int d = k * 128 + lane * 2;
+              ek::vload_u<float, 2>(v[h][j][k], src + (d < a.dim ? d : 0));
+            }
           }
-        }
       }
     __builtin_amdgcn_sched_barrier(0);               // all of them before the first wait
     mi = i < count ? mi : -__builtin_inff();
     li = i < count ? li : 0.0f;
-    // lanes that differ in their upper bits have the same chunks
+    // over the lanes of a head's chunks
     float top = ek::reduce_xor<ek::Max, 1>(mi);
     top = ek::reduce_xor<ek::Max, 2>(top);
-    top = ek::reduce_xor<ek::Max, 4>(top);
-    top = __builtin_fmaxf(m, ek::reduce_xor<ek::Max, 8>(top));
+    if constexpr (CHUNKS == 16) {
+      top = ek::reduce_xor<ek::Max, 4>(top);
+      top = ek::reduce_xor<ek::Max, 8>(top);
+    }
+    top = __builtin_fmaxf(m, top);
     const float use = top == -__builtin_inff() ? 0.0f : top;
     const float f = ek::exp2_fast((m - use) * scale), w = ek::exp2_fast((mi - use) * scale);
     float sum = ek::reduce_xor<ek::Sum, 1>(li * w);
     sum = ek::reduce_xor<ek::Sum, 2>(sum);
-    sum = ek::reduce_xor<ek::Sum, 4>(sum);
-    sum = ek::reduce_xor<ek::Sum, 8>(sum);
+    if constexpr (CHUNKS == 16) {
+      sum = ek::reduce_xor<ek::Sum, 4>(sum);
+      sum = ek::reduce_xor<ek::Sum, 8>(sum);
+    }
     l = __builtin_fmaf(l, f, sum);
     m = top;
 #pragma unroll
-    for (int k = 0; k < DW; ++k) x[k][0] *= f, x[k][1] *= f;
+    for (int h = 0; h < H; ++h) {
+      const float less = lane_value(f, h * CHUNKS);
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j)
-      if (j < count) {
-        const float y = ek::bits_f32((u32)__builtin_amdgcn_readlane((int)ek::f32_bits(w), j));
+      for (int k = 0; k < DW; ++k) x[h][k][0] *= less, x[h][k][1] *= less;
 #pragma unroll
-        for (int k = 0; k < DW; ++k) {
-          x[k][0] = __builtin_fmaf(v[j][k][0], y, x[k][0]);
-          x[k][1] = __builtin_fmaf(v[j][k][1], y, x[k][1]);
+      for (int j = 0; j < CHUNKS; ++j)
+        if (j < count) {
+          const float y = lane_value(w, h * CHUNKS + j);
+#pragma unroll
+          for (int k = 0; k < DW; ++k) {
+            x[h][k][0] = __builtin_fmaf(v[h][j][k][0], y, x[h][k][0]);
+            x[h][k][1] = __builtin_fmaf(v[h][j][k][1], y, x[h][k][1]);
+          }
         }
-      }
-  }
-  if (waves > 1) {
-    // a part whose m is -inf has no weight, whatever wave it is
-#pragma unroll
-    for (int k = 0; k < DW; ++k) {
-      const int d = k * 128 + lane * 2;
-      if (d < DP) s_o[wave][d] = x[k][0], s_o[wave][d + 1] = x[k][1];
     }
-    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float mo = s_m[w], top = __builtin_fmaxf(m, mo);
-      const float use = top == -__builtin_inff() ? 0.0f : top;
-      const float f = ek::exp2_fast((m - use) * scale), fo = ek::exp2_fast((mo - use) * scale);
-      l = l * f + s_l[w] * fo;
-      m = top;
+  }
+  if constexpr (H == 1) {
+    if (waves > 1) {
+      // a part whose m is -inf has no weight, whatever wave it is
 #pragma unroll
       for (int k = 0; k < DW; ++k) {
         const int d = k * 128 + lane * 2;
-        if (d < DP) {
-          x[k][0] = x[k][0] * f + s_o[w][d] * fo;
-          x[k][1] = x[k][1] * f + s_o[w][d + 1] * fo;
+        if (d < DP) s_o[first][d] = x[0][k][0], s_o[first][d + 1] = x[0][k][1];
+      }
+      if (lane == 0) s_m[first] = m, s_l[first] = l;
+      __syncthreads();
+      if (first != 0) return;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float mo = s_m[w], top = __builtin_fmaxf(m, mo);
+        const float use = top == -__builtin_inff() ? 0.0f : top;
+        const float f = ek::exp2_fast((m - use) * scale), fo = ek::exp2_fast((mo - use) * scale);
+        l = l * f + s_l[w] * fo;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < DW; ++k) {
+          const int d = k * 128 + lane * 2;
+          if (d < DP) {
+            x[0][k][0] = x[0][k][0] * f + s_o[w][d] * fo;
+            x[0][k][1] = x[0][k][1] * f + s_o[w][d + 1] * fo;
+          }
         }
       }
     }
   }
   const bool any = l > 0.0f || l != l;
   const float f = any ? a.v_scale / l : 0.0f;
-  T* dst = a.out + token * a.out_row + head * a.out_head;
 #pragma unroll
-  for (int k = 0; k < DW; ++k) {
-    const int d = k * 128 + lane * 2;
-    if (d < a.dim) {
-      T y[2] = {result(x[k][0], f, any), result(x[k][1], f, any)};
-      ek::vstore_u<T, 2>(dst + d, y);
+  for (int h = 0; h < H; ++h) {
+    if (head0 + h >= a.heads) break;
+    T* dst = a.out + token * a.out_row + (head0 + h) * a.out_head;
+    const float fh = lane_value(f, h * CHUNKS);
+    const bool some = lane_value(any ? 1.0f : 0.0f, h * CHUNKS) != 0.0f;
+#pragma unroll
+    for (int k = 0; k < DW; ++k) {
+      const int d = k * 128 + lane * 2;
+      if (d < a.dim) {
+        T y[2] = {result(x[h][k][0], fh, some), result(x[h][k][1], fh, some)};
+        ek::vstore_u<T, 2>(dst + d, y);
+      }
     }
   }
-  if (a.lse && lane == 0)
-    a.lse[(int64_t)token * a.heads + head] =
+  if (a.lse && lane < H * CHUNKS && i == 0 && mine < a.heads)
+    a.lse[(int64_t)token * a.heads + mine] =
         any ? (m * scale + (__builtin_log2f(l) - LIFT)) * LN2 : -__builtin_inff();
+}
+
+extern "C" __global__ __launch_bounds__(256) void ek_tree_attention_join(Params a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x;
+  const int at = blockIdx.y * 4 + wave;
+  if (a.join == 4) join_heads<4>(a, token, at * 4, 0, 1);
+  else if (a.join == 1) join_heads<1>(a, token, at, 0, 1);
+  else join_heads<1>(a, token, blockIdx.y, wave, 4);
 }

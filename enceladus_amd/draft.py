@@ -219,10 +219,11 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
     if most > 1 and not (batch == 1 and blocks >= items):
         slots = 2 * items
         workspace = slots * kv_heads * cols * (dim + 2) * 4 + 16 * tokens
-        # several waves where a token's head may have many chunks
-        join = 4 if min(items // blocks, most) > 16 else 1
-        launches.append(("ek_tree_attention_join", (tokens, heads if join > 1 else -(-heads // 4)),
-                         256))
+        # four waves for a token's head where it may have many chunks, one for four heads where it
+        # will hardly have more than four
+        join = 0 if min(items // blocks, most) > 16 else 4 if rounds * items <= 4 * blocks else 1
+        launches.append(("ek_tree_attention_join",
+                         (tokens, heads if join == 0 else -(-heads // (4 * join))), 256))
     log2e = 1.4426950408889634
     tail = _ATTEND.pack(
         qa.strides[0], qa.strides[1], oa.strides[0], oa.strides[1],

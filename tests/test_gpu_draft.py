@@ -207,6 +207,20 @@ def test_attention_of_many_sequences(batch):
           trees(gen, new, 1))
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 200), (F32, 96)])
+@pytest.mark.parametrize("batch,kv_heads,group", [(24, 50, 3), (40, 51, 1), (70, 33, 2)])
+def test_attention_of_more_sequences_than_fit_at_once(batch, kv_heads, group, dtype, dim):
+    """Few workgroups for each key head: sequences are split for two rounds of them, and the parts
+    joined by waves of four heads, whose last one has fewer."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 1500, (batch,), generator=gen).tolist()
+    new = [min(n, 1 + i % 4) for i, n in enumerate(lens)]
+    bt, count = table_for(gen, lens, 32)
+    kc, vc = (only_live(cache(gen, count, 32, kv_heads, dim, dtype), bt, lens, 32) for _ in "kv")
+    check(rand(gen, sum(new), kv_heads * group, dim, dtype=dtype), kc, vc, bt, lens,
+          starts_of(new), trees(gen, new, 1))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("group", [1, 4, 7])
 def test_attention_of_prompts(dtype, group):
