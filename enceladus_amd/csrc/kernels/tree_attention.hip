@@ -185,8 +185,16 @@ EK_INLINE int blocks_of(const Params& a, const Seq& s) {
 }
 EK_INLINE int units_of(const Seq& s) { return (s.end - s.first + UNIT - 1) / UNIT; }
 // A sequence without keys has a chunk as well: its rows become zeros.
+// There are few enough of them for a division that is off by one at most before it is put right.
 EK_INLINE int chunks_of(int units, int per) {
-  return units == 0 ? 1 : (int)((u32)(units + per - 1) / (u32)per);
+  int n = (int)((float)(units + per - 1) * __builtin_amdgcn_rcpf((float)per));
+  n += n * per < units;
+  n -= (n - 1) * per >= units;
+  return units == 0 ? 1 : n;
+}
+
+EK_INLINE int even_share(int total, int items) {
+  return total <= items ? 1 : (int)((u32)(total + items - 1) / (u32)items);
 }
 
 struct Item {
@@ -208,31 +216,33 @@ EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
     total += blocks_of(a, s) * units_of(s);
   }
   total = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(total));
-  int per = (int)((u32)(total + a.items - 1) / (u32)a.items);
-  per = per < 1 ? 1 : per;
+  int per = even_share(total, a.items);
   // Each sequence may have a chunk more than its share for each of its blocks, and a few workgroups
   // beyond `items` make a round of their own. So the chunks are made as long as it takes for all of
   // them to fit into one round, or two where the grid has them, whichever ends first if a chunk
-  // costs 3 units besides its own (24 sequences of up to 16384 8-bit keys: 78 us, 82 in even
-  // shares; 64 of up to 8192: 194 us in even shares, 178 in two rounds). Chunks of less than 8
-  // units are not worth two rounds (55 sequences of at most 189 keys: 67 us without, 74 with).
+  // costs 3 units besides its own (24 sequences of up to 16384 8-bit keys: 5% less time than with
+  // even shares; 64 of up to 8192 in two rounds: 8% less). Chunks of less than 8 units are not
+  // worth two rounds (55 sequences of at most 189 keys: 10% more).
   if (a.batch <= 64) {
-    int best = 1 << 30;
+    int best = (per + 3) + (per + 3 >> 1);            // of even shares, with a short round more
+    const int all_blocks = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(blocks_of(a, s0)));
 #pragma unroll 1
     for (int rounds = 1; rounds <= a.rounds; ++rounds) {
+      // the even share, and what leaves room for a chunk more of every block but one
       const int room = rounds * a.items;
-      int try_per = (int)((u32)(total + room - 1) / (u32)room);
-      if (rounds > 1 && try_per < 8) break;
-      try_per = try_per < 1 ? 1 : try_per;
+      int lo = even_share(total, room);
+      if (room < all_blocks || rounds > 1 && lo < 8) continue;
+      int hi = even_share(total, room - all_blocks + 1);
 #pragma unroll 1
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 5 && lo < hi; ++k) {
+        const int middle = lo + hi >> 1;
         const int all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(
-            blocks_of(a, s0) * chunks_of(units_of(s0), try_per)));
-        const int cost = rounds * (try_per + 3);
-        if (cost >= best) break;
-        if (all <= room) { best = cost, per = try_per; break; }
-        try_per += (try_per + 15) >> 4;
+            blocks_of(a, s0) * chunks_of(units_of(s0), middle)));
+        if (all <= room) hi = middle;
+        else lo = middle + 1;
       }
+      const int cost = rounds * (hi + 3);
+      if (cost < best) best = cost, per = hi;
     }
   }
   // without room for parts each has one chunk, as when rows enough for all items are there
@@ -352,6 +362,21 @@ EK_INLINE bool odd_word(u32 w) {
   return ((w & X) + ONE & 0x80008000u) != 0;
 #endif
 }
+// What has been seen of some words' values, in x, and another word: the larger magnitudes, or
+// (e4m3) the carry out of the one magnitude that is not finite.
+EK_INLINE u32 with_word(u32 x, u32 y) {
+#if EK_FP8
+  return x | (y & 0x7F7F7F7Fu) + 0x01010101u;
+#elif EK_Q == 0
+  y &= 0x7FFFFFFFu;
+  return x > y ? x : y;
+#else
+  typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32, __builtin_elementwise_max(
+      __builtin_bit_cast(h2, x), __builtin_bit_cast(h2, y & 0x7FFF7FFFu)));
+#endif
+}
+EK_INLINE bool any_odd(u32 seen) { return EK_FP8 ? (seen & 0x80808080u) != 0 : odd_word(seen); }
 // A word with 0 for each value that is not finite.
 EK_INLINE u32 finite_of(u32 w) {
   constexpr int BITS = CS * 8;
@@ -769,14 +794,15 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     // A value that is not finite must not reach the columns that don't see its key, whose weight
     // is 0: it becomes 0, and what sees it NaN behind the loop.
     if (masks) {
-      bool bad = false;
+      u32 seen = 0;
       char* at = s_stage + stage * STAGE + PART + (lane & (KT - 1)) * ROW;
 #pragma unroll 4
       for (int i = 0; i < CPR; ++i) {
         const words<4> v = lds_words<4>(at + (i ^ k_swap(lane)) * 16);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) bad |= odd_word(v.w[w]);
+        for (int w = 0; w < 4; ++w) seen = with_word(seen, v.w[w]);
       }
+      const bool bad = any_odd(seen);
       if (__builtin_amdgcn_ballot_w64(bad) != 0) {    // all waves see the same
         some_odd = true;
         __syncthreads();
@@ -1058,8 +1084,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #undef valid
 #undef tree_of
 
-// Joins the chunks of H heads of a token in a wave, CHUNKS of each at once: lanes H' CHUNKS + i have
-// head H' and chunk i, and all of their loads are on their way together. With `join` 1 or 4, H is
+// Joins the chunks of H heads of a token in a wave, CHUNKS of each at once: lane h CHUNKS + i has
+// head h and chunk i, and all of their loads are on their way together. With `join` 1 or 4, H is
 // as much: 4 where chunks are few, since a wave takes as long for one head as for four (64
 // sequences of 27 tokens and less, 32 heads, 2 or 3 chunks: 20 us with 1, 12 with 4). Where
 // chunks are many (`join` 0), a workgroup's four waves take one head's in turn and meet in the LDS.
