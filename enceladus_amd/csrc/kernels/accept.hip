@@ -6,8 +6,8 @@
 // was, two instructions per logit; only the row's best vector is looked into, by the second kernel
 // (every lane's own, in the first, read them twice as far as memory goes: 1381 rows of 128000 bf16,
 // 354 MB, 151 us a call instead of 62). Whole numbers alone leave it: the order of a row's
-// stretches does not matter. Of the 354 MB the first kernel takes 57.7 us, 6.1 TB/s, and the walks 6;
-// of 16 rows of 32000, 2.8 and 4.4 us, a launch and a chain of loads each.
+// stretches does not matter. Of the 354 MB the first kernel takes 57.7 us, 6.1 TB/s, and the walks
+// 6; of 16 rows of 32000, 2.8 and 4.4 us, a launch and a chain of loads each.
 //
 // Macros: EK_Q (logits: 0 fp32, 1 fp16, 2 bf16).
 #include "enceladus_cdna4.h"

@@ -12,14 +12,14 @@
 // meet in one lane, so that queries can be rotated in place.
 // Measured: 21152 tokens of 32 query, 8 key and 8 value heads of 128 in bf16, 531 MB: 90 us, 5.9
 // TB/s (the framework's own copies: 6.4). One token of such heads: 3.2 us, a launch and a chain of
-// loads. The same 531 MB by positions of three axes: 91.6 us, the pairs' rows of angles being read
-// for each; 378 drafted tokens by positions of their own 5.5 us.
+// loads. The same 531 MB by positions of three axes: 91.6 us, each pair's
+// row of angles being its own; 378 drafted tokens by positions of their own 5.5 us.
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
 // vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS,
 // EK_STREAM (the rows are more than the caches keep: loaded and stored past them), EK_AXES (0:
-// tokens turn by their slots' positions; else by positions of their own, up to four of them, of which
-// each pair has one: 1 where the pairs of a vector have the same, 2 where they may differ).
+// tokens turn by their slots' positions; else by positions of their own, up to four of them, of
+// which each pair has one: 1 where the pairs of a vector have the same, 2 where they may differ).
 #include "enceladus_cdna4.h"
 #ifndef EK_AXES
 #define EK_AXES 0

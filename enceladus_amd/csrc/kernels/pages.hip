@@ -6,8 +6,8 @@
 // and cost a launch and a chain of dependent loads (counts, ids, pages) when they are small. Every
 // layer's caches have the same pages, so one launch takes them all: their addresses are kernel
 // arguments. 1258 MB of whole pages copied: 197 us, 6.4 TB/s; 192 forks, 206 MB: 5 us for the plan
-// and 36 for the copies; 8 tokens each of 128 sequences moved together in 32 caches, 22 MB: 8 us;
-// 256 sequences take pages: 5 us, and give them back: 3.
+// and 36 for the copies; what is kept of 64 sequences' up to 27 drafted tokens moved together in 32
+// caches, 22 MB: 8 us; 256 sequences take pages: 5 us, and give them back: 3.
 //
 // Macros: EK_CACHES (addresses in the argument block), EK_V (bytes of an access: the largest power
 // of two up to 16 that divides a head), EK_STREAM (more bytes than the caches keep: past them).
@@ -61,8 +61,8 @@ struct Walk {
 
 constexpr int THREADS = 256;
 // Accesses of a thread: whole pages are copied best by small pieces (1258 MB: 197 us with 1, 228
-// with 2, 238 with 4, 243 with 8), parts of them by few (192 forks of 7 tokens in 32 caches, 206 MB:
-// 34 us with 8, 39 with 4, 60 with 1).
+// with 2, 238 with 4, 243 with 8), parts of them by few (192 forks of 7 tokens in 32 caches, 206
+// MB: 34 us with 8, 39 with 4, 60 with 1).
 constexpr int COPY = 1, FORK = 8;
 
 // `tokens` tokens of page `from` into page `to`: piece `piece` of them, in one cache.

@@ -224,18 +224,18 @@ EK_INLINE Item find_item(const Params& a, int item, Seq& found) {
   // even shares; 64 of up to 8192 in two rounds: 8% less). Chunks of less than 8 units are not
   // worth two rounds (55 sequences of at most 189 keys: 10% more).
   if (a.batch <= 64) {
-    int best = (per + 3) + (per + 3 >> 1);            // of even shares, with a short round more
+    int best = (per + 3) + ((per + 3) >> 1);          // of even shares, with a short round more
     const int all_blocks = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(blocks_of(a, s0)));
 #pragma unroll 1
     for (int rounds = 1; rounds <= a.rounds; ++rounds) {
       // the even share, and what leaves room for a chunk more of every block but one
       const int room = rounds * a.items;
       int lo = even_share(total, room);
-      if (room < all_blocks || rounds > 1 && lo < 8) continue;
+      if (room < all_blocks || (rounds > 1 && lo < 8)) continue;
       int hi = even_share(total, room - all_blocks + 1);
 #pragma unroll 1
       for (int k = 0; k < 5 && lo < hi; ++k) {
-        const int middle = lo + hi >> 1;
+        const int middle = (lo + hi) >> 1;
         const int all = __builtin_amdgcn_readfirstlane(wave_all<ek::Sum>(
             blocks_of(a, s0) * chunks_of(units_of(s0), middle)));
         if (all <= room) hi = middle;

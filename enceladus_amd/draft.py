@@ -1,4 +1,5 @@
-"""The operators that check drafted tokens over a paged key-value cache, as hand-written HIP kernels.
+"""The operators that check drafted tokens over a paged key-value cache, as hand-written HIP
+kernels.
 
     q = decode.append_kv(k, v, k_cache, v_cache, block_table, seq_lens, cu_tokens=cu, q=q,
                          cos=cos, sin=sin, positions=positions)
@@ -124,7 +125,17 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
 def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, int, int]:
     """(keys of a stage, columns of a tile, tiles of a wave, waves over columns, waves over keys,
     workgroups of a CU) for sequences of so many columns of a key head, in heads of `width` cached
-    elements of `size` bytes."""
+    elements of `size` bytes.
+
+    Stages of 16 KB each of keys and values leave the LDS to two workgroups. As many columns as there
+    are, in fewer waves and tiles, or else the keys are read again: 8 sequences of up to 16384, 8
+    key heads of 128 in bf16, in tiles of 16 by 1 wave, of 16 by 2, of 32 by 2 and of 32 by 4: 11.5
+    columns 30.8, 31.5, 33.7, 38.4 us; 27 columns 47.0, 32.4, 34.3, 40.0; 52 columns 74.7, 47.8,
+    37.9, 43.0; 111.5 columns 147, 78.2, 53.7, 47.2. Heads of 64 in e4m3 cannot be read in tiles of
+    32: two of 16 (111.5 columns 38.3 us, 47.4 in single ones by 2). Heads of 256 and fp32 have no
+    registers for either: 52 columns by 4 waves 50.9 and 80.6 us, by 2 73.6 and 99.7; 11.5 columns
+    45.0 and 76.6, 43.0 and 54.9.
+    """
     keys = max(16, min(64, 16384 // (width * size)))
     if size == 4 or width == 256:
         over = 1
@@ -132,8 +143,8 @@ def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, i
             over *= 2
         return keys, 16, 1, over, 4 // over, 1 if width * size == 1024 else 2
     if columns <= 32:
-        # 94 to 113 registers at 64 elements; 129 to 152 at 128, of which only the 8-bit ones' stages
-        # leave the LDS to a third workgroup
+        # 94 to 113 registers at 64 elements; 129 to 152 at 128, of which only the 8-bit ones'
+        # stages leave the LDS to a third workgroup
         at_once = 4 if width == 64 else 3 if size == 1 else 2
         return (keys, 16, 1, 1, 4, at_once) if columns <= 16 else (keys, 16, 1, 2, 2, at_once)
     over = 2 if columns <= 64 else 4

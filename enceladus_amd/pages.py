@@ -93,8 +93,8 @@ def _check_caches(caches: list) -> _d._Array:
 
 
 def _check_apart(plan, at: list) -> None:
-    """Refuses caches that share elements, from their addresses. Whether two do goes by their distance
-    alone, so what was found for one is kept."""
+    """Refuses caches that share elements, from their addresses. Whether two do goes by their
+    distance alone, so what was found for one is kept."""
     span, last = plan.span, None
     at = sorted(at)
     for i, p in enumerate(at):
