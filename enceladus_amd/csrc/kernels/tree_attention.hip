@@ -193,8 +193,12 @@ EK_INLINE int chunks_of(int units, int per) {
   return units == 0 ? 1 : n;
 }
 
+// A chunk of MOST_UNITS has all of any sequence (at most 2^30 tokens), and keeps the sums above in
+// 32 bits.
+constexpr int MOST_UNITS = (1 << 30) / UNIT;
 EK_INLINE int even_share(int total, int items) {
-  return total <= items ? 1 : (int)((u32)(total + items - 1) / (u32)items);
+  const u32 per = total <= items ? 1 : ((u32)total + (u32)items - 1) / (u32)items;
+  return per < MOST_UNITS ? (int)per : MOST_UNITS;
 }
 
 struct Item {

@@ -221,6 +221,20 @@ def test_attention_of_more_sequences_than_fit_at_once(batch, kv_heads, group, dt
           starts_of(new), trees(gen, new, 1))
 
 
+@pytest.mark.parametrize("batch,kv_heads", [(2, 1), (33, 16), (64, 40), (64, 300)])
+def test_attention_of_one_long_among_many(batch, kv_heads):
+    """Even shares, shares of whole rounds and shares of all of a sequence."""
+    gen = torch.Generator().manual_seed(kv_heads)
+    lens = [2000] + torch.randint(0, 70, (batch - 1,), generator=gen).tolist()
+    lens[1::7] = [0] * len(lens[1::7])
+    new = [min(n, 1 + i % 3) for i, n in enumerate(lens)]
+    bt, count = table_for(gen, lens, 16)
+    kc, vc = (only_live(cache(gen, count, 16, kv_heads, 32, F16), bt, lens, 16) for _ in "kv")
+    q = rand(gen, sum(new), kv_heads, 32, dtype=F16)
+    check(q, kc, vc, bt, lens, starts_of(new))
+    check(q, kc, vc, bt, lens, starts_of(new), window=1500)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("group", [1, 4, 7])
 def test_attention_of_prompts(dtype, group):
