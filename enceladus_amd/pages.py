@@ -95,13 +95,8 @@ def _check_caches(caches: list) -> _d._Array:
 def _check_apart(plan, at: list) -> None:
     """Refuses caches that share elements, from their addresses. Whether two do goes by their
     distance alone, so what was found for one is kept."""
-    span, last = plan.span, None
-    at = sorted(at)
-    for i, p in enumerate(at):
-        if last is not None and p - last < span:
-            break
-        last = p
-    else:
+    span, at = plan.span, sorted(at)
+    if min(map(operator.sub, at[1:], at)) >= span:
         return
     for i, p in enumerate(at):
         for q in at[i + 1:]:
@@ -394,7 +389,7 @@ def _fork_plan(caches, refs, block_table, seq_lens, source, target):
         [c] * len(caches), arrays, {0, 1, 2, 6}, 4 * (2 * rows + 3 * n),
         (*strides, bt.strides[0], _step(sl), _step(sa), _step(ta), 0, n, rows, bt.shape[1],
          c.shape[0], c.shape[1], heads, row, len(caches), pieces, 0), v, False,
-        [(i, j) for i in (0, 1, 2) for j in (0, 1, 2, 3, 4) if i != j])
+        [(i, j) for i in (0, 1, 2) for j in range(i + 1, 5)])
 
 
 # -- taking and giving back --------------------------------------------------------------------
@@ -484,7 +479,7 @@ def _rows_plan(refs, block_table, seq_lens, new_lens, page: int, grow: bool):
     most = min(pages, rows * bt.shape[1])
     return _pages_plan([("ek_take_pages", (1, 1), 1024)], [], arrays, {0, 1, 2, 6},
                        4 * (rows + most), numbers,
-                       apart=[(i, j) for i in (0, 1, 2) for j in (0, 1, 2, 3) if i != j])
+                       apart=[(i, j) for i in (0, 1, 2) for j in range(i + 1, 4)])
 
 
 def specializations():
