@@ -62,6 +62,10 @@ def _source(file: str, macros: tuple) -> str:
     return "".join(f"#define {k} {v}\n" for k, v in macros) + text
 
 
+def _is_cached(file: str, macros: tuple) -> bool:
+    return C.is_cached(_source(file, macros), file.removesuffix(".hip"))
+
+
 def _code(file: str, macros: tuple) -> bytes:
     return C.compile_code(_source(file, macros), file.removesuffix(".hip"))
 

@@ -10,6 +10,11 @@ kernels of `enceladus.decode`, `enceladus.draft` and `enceladus.pages`.
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 
 
@@ -89,6 +94,31 @@ def _input_shapes(wl) -> dict:
     raise KeyError(wl.name)
 
 
+def hand_written() -> list:
+    """(source, macros) of the hand-written kernels' listed specializations."""
+    from enceladus_amd import decode, draft, pages
+    return [x for module in (decode, draft, pages) for x in module.specializations()]
+
+
+def _compile_in_processes() -> None:
+    """Fills the code-object cache with the hand-written kernels from several processes: hiprtc
+    compiles one program of a process at a time. What one of them leaves out is compiled later."""
+    from enceladus_amd import decode
+    n = min(8, len(os.sched_getaffinity(0)))
+    missing = [i for i, spec in enumerate(hand_written()) if not decode._is_cached(*spec)]
+    if len(missing) < 2 * n or os.environ.get("ENCELADUS_ALWAYS_COMPILE") == "1":
+        return
+    root = str(Path(__file__).resolve().parent.parent)
+    path = os.pathsep.join([root, *filter(None, [os.environ.get("PYTHONPATH")])])
+    code = ("import sys\nfrom enceladus_amd import decode, kernels_catalog\n"
+            "specs = kernels_catalog.hand_written()\n"
+            "for i in sys.argv[1].split(','):\n    decode._code(*specs[int(i)])\n")
+    workers = [subprocess.Popen([sys.executable, "-c", code, ",".join(map(str, missing[k::n]))],
+                                env={**os.environ, "PYTHONPATH": path}) for k in range(n)]
+    for w in workers:
+        w.wait()
+
+
 def compile_all(verbose: bool = False) -> int:
     """Generates and hiprtc-compiles every listed specialization (hiprtc runs on a thread
     pool: each program is its own hiprtc object, and ctypes releases the GIL)."""
@@ -113,8 +143,9 @@ def compile_all(verbose: bool = False) -> int:
         kern, types, facts, consts, nw, dw = job
         return kern._compile_for(types, facts, consts, nw, dw).ck
 
-    from enceladus_amd import decode, draft, pages
-    hand = [x for module in (decode, draft, pages) for x in module.specializations()]
+    from enceladus_amd import decode
+    hand = hand_written()
+    _compile_in_processes()
 
     def one_hand(spec):
         decode._code(*spec)

@@ -66,19 +66,29 @@ def compile_options(extra=()) -> list[str]:
     return [f"--offload-arch={ARCH}", *BASE_OPTIONS, f"-I{hip.INCLUDE_DIR}", *extra]
 
 
-def compile_code(src: str, name: str, extra=()) -> bytes:
-    """hiprtc-compiles `src` (cached by source hash)."""
+def _code_key(src: str, name: str, opts: list) -> tuple[str, Path]:
+    """What a code object is cached by, and its file."""
     global _HDR
     if _HDR is None:
         _HDR = _header_hash()
-    opts = compile_options(extra)
     key = hashlib.sha256("\0".join([src, name, _HDR, *opts]).encode()).hexdigest()
+    return key, cache_dir() / key[:2] / f"{key}.hsaco"
+
+
+def is_cached(src: str, name: str, extra=()) -> bool:
+    """Whether `compile_code` would find a file for `src`."""
+    return _code_key(src, name, compile_options(extra))[1].exists()
+
+
+def compile_code(src: str, name: str, extra=()) -> bytes:
+    """hiprtc-compiles `src` (cached by source hash)."""
+    opts = compile_options(extra)
+    key, path = _code_key(src, name, opts)
     with _lock:
         hit = _mem_cache.get(key)
     if hit is not None:
         return hit
     always = os.environ.get("ENCELADUS_ALWAYS_COMPILE") == "1"
-    path = cache_dir() / key[:2] / f"{key}.hsaco"
     if not always and path.exists():
         data = path.read_bytes()
         if data[:4] == b"\x7fELF":
