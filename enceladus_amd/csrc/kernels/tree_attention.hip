@@ -23,9 +23,11 @@
 //   own second run, so that P is where S left it. 16-bit values come transposed out of the LDS
 //   (tr_read4: 4 keys of one element); of others lane l reads VE consecutive elements of those keys
 //   from element VE r on, and the m-th product takes element VE r + m of them.
-// - A weight is two terms of the values' 16-bit type, a product each: 2^-17 of it is left out in
-//   bf16 and 2^-22 in fp16 and e4m3 (whose values are exact in fp16). One term would be half a
-//   step of the output's own type off in every weight, as much again as its rounding.
+// - A weight is some terms of the values' 16-bit type, a product each: three in bf16, which hold
+//   it exactly, and two in fp16 and for e4m3 (whose values are exact in fp16), which leave out
+//   2^-22 of it. Two in bf16 would leave out 2^-17: trees of up to 27 tokens in 64 sequences of up
+//   to 8192 take 166 us with two and 181 with three, and 4.1 and 0.3 of 1000 results are not the
+//   nearest to the exact ones.
 // - In the LDS a row's 16-byte chunks are swapped by its key's number, so that no two lanes of a
 //   pass (256 bytes) meet in a bank: chunk x of key k is at x ^ k_swap(k) or x ^ v_swap(k). The
 //   copy does it for nothing: each lane picks the chunk that belongs at its place.
@@ -85,7 +87,7 @@ static_assert(TR || VE * CS >= 4, "values are read in words");
 // capped) and scaled after that: the largest is 1 exactly, however large the scores are. fp16 terms
 // are lifted by 2^14: they keep a weight down to 2^-39 of the largest one.
 constexpr bool HALF = EK_Q == 1 || EK_FP8;          // the weights' terms are fp16
-constexpr int TERMS = 2;
+constexpr int TERMS = HALF ? 2 : 3;
 constexpr float LIFT = HALF ? 14.0f : 0.0f;        // log2, in the exponents: l is lifted too
 
 #define EK_HERE __attribute__((always_inline))      // of a lambda: its captures stay in registers
@@ -334,22 +336,23 @@ template <bool FP16, typename A> EK_INLINE void mma_short(A& acc, const u32* a, 
                                                     ek::pack<ek::s16x4>(b), acc, 0, 0, 0);
 }
 typedef float f2 __attribute__((ext_vector_type(2)));
-// The two terms of two weights. bf16: the first is cut off, the second rounded.
-EK_INLINE void split(float x0, float x1, u32& first, u32& second) {
+// The terms of two weights. bf16 cuts off: three of them are the 24 bits of a weight exactly.
+EK_INLINE void split(float x0, float x1, u32 (&y)[TERMS]) {
   if constexpr (HALF) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 y = __builtin_convertvector((f2{x0, x1}), h2);
-    first = __builtin_bit_cast(u32, y);
-    second = __builtin_bit_cast(
-        u32, __builtin_convertvector((f2{__builtin_fmaf((float)y[0], -1.0f, x0),
-                                         __builtin_fmaf((float)y[1], -1.0f, x1)}), h2));
+    const h2 h = __builtin_convertvector((f2{x0, x1}), h2);
+    y[0] = __builtin_bit_cast(u32, h);
+    y[1] = __builtin_bit_cast(
+        u32, __builtin_convertvector((f2{__builtin_fmaf((float)h[0], -1.0f, x0),
+                                         __builtin_fmaf((float)h[1], -1.0f, x1)}), h2));
   } else {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const u32 u0 = ek::f32_bits(x0), u1 = ek::f32_bits(x1);
-    first = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-    second = __builtin_bit_cast(
-        u32, __builtin_convertvector((f2{x0 - ek::bits_f32(u0 & 0xFFFF0000u),
-                                         x1 - ek::bits_f32(u1 & 0xFFFF0000u)}), b2));
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+      const u32 u0 = ek::f32_bits(x0), u1 = ek::f32_bits(x1);
+      y[k] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+      x0 -= ek::bits_f32(u0 & 0xFFFF0000u);
+      x1 -= ek::bits_f32(u1 & 0xFFFF0000u);
+    }
   }
 }
 #endif
@@ -770,8 +773,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #pragma unroll
         for (int p = 0; p < NP; ++p) o[t][p] *= alpha;
       }
-      // The weights are exp2(scale (s - m)): in one step where scale m has digits to spare next to
-      // 2^-17, which a weight's terms leave out, else the difference first.
+      // The weights are exp2(scale (s - m)): in one step where scale m is off by no more than
+      // 2^-17 (as a 32-bit score of that size is by itself), else the difference first.
       const float top = m_use * scale;
       less[t] = LIFT - top;
       if (__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(top) < 256.0f)) != 0) {
@@ -859,7 +862,10 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
 #pragma unroll
         for (int i = 0; i < 2 * SS; ++i) {
           const int s = k * SS + i / 2, x = i % 2 * 2;
-          split(score(t, s, x), score(t, s, x + 1), w_p[k & 1][t][0][i], w_p[k & 1][t][1][i]);
+          u32 y[TERMS];
+          split(score(t, s, x), score(t, s, x + 1), y);
+#pragma unroll
+          for (int n = 0; n < TERMS; ++n) w_p[k & 1][t][n][i] = y[n];
         }
     };
     const auto products = [&](int k, int p, const auto* w) EK_HERE {

@@ -194,6 +194,41 @@ def test_attention_of_large_scores(scale, dtype):
         close(got[i].cpu(), v[x.argmax(-1)].to(dtype).double(), torch.zeros(2, 64).double())
 
 
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F16), (BF16, BF16), (F16, F8),
+                                          (BF16, F8)])
+@pytest.mark.parametrize("dim", [16, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 12, 30])
+def test_attention_weights_keep_32_bits(dtype, cdtype, dim, new):
+    """Two nearly equal weights w1, w2 of 0.37 to 0.61 whose values are 1 and -1, beside a weight
+    of 1 whose value is 0: the result, (w1 - w2) / (1 + w1 + w2), is about 2^-16, so that it shows
+    the weights' errors of 2^-24 and not its own rounding.
+
+    In units of U = 2^-24: the scores are exact; their product with the scale, and that one's
+    own rounding, put 2 U of up to 0.73 into the exponent, exp2 is off by at most 2 U of the
+    weight: 0.61 (0.73 * 2 + 2) = 2.2 U for each weight, 4.4 U for both. fp16's terms have 14 added
+    to the exponent, which rounds it by 2^-21, 5.6 U of the weight, and add 2^-22 = 4 U of it: 11.7
+    U for both. The two products' sums are below 1, their terms (up to 6) are added with 1 U each
+    or, if the matrix unit cuts off, 2 U: 12 U. All that is divided by 1 + w1 + w2 >= 1.73: 9.5 U,
+    and 16.3 U in fp16. Errors of the divisor count by the result, 2^-16."""
+    gen = torch.Generator().manual_seed(dim + new)
+    batch, group = 8, 4
+    kc, vc = (torch.zeros(1, 64, 1, dim) for _ in "kv")
+    kc[0, 1, 0, 0] = kc[0, 2, 0, 0] = kc[0, 2, 0, 1] = 1.0
+    vc[0, 1], vc[0, 2] = 1.0, -1.0
+    kc, vc = kc.to(cdtype), vc.to(cdtype)
+    q = torch.zeros(batch * new, group, dim)
+    q[..., 0] = -torch.rand(batch * new, group, generator=gen) / 2 - 0.5
+    q[..., 1] = -torch.rand(batch * new, group, generator=gen) * 2.0 ** -14
+    q = q.to(dtype)
+    bt, lens = torch.zeros(batch, 1, dtype=torch.int32), [3 + new] * batch
+    cu, tree = starts_of([new] * batch), torch.zeros(batch * new, 1, dtype=torch.int32)
+    want, _, _, _, _ = R.tree_attention(q, kc, vc, bt, lens, cu, tree, scale=1.0)
+    got = draft.tree_attention(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(), int32(lens).cuda(),
+                               cu.cuda(), tree=tree.cuda(), scale=1.0)
+    units = 16.3 if F16 in (dtype, cdtype) or cdtype is F8 else 9.5
+    close(got, want, half_step(dtype) * want.abs() + units * U, "out")
+
+
 @pytest.mark.parametrize("batch", [1, 63, 64, 65, 200])
 def test_attention_of_many_sequences(batch):
     gen = torch.Generator().manual_seed(batch)
