@@ -162,7 +162,9 @@ EK_INLINE int pages_of(int64_t tokens, int page) { return (int)((tokens + page -
 
 // Sequence b is cut to first[b] tokens (no longer than it is): the pages behind them lose a
 // holder. A count never falls below 0: each of the decrements that the count allows meets a value
-// above 0, in any order, and a further one is taken back.
+// above 0, in any order, and a further one is taken back. So a count that is seen at 0 or below has
+// no decrement left; one that began there is not touched (-2^31 would wrap round under another
+// row's eyes).
 extern "C" __global__ __launch_bounds__(THREADS) void ek_free_pages(Params a) {
   const int b = blockIdx.x, len = a.lens[b * a.lens_step];
   int to = a.first ? a.first[b * a.first_step] : 0;
@@ -172,7 +174,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_free_pages(Params a) {
   const int have = pages_of(len, a.page), end = have < a.width ? have : a.width;
   for (int i = pages_of(to, a.page) + threadIdx.x; i < end; i += THREADS) {
     const int id = a.table[b * a.table_row + i];
-    if ((u32)id < (u32)a.pages && atomicSub(&a.refs[id], 1) <= 0) atomicAdd(&a.refs[id], 1);
+    if ((u32)id < (u32)a.pages && a.refs[id] > 0 && atomicSub(&a.refs[id], 1) <= 0)
+      atomicAdd(&a.refs[id], 1);
   }
   if (threadIdx.x == 0) a.lens[b * a.lens_step] = to;
 }

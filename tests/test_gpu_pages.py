@@ -250,6 +250,17 @@ def test_free_of_a_page_that_many_hold_counts_down_to_zero():
     assert refs.tolist() == [0, 0, 7] and not lens.any()
 
 
+def test_free_of_pages_that_are_never_taken():
+    """Whatever their count below 0 is, and however many rows hold them."""
+    rows = 4000
+    refs = int32([-2 ** 31, -1, rows, -2 ** 31 + 1, 0, -7])
+    table = torch.arange(6, dtype=torch.int32).repeat(rows, 1).cuda()
+    lens = torch.full((rows,), 6 * 16, dtype=torch.int32).cuda()
+    r = refs.cuda()
+    pages.free(r, table, lens, page_size=16)
+    assert r.tolist() == [-2 ** 31, -1, 0, -2 ** 31 + 1, 0, -7] and not lens.any()
+
+
 FORKS = [
     ([0, 1, 2, 0, 0], [4, 5, 6, 7, 8]),
     ([0, 1, 1, 2], [4, 4, 5, 0]),                          # a row twice, a source as a target
