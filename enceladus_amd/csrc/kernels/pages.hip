@@ -362,7 +362,8 @@ extern "C" __global__ __launch_bounds__(WG) void ek_fork_plan(Params a) {
 }
 
 // The served forks: the live part of a page that is not whole goes to the fresh one in every
-// cache; the last workgroups of a fork take its row of the table, the counts and the length.
+// cache; the last workgroups of a fork take its row of the table, the counts and the length. A
+// count below 0 stays: nothing lowers one here, so its sign is the same whoever added before.
 extern "C" __global__ __launch_bounds__(THREADS) void ek_fork_copy(Params a) {
   const int i = blockIdx.x / (u32)a.pieces, piece = blockIdx.x - i * a.pieces;
   if (!a.served[i]) return;
@@ -381,7 +382,7 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_fork_copy(Params a) {
     const int id = old[p];
     const bool own = p == whole && fresh >= 0;
     row[p] = own ? fresh : id;
-    if (!own && (u32)id < (u32)a.pages) atomicAdd(&a.refs[id], 1);
+    if (!own && (u32)id < (u32)a.pages && a.refs[id] >= 0) atomicAdd(&a.refs[id], 1);
   }
   if (piece == 0 && threadIdx.x == 0) a.lens[to * a.lens_step] = len < 0 ? 0 : len;
 }

@@ -12,8 +12,8 @@ values alike (`enceladus.decode` has their form): a list of them, or one array w
 dimension in front. They have one shape, one type and the same strides, and share no element; the
 same pages of all of them move in one launch. `block_table` (int32 `[rows, pages of a sequence]`)
 and `seq_lens` (int32 `[rows]`) are those of `enceladus.decode`. `refs` (int32 `[pages]`) counts
-the sequences that hold each page: 0 is a free page, and one below 0 is never taken. What decides
-is on the device, where lengths and counts are, so nothing waits for them and all of it can be
+the sequences that hold each page: 0 is a free page, and one below 0 is never taken, nor changed
+by any call, whichever rows hold it. What decides is on the device, where lengths and counts are, so nothing waits for them and all of it can be
 captured: the order in which pages are taken is fixed (the lowest free ones, by the rows in their
 order), so that the same calls give the same tables.
 
@@ -332,8 +332,8 @@ def _compact_plan(caches, block_table, starts, keep, counts, seq_lens):
 def fork(caches, refs, block_table, seq_lens, source, target):
     """Lets sequences go on from others: row `target[i]` gets the tokens of row `source[i]`.
 
-    Whole pages are shared (their `refs` count one more); a last page that is not whole is copied
-    to the lowest free one, so that both may append. A target must be an empty row (length 0), no
+    Whole pages are shared (their `refs` count one more; one below 0 stays); a last page that is
+    not whole is copied to the lowest free one, so that both may append. A target must be an empty row (length 0), no
     source itself, and a row is the target of one fork: of several the first counts. A fork with
     another target, with a row outside of the table, or for which no page is left, is not served
     and changes nothing; forks get pages in their order.

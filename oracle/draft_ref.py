@@ -227,7 +227,7 @@ def fork(refs, table, lens, source, target, page):
                 table[b][i], refs[new] = new, 1
             else:
                 table[b][i] = p
-                if 0 <= p < len(refs):
+                if 0 <= p < len(refs) and refs[p] >= 0:
                     refs[p] += 1
         lens[b] = n
     return served, refs, table, lens, copies

@@ -301,6 +301,33 @@ def test_fork_of_a_last_page_that_is_not_in_the_cache():
         assert r.tolist() == [2, 0, 0] and t[1].tolist() == [0, wild] and m.tolist() == [20, 20]
 
 
+def test_fork_leaves_counts_below_zero():
+    """Pages that are never taken stay so, however often rows that hold them are shared, cut and
+    ended: whole ones, and one that is not whole, of which children have copies."""
+    page, rows = 16, 7
+    refs, lens = int32([-1, 1, -2, 0, 0, 0, -2 ** 31, 0]), int32([40, 32, 0, 0, 0, 0, 0])
+    table = torch.full((rows, 4), -1, dtype=torch.int32)
+    table[0, :3], table[1, :2] = int32([0, 1, 2]), int32([6, 0])
+    c = rand(torch.Generator().manual_seed(11), 8, page, 1, 8)
+    plain = refs.tolist(), table.tolist(), lens.tolist()
+    r, t, m, g = refs.cuda(), table.cuda(), lens.cuda(), c.cuda()
+    for source, target in (([0, 1], [2, 3]), ([0, 1, 1], [4, 5, 6])):
+        served = pages.fork([g], r, t, m, int32(source).cuda(), int32(target).cuda())
+        want, *plain, copies = R.fork(*plain, source, target, page)
+        assert (served.tolist(), r.tolist(), t.tolist(), m.tolist()) == (want, *plain)
+        assert want == [1] * len(source)
+        for a, b, rest in copies:
+            c[b, :rest] = c[a, :rest]
+    same([g], [c])
+    new = [40, 64, 40, 32, 40, 32, 64]                     # no more than one page is left
+    served, *plain = R.take(*plain, new, page)
+    assert pages.take(r, t, m, int32(new).cuda(), page_size=page).tolist() == served
+    assert (r.tolist(), t.tolist(), m.tolist()) == tuple(plain)
+    assert not {0, 2, 6} & set(t[1, 2:].tolist() + t[6, 2:].tolist())
+    pages.free(r, t, m, page_size=page)
+    assert r.tolist() == [-1, 0, -2, 0, 0, 0, -2 ** 31, 0] and not m.any()
+
+
 @pytest.mark.parametrize("forks", [1, 1024, 1500, 5000])
 def test_fork_of_many(forks):
     gen = torch.Generator().manual_seed(forks)
