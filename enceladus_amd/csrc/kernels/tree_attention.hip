@@ -3,7 +3,8 @@
 //
 // Sequence b of n cached tokens has the rows [cu[b], cu[b + 1]) of the queries, its last ones: with
 // past = n - rows, new token i is at slot past + i. It sees the slots before `past` and the new
-// tokens j whose bit j its row of `tree` has (a chain: j <= i); of these the last `window`.
+// tokens j whose bit j its row of `tree` has (a chain: j <= i); of these, as far as the table goes,
+// the last `window`.
 // s_j = scale q . k_j, optionally capped to c tanh(s_j / c); out = sum_j softmax(s)_j v_j over what
 // it sees, lse = log sum_j exp(s_j). Nothing seen: out = 0, lse = -inf.
 //
@@ -176,8 +177,9 @@ EK_INLINE Seq seq_of(const Params& a, int b) {
   s.rows = b < a.batch ? end - begin : 0;
   s.past = len - s.rows;
   s.end = len < a.capacity ? len : a.capacity;
-  // the first key that any row may see: a tree's row may have no bit at all
-  const int from = s.past + (a.tree ? 0 : 1) - a.window;
+  // The first key that any row may see: a tree's row may have no bit at all. Where the table ends
+  // before the new tokens, all see the same.
+  const int from = (s.past < s.end ? s.past + (a.tree ? 0 : 1) : s.end) - a.window;
   s.first = a.window > 0 && from > 0 ? (from < s.end ? from : s.end) : 0;
   return s;
 }
@@ -520,17 +522,20 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     }
     from[t] = 0;
     if (a.window > 0) {
-      int seen = index[t] + 1;
-      if (a.tree)
-        seen = tree_count(a, tree_of(t), sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
-      from[t] = sq.past + seen - a.window;
-      deep |= a.tree && seen > a.window;
+      if (a.tree) {
+        const int seen = tree_count(a, tree_of(t), sq.past < 0 ? -sq.past : 0, sq.end - sq.past);
+        from[t] = (sq.past < sq.end ? sq.past : sq.end) + seen - a.window;
+        deep |= seen > a.window;
+      } else {
+        const int stop = sq.past + index[t] + 1;
+        from[t] = (stop < sq.end ? stop : sq.end) - a.window;
+      }
     }
   }
   deep = __builtin_amdgcn_ballot_w64(deep) != 0;
   // Whether a column may not see a key before `next` from `base` on that is there: new ones, and
   // where windows begin (one for all waves: no column's begins behind this).
-  const int from_most = a.window > 0 ? sq.past + sq.rows - a.window : 0;
+  const int from_most = a.window > 0 ? sq.end - a.window : 0;
   const int past = sq.past;
   const auto edge = [past, from_most](int base) EK_HERE {
     return base + KT > past || base < from_most;
@@ -541,7 +546,8 @@ extern "C" __global__ __launch_bounds__(64 * W, EK_OCC) void ek_tree_attention(P
     const int stop = sq.past + (last - 1) / a.group + 1;
     hi = hi < stop ? hi : stop;
     if (a.window > 0) {
-      const int begin = sq.past + block0 / a.group + 1 - a.window;
+      const int first = sq.past + block0 / a.group + 1;
+      const int begin = (first < sq.end ? first : sq.end) - a.window;
       if (begin > lo) lo += (begin - lo) / UNIT * UNIT;
     }
   }

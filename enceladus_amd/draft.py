@@ -65,7 +65,7 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
     Token i of the n new ones of sequence b sees the slots before `seq_lens[b] - n` and, of the new
     tokens j, at slot `seq_lens[b] - n + j`, those whose bit is set in its row of `tree` (without
     `tree`: j <= i). Of what it sees only the last `window`, in the order of their slots, count
-    when that is above 0. For these and query head h: s_j = `scale` * q . k_j, made
+    when that is above 0 (slots on a page outside the cache are counted among them). For these and query head h: s_j = `scale` * q . k_j, made
     `softcap` * tanh(s_j / `softcap`) when that is above 0; the result is the sum of
     softmax(s)_j v_j. Heads are shared as in `decode.paged_attention`. A token that sees nothing,
     or no score above -inf, gives zeros. Tokens on a page outside the cache, beyond the block table

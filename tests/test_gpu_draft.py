@@ -129,6 +129,31 @@ def test_attention_of_rows_that_see_nothing(dtype, window):
     assert (check(q, empty, empty, bt, lens, starts_of(new), tree) == 0).all()
 
 
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F16), (BF16, F8)])
+@pytest.mark.parametrize("window", [0, 1, 4, 20, 31, 700])
+@pytest.mark.parametrize("width", [4, 200])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_lengths_beyond_the_table(dtype, cdtype, window, width, tree):
+    """Tokens behind the table are absent: a window is of the last ones that are in it. Some, all
+    and none of the new ones are."""
+    gen = torch.Generator().manual_seed(window + width)
+    page, group = 8, 4
+    end = width * page
+    lens = [end + 8, end + 1, end, end + 68, 2 ** 31 - 1, end - 12, end + 2, 2 * end]
+    new = [1, 5, 4, 70, 7, 3, 33, 2]
+    bt = torch.randperm(len(lens) * width, generator=gen).to(torch.int32).reshape(-1, width)
+    kc, vc = (cache(gen, bt.numel(), page, 1, 64, cdtype) for _ in "kv")
+    q = rand(gen, sum(new), group, 64, dtype=dtype)
+    mask, cu = trees(gen, new, 3, 0.1) if tree else None, starts_of(new)
+    want, lse, mag, smax, _ = R.tree_attention(q, kc, vc, bt, lens, cu, mask, window=window)
+    got, got_lse = draft.tree_attention(
+        *(x.cuda() for x in (q, kc, vc, bt, int32(lens), cu)),
+        tree=None if mask is None else mask.cuda(), window=window, return_lse=True)
+    close(got, want, attention_tolerance(q, want, mag, smax, end + 8, dtype), "out")
+    close(got_lse, lse, (64 + 16) * U * smax + (end + 64) * U +
+          lse.abs().nan_to_num(0, 0, 0) * 4 * U, "lse")
+
+
 @pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F8)])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("tree,window", [(True, 0), (False, 0), (False, 6), (True, 6)])
