@@ -188,6 +188,65 @@ def test_attention_values_that_are_not_finite_reach_only_what_sees_them(dtype, c
     close(got[~hit.cuda()], want[~hit], tol[~hit])
 
 
+def deep_trees(gen, new, words):
+    """Masks of trees whose nodes follow one of the three before them: paths of hundreds."""
+    rows = []
+    for n in new:
+        masks = []
+        for j in range(n):
+            up = j - 1 - int(torch.randint(0, min(3, j), (1,), generator=gen)) if j else None
+            masks.append(1 << j | (masks[up] if j else 0))
+        rows += [[m >> 32 * w & 0xFFFFFFFF for w in range(words)] for m in masks]
+    t = torch.tensor(rows, dtype=torch.int64)
+    return torch.where(t >= 1 << 31, t - (1 << 32), t).to(torch.int32)
+
+
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (BF16, BF16), (F16, F8)])
+@pytest.mark.parametrize("window", [2, 7, 50, 150, 330])
+@pytest.mark.parametrize("make", [trees, deep_trees])
+def test_attention_windows_of_masks_of_many_words(dtype, cdtype, window, make):
+    """Windows that end among the new tokens, before them, and at the borders of a mask's words;
+    lengths with and without a past, and beyond the table; masks that end before the tokens do."""
+    gen = torch.Generator().manual_seed(window)
+    lens, new = [350, 130, 95, 420], [300, 130, 96, 97]
+    bt, count = table_for(gen, lens, 16)
+    bt = bt[:, :25]                                        # 400 tokens
+    kc, vc = (only_live(cache(gen, count, 16, 1, 64, cdtype), bt, lens, 16) for _ in "kv")
+    q = rand(gen, sum(new), 2, 64, dtype=dtype)
+    tree = make(gen, new, 10)
+    check(q, kc, vc, bt, lens, starts_of(new), tree, window=window)
+    check(q, kc, vc, bt, lens, starts_of(new), tree[:, :3].contiguous(), window=window)
+
+
+@pytest.mark.parametrize("dtype,cdtype", [(F32, F32), (BF16, BF16), (F16, F8)])
+@pytest.mark.parametrize("window", [0, 5, 64, 200])
+@pytest.mark.parametrize("make", [trees, deep_trees])
+def test_attention_values_not_finite_under_masks_of_many_words(dtype, cdtype, window, make):
+    gen = torch.Generator().manual_seed(window + 1)
+    lens, new, dim = [320, 150], [230, 150], 64
+    bt, count = table_for(gen, lens, 16)
+    kc, vc = (cache(gen, count, 16, 1, dim, cdtype) for _ in "kv")
+    mask, cu = make(gen, new, 8), starts_of(new)
+    q = rand(gen, sum(new), 2, dim, dtype=dtype)
+    want, _, mag, smax, _ = R.tree_attention(q, kc, vc, bt, lens, cu, mask, window=window)
+    hit = torch.zeros(want.shape, dtype=torch.bool)
+    bad = vc.float()
+    for b, j, d in ((0, -40, 3), (0, 64, 7), (0, 95, 8), (0, 170, 63), (0, 229, 31), (1, 0, 1),
+                    (1, 63, 40), (1, 128, 5)):
+        at = lens[b] - new[b] + j
+        bad[int(bt[b, at // 16]), at % 16, 0, d] = math.nan
+        for i in range(new[b]):
+            row = int(cu[b]) + i
+            line = [1] * (lens[b] - new[b]) + R.seen_by(mask, row, i, new[b]).int().tolist()
+            if line[at] and (not window or sum(line[at:]) <= window):
+                hit[row, :, d] = True
+    got = draft.tree_attention(*(x.cuda() for x in (q, kc, bad.to(cdtype), bt, int32(lens), cu)),
+                               tree=mask.cuda(), window=window)
+    assert hit.any() and torch.isnan(got[hit.cuda()]).all()
+    tol = attention_tolerance(q, want, mag, smax, 330, dtype)
+    close(got[~hit.cuda()], want[~hit], tol[~hit])
+
+
 def test_attention_keys_that_are_not_finite():
     """In masked places they count for nothing; elsewhere the token that sees them is NaN."""
     gen = torch.Generator().manual_seed(4)
