@@ -111,8 +111,12 @@ extern "C" __global__ __launch_bounds__(64) void ek_compact(Params a) {
   const int start = a.first[b * a.first_step];
   count = count < 0 ? 0 : count > a.most ? a.most : count;
   const int64_t capacity = (int64_t)a.width * a.page;
-  if (start < 0 || start >= capacity) return;
-  if (a.lens && part == 0 && blockIdx.y == 0 && lane == 0) a.lens[b * a.lens_step] = start + count;
+  if (start < 0) return;
+  if (a.lens && part == 0 && blockIdx.y == 0 && lane == 0) {
+    const int64_t len = (int64_t)start + count;
+    a.lens[b * a.lens_step] = len < 0x7FFFFFFF ? (int)len : 0x7FFFFFFF;
+  }
+  if (start >= capacity) return;                   // nothing is there to move
   const u32 per = (u32)(a.row_bytes / V), chunk = (u32)part * 64 + lane;
   const bool mine = chunk < per * (u32)a.heads;
   const u32 h = mine ? chunk / per : 0;

@@ -284,8 +284,8 @@ def compact(caches, block_table, starts, keep, counts, *, seq_lens=None) -> None
         starts: int32 `[rows]`; rows with a negative one are left as they are.
         keep: int32 `[rows, most]`.
         counts: int32 `[rows]`; at most `most` count.
-        seq_lens: int32 `[rows]`, which becomes `starts[b] + counts[b]`; without it nothing is
-            written but the caches.
+        seq_lens: int32 `[rows]`, which becomes `starts[b] + counts[b]` (at most 2^31 - 1), also
+            where that is beyond the block table; without it nothing is written but the caches.
     """
     try:
         key = (4, *_key(caches), _d._of(block_table), _d._of(starts), _d._of(keep),

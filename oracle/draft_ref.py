@@ -240,8 +240,8 @@ def compact(cache, table, starts, keep, counts):
     for b, (start, count) in enumerate(zip(starts, counts)):
         count = min(max(count, 0), len(keep[b]))
         capacity = len(table[b]) * page
+        lens.append(None if start < 0 else min(start + count, 2 ** 31 - 1))
         if not 0 <= start < capacity:
-            lens.append(None)
             continue
         for i in range(count):
             old, new = start + keep[b][i], start + i
@@ -250,5 +250,4 @@ def compact(cache, table, starts, keep, counts):
             p, q = table[b][old // page], table[b][new // page]
             if 0 <= p < pages and 0 <= q < pages:
                 out[q, new % page] = cache[p, old % page]
-        lens.append(start + count)
     return out, lens

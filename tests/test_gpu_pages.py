@@ -144,6 +144,22 @@ def test_compact(dtype, dim, kv, page, layout, count):
     same(again, want)
 
 
+@pytest.mark.parametrize("width", [0, 4])
+def test_compact_of_full_rows(width):
+    """A sequence that fills its table has no token to move; its length is that of what was kept."""
+    c = rand(torch.Generator().manual_seed(12), 4, 8, 1, 16)
+    end = 8 * width
+    starts = [end, end + 1, end + 100, 2 ** 31 - 2, 2 ** 31 - 1, -1, end]
+    counts = [3, 1, 0, 1, 2, 2, -4]
+    table = torch.arange(width, dtype=torch.int32).repeat(7, 1)
+    keep, lens = int32([[1, 2, 4]]).repeat(7, 1), torch.full((7,), end + 5, dtype=torch.int32)
+    g, m = c.cuda(), lens.cuda()
+    pages.compact([g], table.cuda(), int32(starts).cuda(), keep.cuda(), int32(counts).cuda(),
+                  seq_lens=m)
+    same([g], [c])
+    assert m.tolist() == [end + 3, end + 2, end + 100, 2 ** 31 - 1, 2 ** 31 - 1, end + 5, end]
+
+
 @pytest.mark.parametrize("n,share", [(70, 0.9), (1000, 0.5), (5000, 0.03), (3001, 0.99)])
 @pytest.mark.parametrize("page", [1, 16, 100])
 def test_compact_long_histories(n, share, page):
