@@ -7,6 +7,9 @@ kernels.
     path, count, token = draft.accept(logits, tokens, cu, tree=tree)
     pages.compact(caches, block_table, past, path, count, seq_lens=seq_lens)
 
+(`pages.take` gives the slots before, and says of which rows the new tokens have none: a length of 0
+here and a negative `past` keep such a row out.)
+
 Each of `batch` sequences has some new tokens in a row: the last one that was chosen, and drafted
 ones that may follow it. Sequence b's are the rows `cu_tokens[b]` to `cu_tokens[b + 1]`, and its
 last ones in the cache. `tree` (int32 `[tokens, words]`) says which of them a token sees: bit j % 32

@@ -2,9 +2,11 @@
 and given back, and the tokens on them compacted, as hand-written HIP kernels.
 
     served = pages.take(refs, block_table, seq_lens, new_lens, page_size=16)
-    pages.compact(caches, block_table, starts, keep, counts, seq_lens=seq_lens)
+    held = seq_lens.clone()
+    pages.compact(caches, block_table, torch.where(served > 0, starts, -1), keep, counts,
+                  seq_lens=seq_lens)
     served = pages.fork(caches, refs, block_table, seq_lens, source, target)
-    pages.free(refs, block_table, seq_lens, new_lens, page_size=16)
+    pages.free(refs, block_table, held, seq_lens, page_size=16)
     pages.copy(caches, source, target)
 
 `caches` are the arrays `[pages, page size, key heads, head dimension]` of all layers, keys and
@@ -402,6 +404,12 @@ def take(refs, block_table, seq_lens, new_lens, *, page_size: int):
     A row that does not grow stays as it is. A row is served if the pages for it and all rows
     before it are there; one that is not, or that the table has no room for (it then takes no
     part), keeps its length and its pages.
+
+    A row that is not served must be kept out of what the pages were for, since with its old length
+    new tokens would be written over its last ones: `seq_lens * served` as the lengths of
+    `decode.append_kv` and `draft.tree_attention` does that (its tokens are skipped and give zeros),
+    and in `compact` a start of -1. What it may give back again to `free` are the lengths after this
+    call, not `new_lens`.
 
     Args:
         refs: int32 `[pages]`, written in place.

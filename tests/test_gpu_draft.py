@@ -805,6 +805,118 @@ def test_drafted_decoding_writes_what_plain_decoding_does(capture):
         assert got == want[:len(got)]
 
 
+def serve_short_of_pages(model, prompts, want, most, gen, capture=False):
+    """Drafted decoding with fewer pages than all sequences need at once: a row that `take` does not
+    serve waits for the next step, and one that has `most` tokens ends, as does the last where none
+    can go on. Returns what was written, how often a row waited, and how many wrote to the end."""
+    batch, page, width, nodes, pool = len(prompts), 8, 12, 7, 19
+    caches = [torch.full((pool, page, model.kv, model.dim), math.nan, device="cuda")
+              for _ in "kv"]
+    refs = torch.zeros(pool, dtype=torch.int32, device="cuda")
+    refs[::7] = -1                                     # not to be taken
+    table = torch.full((batch, width), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    going = torch.ones(batch, dtype=torch.int32, device="cuda")      # 0: the row has ended
+
+    def forward(tokens, cu, tree, positions, live):
+        q, k, v = model.project(tokens)
+        q = decode.append_kv(k, v, *caches, table, live, cu_tokens=cu, q=q, cos=model.cos,
+                             sin=model.sin, positions=positions)
+        return model.logits(draft.tree_attention(q, *caches, table, live, cu, tree=tree))
+
+    new = [len(p) - 1 for p in prompts]
+    served = pages.take(refs, table, lens, int32(new).cuda(), page_size=page)
+    assert served.tolist() == [1] * batch
+    forward(int32([t for p in prompts for t in p[:-1]]).cuda(), starts_of(new).cuda(), None,
+            int32([i for n in new for i in range(n)]).cuda(), lens)
+    tree = int32([[1], [3], [5], [9], [5 + 16], [9 + 32], [5 + 16 + 64]]).cuda()
+    depth = int32([0, 1, 1, 1, 2, 2, 3]).cuda()
+    cu = starts_of([nodes] * batch).cuda()
+    drafted = torch.zeros(batch * nodes, dtype=torch.int32, device="cuda")
+    masks = tree.repeat(batch, 1)
+
+    def step():
+        starts = lens.clone()
+        served = pages.take(refs, table, lens, lens + nodes * going, page_size=page) * going
+        held, live = lens.clone(), lens * served
+        logits = forward(drafted, cu, masks, (starts[:, None] + depth).flatten(), live)
+        path, count, token = draft.accept(logits, drafted, cu, tree=masks, most=4)
+        count = count * served
+        pages.compact(caches, table, torch.where(served > 0, starts, -1), path, count,
+                      seq_lens=lens)
+        pages.free(refs, table, held, lens, page_size=page)
+        return served, path, count, token
+
+    def guesses(s):
+        out = []
+        for b in range(batch):
+            right = want[b][len(texts[b]) - 1:]
+            line = [texts[b][-1]] + torch.randint(0, model.vocab, (6,), generator=gen).tolist()
+            good = [(), (1,), (2,), (2, 4), (2, 4, 6), (3, 5)][(s + b) % 6]
+            for d, j in enumerate(good):
+                if d + 1 < len(right):
+                    line[j] = right[d + 1]
+            out += line
+        return out
+
+    texts, active = [list(p) for p in prompts], list(range(batch))
+    graph = out = None
+    waited = ended = s = 0
+    while active:
+        guess = guesses(s)
+        drafted.copy_(int32(guess))
+        if capture and s == 1:
+            graph = torch.cuda.CUDAGraph()
+            state = [x.clone() for x in (*caches, refs, table, lens)]
+            with torch.cuda.graph(graph):
+                out = step()
+            for x, y in zip((*caches, refs, table, lens), state):
+                x.copy_(y)
+        if graph is not None:
+            graph.replay()
+        else:
+            out = step()
+        served, path, count, token = (x.cpu() for x in out)
+        for b in range(batch):
+            assert (int(count[b]) > 0) == (int(served[b]) > 0) and (b in active or not served[b])
+            if served[b]:
+                texts[b] += [guess[b * nodes + j] for j in path[b, 1:int(count[b])].tolist()]
+                texts[b].append(int(token[b]))
+        waited += sum(1 - int(served[b]) for b in active)
+        assert lens.tolist() == [len(t) - 1 if b in active else 0 for b, t in enumerate(texts)]
+        over = [b for b in active if len(texts[b]) >= most]
+        ended += len(over)
+        if not over and not served.any():
+            over = active[-1:]
+        for b in over:
+            active.remove(b)
+            going[b] = 0
+            pages.free(refs, table, lens, lens * going, page_size=page)
+        # every page is counted as often as rows hold it
+        uses = [-1 if p % 7 == 0 else 0 for p in range(pool)]
+        for b, n in enumerate(lens.tolist()):
+            for p in table[b, :-(-n // page)].tolist():
+                uses[p] += 1
+        assert refs.tolist() == uses
+        s += 1
+    return texts, waited, ended
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_drafted_decoding_short_of_pages(capture):
+    model = Model(5)
+    gen = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, model.vocab, (n,), generator=gen).tolist() for n in (17, 5, 20, 9)]
+    most = 44
+    plain = [model.plain(p, most + 8 - len(p)) for p in prompts]
+    assert min(lead for _, lead in plain) > 1e-3       # no choice that 32 bits could turn
+    texts, waited, ended = serve_short_of_pages(model, prompts, [t for t, _ in plain], most, gen,
+                                                capture)
+    assert waited > 5 and ended > 1
+    for got, (want, _) in zip(texts, plain):
+        assert got == want[:len(got)]
+
+
 def attend_state(seed, lens):
     gen = torch.Generator().manual_seed(seed)
     new = [5, 9, 2]
