@@ -231,7 +231,7 @@ def _attention_plan(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, tree,
     join = 1
     # one sequence of as many blocks as there are items has one chunk
     if most > 1 and not (batch == 1 and blocks >= items):
-        slots = 2 * items
+        slots = min(2 * items, x)      # each is a workgroup's
         workspace = slots * kv_heads * cols * (dim + 2) * 4 + 16 * tokens
         # four waves for a token's head where it may have many chunks, one for four heads where it
         # will hardly have more than four

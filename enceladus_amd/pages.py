@@ -15,9 +15,9 @@ dimension in front. They have one shape, one type and the same strides, and shar
 same pages of all of them move in one launch. `block_table` (int32 `[rows, pages of a sequence]`)
 and `seq_lens` (int32 `[rows]`) are those of `enceladus.decode`. `refs` (int32 `[pages]`) counts
 the sequences that hold each page: 0 is a free page, and one below 0 is never taken, nor changed
-by any call, whichever rows hold it. What decides is on the device, where lengths and counts are, so nothing waits for them and all of it can be
-captured: the order in which pages are taken is fixed (the lowest free ones, by the rows in their
-order), so that the same calls give the same tables.
+by any call, whichever rows hold it. What decides is on the device, where lengths and counts are, so
+nothing waits for them and all of it can be captured: the order in which pages are taken is fixed
+(the lowest free ones, by the rows in their order), so that the same calls give the same tables.
 
 Arrays, streams, captures and errors are as in `enceladus.decode`. Ids outside of the cache or the
 table are neither read nor written through, a negative length counts as none. `seq_lens`, `refs`

@@ -428,6 +428,26 @@ def test_attention_strides_places_and_padding():
     assert torch.equal(q[before:-behind], keep)
 
 
+@pytest.mark.parametrize("length", [500, 1999])
+@pytest.mark.parametrize("batch", [1, 3])
+def test_attention_workspace_goes_by_the_call(length, batch):
+    """No more room for partial results than the sequences have units of 64 tokens."""
+    gen = torch.Generator().manual_seed(length)
+    kv, group, dim, n = 8, 4, 128, 16
+    bt, count = table_for(gen, [length] * batch, 16)
+    kc, vc = (cache(gen, count, 16, kv, dim, BF16).cuda() for _ in "kv")
+    q = rand(gen, batch * n, kv * group, dim, dtype=BF16).cuda()
+    args = [q, kc, vc, bt.cuda(), int32([length] * batch).cuda(), starts_of([n] * batch).cuda()]
+    out = draft.tree_attention(*args)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    draft.tree_attention(*args, out=out)
+    most = batch * -(-length // 64) * kv * n * group * (dim + 2) * 4 + 16 * batch * n
+    blocks = 2 if batch > 1 else 1                         # the host knows the sum of the rows
+    assert torch.cuda.max_memory_allocated() - before <= blocks * most + 1024
+
+
 def test_attention_padded_rows_of_one_long_sequence():
     """Few tokens in rows for many: the split goes by the tokens."""
     gen = torch.Generator().manual_seed(9)
