@@ -12,8 +12,9 @@
 // meet in one lane, so that queries can be rotated in place.
 // Measured: 21152 tokens of 32 query, 8 key and 8 value heads of 128 in bf16, 531 MB: 90 us, 5.9
 // TB/s (the framework's own copies: 6.4). One token of such heads: 3.2 us, a launch and a chain of
-// loads. The same 531 MB by positions of three axes: 91.6 us, each pair's row of angles being its
-// own; 378 drafted tokens by positions of their own: 5.5 us.
+// loads. The same 531 MB by positions of three axes: 92 us, each pair's row of angles being its
+// own; 115 to 120 with the axes woven pair by pair, a load for each pair. 378 drafted tokens by
+// positions of their own: 5.5 us.
 //
 // Macros: EK_Q (new rows: 0 fp32, 1 fp16, 2 bf16), EK_FP8 (e4m3 cache), EK_V (elements of a
 // vector access: a power of two up to 16 bytes that divides the parts of a head), EK_PAIRS,

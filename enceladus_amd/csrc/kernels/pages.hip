@@ -7,7 +7,8 @@
 // layer's caches have the same pages, so one launch takes them all: their addresses are kernel
 // arguments. 1258 MB of whole pages copied: 197 us, 6.4 TB/s; 192 forks, 206 MB: 5 us for the plan
 // and 36 for the copies; what is kept of 64 sequences' up to 27 drafted tokens moved together in 32
-// caches, 22 MB: 8 us; 256 sequences take pages: 5 us, and give them back: 3.
+// caches, 22 MB: 8 us; 256 sequences take pages: 5 us, and give them back: 3. Long histories are
+// compacted far below that rate: see ek_compact.
 //
 // Macros: EK_CACHES (addresses in the argument block), EK_V (bytes of an access: the largest power
 // of two up to 16 that divides a head), EK_STREAM (more bytes than the caches keep: past them).
@@ -98,7 +99,10 @@ extern "C" __global__ __launch_bounds__(THREADS) void ek_copy_pages(Params a) {
 // every cache. The tokens kept ascend, so each moves to the front or stays, and a slot is read
 // before any later token is written to it: a wave takes one part of the heads of a sequence's
 // tokens in one cache through all of them, in their order, and reads BATCH of them before it
-// writes those (what later ones are read from lies behind all that is written before).
+// writes those (what later ones are read from lies behind all that is written before). So few
+// sequences are few waves, each bound by its round trips: of 8192 tokens in 32 caches every second
+// one kept, 537 MB, takes 1930 us; of 8 such sequences, 4.3 GB, 2570 us, 1.7 TB/s; of 64 with 1024
+// tokens, 4.3 GB, 907 us, 4.7 TB/s.
 constexpr int BATCH = 16;
 EK_INLINE int64_t lane_value(int64_t x, int lane) {
   return (int64_t)((uint64_t)(u32)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
@@ -261,8 +265,9 @@ EK_INLINE int need_of(const Params& a, int b, int& have) {
 
 // Sequence b grows to first[b] tokens: rows in their order take the lowest free pages. A row is
 // served if the pages that it and the rows before it need are there. `work`: the ends of the rows'
-// shares [rows], then the pages found [most]. 256 rows, 65536 pages: a chain of loads and barriers,
-// 5.2 us.
+// shares [rows], then the pages found [most]. 256 rows: a chain of loads and barriers, 5.2 us where
+// the first 8192 counts have pages enough, whether a tenth of them are free or all; each further
+// 8192 counts are a round of 0.8 us (65536 pages of which the last tenth is free: 10.7 us).
 extern "C" __global__ __launch_bounds__(WG) void ek_take_pages(Params a) {
   __shared__ u32 s_wave[WG / 64];
   __shared__ int32_t s_ends[SMALL];

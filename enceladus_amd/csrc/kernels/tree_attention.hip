@@ -27,7 +27,7 @@
 // - A weight is some terms of the values' 16-bit type, a product each: three in bf16, which hold
 //   it exactly, and two in fp16 and for e4m3 (whose values are exact in fp16), which leave out
 //   2^-22 of it. Two in bf16 would leave out 2^-17: trees of up to 27 tokens in 64 sequences of up
-//   to 8192 take 166 us with two and 181 with three, and 4.1 and 0.3 of 1000 results are not the
+//   to 8192 take 167 us with two and 187 with three, and 4.1 and 0.3 of 1000 results are not the
 //   nearest to the exact ones.
 // - In the LDS a row's 16-byte chunks are swapped by its key's number, so that no two lanes of a
 //   pass (256 bytes) meet in a bank: chunk x of key k is at x ^ k_swap(k) or x ^ v_swap(k). The
@@ -38,9 +38,11 @@
 // Sequences of one chunk are finished here; the others leave (O, m, l) per chunk and column to the
 // second kernel.
 //
-// 128 columns over 131075 fp16 keys of 8 heads (537 MB, 103 GFLOP of products): 143 us and 11 to
-// join, 3.8 TB/s. The copies alone take 100 us, the rest without them 101 (softmax and products
-// in turn, each about half): one covers the other only in part. Some 25 columns of each of 24
+// 128 columns over 131075 fp16 keys of 8 heads (537 MB, 103 GFLOP of products): 145 to 153 us and
+// 10 to join, 3.3 to 3.5 TB/s. The copies alone take 100 us, the rest without them 101 (softmax and
+// products in turn, each about half): one covers the other only in part. The matrix units are busy
+// 38% of the time, 40% for the bf16 trees above: a stage's softmax has no product beside it, and
+// the barriers keep a workgroup's waves in the same part of a stage. Some 33 columns of each of 24
 // sequences of up to 16384 8-bit keys (156 MB): 78 us. A tree of 16 tokens after 1983 (8.4 MB, one
 // stage for each workgroup): 14 us, of which 6 are the way to the first key (lengths, pages, keys:
 // three reads, each waiting for the one before).

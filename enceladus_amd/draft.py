@@ -68,14 +68,15 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, *, tre
     Token i of the n new ones of sequence b sees the slots before `seq_lens[b] - n` and, of the new
     tokens j, at slot `seq_lens[b] - n + j`, those whose bit is set in its row of `tree` (without
     `tree`: j <= i). Of what it sees only the last `window`, in the order of their slots, count
-    when that is above 0 (slots on a page outside the cache are counted among them). For these and query head h: s_j = `scale` * q . k_j, made
-    `softcap` * tanh(s_j / `softcap`) when that is above 0; the result is the sum of
-    softmax(s)_j v_j. Heads are shared as in `decode.paged_attention`. A token that sees nothing,
-    or no score above -inf, gives zeros. Tokens on a page outside the cache, beyond the block table
-    or before the sequence's first (new ones, where there are more of them than tokens) count as
-    absent. Cache memory that no sequence's length reaches may hold anything, NaN included; a
-    value that is not finite reaches the tokens that see it alone, whose elements it makes infinite
-    or NaN. Rows of no sequence (padding behind the last, or before the first) are skipped: `out`
+    when that is above 0 (slots on a page outside the cache are counted among them). For these and
+    query head h: s_j = `scale` * q . k_j, made `softcap` * tanh(s_j / `softcap`) when that is above
+    0; the result is the sum of softmax(s)_j v_j. Scores, weights and sums have 32 bits; where the
+    cache is float16 or float8, a weight is rounded by up to 2^-20 of it before its product. Heads
+    are shared as in `decode.paged_attention`. A token that sees nothing, or no score above -inf,
+    gives zeros. Tokens on a page outside the cache, beyond the block table or before the sequence's
+    first (new ones, where there are more of them than tokens) count as absent. Cache memory that no
+    sequence's length reaches may hold anything, NaN included; a value that is not finite reaches
+    the tokens that see it alone, whose elements it makes infinite or NaN. Rows of no sequence (padding behind the last, or before the first) are skipped: `out`
     is not written for them (a new one holds anything there).
 
     Args:
@@ -130,14 +131,14 @@ def _shape(columns: float, width: int, size: int) -> tuple[int, int, int, int, i
     workgroups of a CU) for sequences of so many columns of a key head, in heads of `width` cached
     elements of `size` bytes.
 
-    Stages of 16 KB each of keys and values leave the LDS to two workgroups. As many columns as there
-    are, in fewer waves and tiles, or else the keys are read again: 8 sequences of up to 16384, 8
-    key heads of 128 in bf16, in tiles of 16 by 1 wave, of 16 by 2, of 32 by 2 and of 32 by 4: 11.5
-    columns 30.8, 31.5, 33.7, 38.4 us; 27 columns 47.0, 32.4, 34.3, 40.0; 52 columns 74.7, 47.8,
-    37.9, 43.0; 111.5 columns 147, 78.2, 53.7, 47.2. Heads of 64 in e4m3 cannot be read in tiles of
+    Stages of 16 KB each of keys and values leave the LDS to two workgroups. As many columns as
+    there are, in fewer waves and tiles, or else the keys are read again: 8 sequences of up to
+    16384, 8 key heads of 128 in bf16, in tiles of 16 by 1 wave, of 16 by 2, of 32 by 2 and of 32 by 4: 11.5
+    columns 30.7, 31.6, 36.1, 41.6 us; 27 columns 47.3, 32.6, 37.2, 42.9; 52 columns 74.8, 48.0,
+    40.3, 46.3; 111.5 columns 147, 79.0, 58.9, 52.9. Heads of 64 in e4m3 cannot be read in tiles of
     32: two of 16 (111.5 columns 38.3 us, 47.4 in single ones by 2). Heads of 256 and fp32 have no
-    registers for either: 52 columns by 4 waves 50.9 and 80.6 us, by 2 73.6 and 99.7; 11.5 columns
-    45.0 and 76.6, 43.0 and 54.9.
+    registers for either: 52 columns (up to 8192 tokens) by 4 waves 52.3 and 80.3 us, by 2 74.7 and
+    99.2; 11.5 columns 46.1 and 76.3, 43.7 and 54.5.
     """
     keys = max(16, min(64, 16384 // (width * size)))
     if size == 4 or width == 256:

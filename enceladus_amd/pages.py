@@ -335,10 +335,10 @@ def fork(caches, refs, block_table, seq_lens, source, target):
     """Lets sequences go on from others: row `target[i]` gets the tokens of row `source[i]`.
 
     Whole pages are shared (their `refs` count one more; one below 0 stays); a last page that is
-    not whole is copied to the lowest free one, so that both may append. A target must be an empty row (length 0), no
-    source itself, and a row is the target of one fork: of several the first counts. A fork with
-    another target, with a row outside of the table, or for which no page is left, is not served
-    and changes nothing; forks get pages in their order.
+    not whole is copied to the lowest free one, so that both may append. A target must be an empty
+    row (length 0), no source itself, and a row is the target of one fork: of several the first
+    counts. A fork with another target, with a row outside of the table, or for which no page is
+    left, is not served and changes nothing; forks get pages in their order.
 
     Args:
         caches: the caches, written in place.
